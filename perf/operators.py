@@ -1,0 +1,346 @@
+"""Cases of the fine-tuning operators on rows: activations kept in 8 bits for the backward pass, and low-rank adapters beside a
+shared projection.
+
+Four operators, each beside its kind in `jmodt_amd.ops.rows` (dense layers on (rows, channels) activations):
+
+  keep      checkpoint_rows / restore_rows: a row tensor as e4m3 codes with one power-of-two scale per 32 channels of a row, and back
+  wgrad8    linear_wgrad8: dW = dY^T X and db = column sums of dY, with X a kept (8-bit) input
+  adapt     adapter_forward: out[r] = base[r] + s_a B_a (A_a x[r]) with a = the adapter of row r (rows without one: out = base)
+  adapt_bwd adapter_grad: the gradients of that for x, A and B, with x as it is or as it was kept in 8 bits
+
+The format (keep): for a block of 32 channels, amax = the largest finite |x|, the scale 2^e is the smallest power of two with
+amax <= 448 * 2^e, -100 <= e (an empty block: e = -100), kept as the byte e + 127; the code is x / 2^e rounded to the nearest e4m3
+value, ties to even, except that a value that is not zero never becomes zero (it takes the smallest code of its sign, so that a
+ReLU's mask can be read off the codes) and that a value that is not finite becomes NaN.  Every step is exact or a defined rounding.
+
+Where `own` is false the operators are computed by elementary torch operations in 32 bits.
+"""
+import math
+
+import torch
+
+own = False
+
+_T = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+_SIZE = {"f32": 4, "bf16": 2, "f16": 2, "e4m3": 1}
+
+
+def listed():
+    return [
+        # the pooled 512-channel features of 4 frames x 128 RoIs, kept for the RCNN heads' backward: a call where latency counts
+        {"name": "keep_roi_features", "op": "keep", "m": 512, "c": 512, "type": "f32", "relu": True},
+        # the point features of 4 frames x 16384 points behind a feature-propagation layer of 128 channels
+        {"name": "keep_points", "op": "keep", "m": 65536, "c": 128, "type": "f32", "relu": True},
+        # the distinct rows of a set-abstraction level with the 196-wide hidden layer, in bfloat16, before the activation: an odd
+        # count and a width that fills neither its last block of 32 nor its last 16 bytes
+        {"name": "keep_odd_level", "op": "keep", "m": 100003, "c": 196, "type": "bf16", "relu": False},
+
+        # weight gradient of a 512 x 512 RCNN head layer over 4 frames x 128 RoIs
+        {"name": "wgrad_roi_head", "op": "wgrad8", "m": 512, "n": 512, "k": 512, "type": "f32"},
+        # a 256-wide layer over all points of 4 frames
+        {"name": "wgrad_points", "op": "wgrad8", "m": 65536, "n": 256, "k": 256, "type": "f32"},
+        # the widest layer over the points of 8 frames, gradients in bfloat16: the largest product
+        {"name": "wgrad_wide", "op": "wgrad8", "m": 131072, "n": 512, "k": 512, "type": "bf16"},
+        # the 196-wide layer over an odd count of rows with an input of 131 channels (128 features + xyz), gradients in float16
+        {"name": "wgrad_odd", "op": "wgrad8", "m": 30001, "n": 196, "k": 131, "type": "f16"},
+
+        # eight tracked objects, each of another sensor rig, one row each; which adapters meet is new with every call, so the plan
+        # is made within it
+        {"name": "adapt_few_rows", "op": "adapt", "m": 8, "k": 512, "n": 512, "rank": 16, "adapters": 8, "type": "bf16",
+         "order": "mixed", "none": 0.0, "plan": True, "t": False},
+        # 8 frames x 128 RoIs, each frame with the adapter of its rig, two of ten frames without one, a plan that all layers share
+        {"name": "adapt_roi_heads", "op": "adapt", "m": 1024, "k": 512, "n": 512, "rank": 16, "adapters": 6, "type": "f32",
+         "order": "frames", "none": 0.2, "plan": False, "t": False},
+        # training over the points of 4 frames, the low-rank activations kept for the backward
+        {"name": "adapt_points", "op": "adapt", "m": 65536, "k": 256, "n": 256, "rank": 32, "adapters": 4, "type": "bf16",
+         "order": "frames", "none": 0.0, "plan": False, "t": True},
+
+        # the backward over 4 frames x 128 RoIs in float32
+        {"name": "adapt_bwd_roi_heads", "op": "adapt_bwd", "m": 512, "k": 512, "n": 512, "rank": 16, "adapters": 4, "type": "f32",
+         "x": "f32", "order": "frames", "none": 0.0},
+        # the backward over the points of 4 frames from inputs kept in 8 bits
+        {"name": "adapt_bwd_points", "op": "adapt_bwd", "m": 65536, "k": 512, "n": 256, "rank": 16, "adapters": 4, "type": "bf16",
+         "x": "e4m3", "order": "frames", "none": 0.0},
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    """one more case: rows from one to 131072, widths from 1 to 1024, ranks from 1 to 64, every type; an operator's draw costs no
+    more than the largest listed case of that operator"""
+    op = rng.choice(["keep", "wgrad8", "adapt", "adapt_bwd"])
+    limit = max(_cost(c) for c in listed() if c["op"] == op)
+    while True:
+        case = {"op": op, "m": _log(rng, 1, 131072), "type": rng.choice(["f32", "bf16", "f16"])}
+        if op == "keep":
+            case.update(c=_log(rng, 1, 1024), relu=rng.random() < 0.6)
+        elif op == "wgrad8":
+            case.update(n=_log(rng, 4, 1024), k=_log(rng, 4, 1024))
+        else:
+            case.update(k=_log(rng, 4, 1024), n=_log(rng, 4, 1024), rank=_log(rng, 1, 64), adapters=_log(rng, 1, 64),
+                        order=rng.choice(["frames", "mixed"]), none=rng.choice([0.0, 0.1, 0.5]))
+            if op == "adapt":
+                case.update(plan=rng.random() < 0.5, t=rng.random() < 0.5)
+            else:
+                case.update(x=rng.choice([case["type"], "e4m3"]))
+        if _cost(case) <= limit:
+            return case
+
+
+def _cost(case):
+    w = work(case)
+    return w["bytes"] + w["flops"] / 64
+
+
+def work(case):
+    m, s = case["m"], _SIZE[case["type"]]
+    if case["op"] == "keep":
+        c = case["c"]
+        kept = m * c + m * (-(-c // 32))
+        return {"bytes": 2 * m * c * s + 2 * kept, "flops": 4 * m * c}
+    if case["op"] == "wgrad8":
+        n, k = case["n"], case["k"]
+        return {"bytes": m * n * s + m * k + m * (-(-k // 32)) + 4 * n * k + 4 * n, "flops": 2 * m * n * k + m * n}
+    n, k, r = case["n"], case["k"], case["rank"]
+    live = m * (1.0 - case["none"])
+    weights = min(case["adapters"], max(1, m)) * (k + n) * r * s
+    if case["op"] == "adapt":
+        return {"bytes": int(m * k * s + 2 * m * n * s + weights + (4 * m * r if case["t"] else 0) + 4 * m),
+                "flops": int(2 * live * r * (k + n))}
+    x = m * k * _SIZE[case["x"]] + (m * (-(-k // 32)) if case["x"] == "e4m3" else 0)
+    full = case["adapters"] * (k + n) * r * s
+    return {"bytes": int(m * n * s + x + 2 * m * k * s + 4 * m * r + weights + full + 4 * m), "flops": int(4 * live * r * (k + n))}
+
+
+# ------------------------------------------------------------------------------------------------------------------- inputs
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _activations(m, c, relu, g):
+    """channels of different magnitude, rows of different magnitude, half of it zero behind a ReLU"""
+    x = torch.randn(m, c, generator=g, device="cuda")
+    x *= torch.exp(0.7 * torch.randn(c, generator=g, device="cuda"))
+    x *= torch.exp(0.5 * torch.randn(m, 1, generator=g, device="cuda"))
+    return x.clamp_(min=0.0) if relu else x
+
+
+def _gradients(m, n, g):
+    """small, and of very different magnitude from row to row (few points lie on an object)"""
+    return torch.randn(m, n, generator=g, device="cuda") * torch.exp(1.5 * torch.randn(m, 1, generator=g, device="cuda")) * 1e-2
+
+
+def _encode(x):
+    """the kept form of x: (codes as bytes (m, c), scales as bytes (m, blocks of 32))"""
+    x = x.float()
+    m, c = x.shape
+    nb = -(-c // 32)
+    blocks = torch.zeros(m, nb * 32, device=x.device)
+    blocks[:, :c] = x
+    blocks = blocks.view(m, nb, 32)
+    finite = torch.isfinite(blocks)
+    amax = torch.where(finite, blocks.abs(), torch.zeros_like(blocks)).amax(dim=2)
+    mant, expo = torch.frexp(amax)                                 # amax = mant 2^expo, 0.5 <= mant < 1 (amax 0: 0, 0)
+    e = expo - 9 + (mant > 0.875).to(expo.dtype)                   # amax <= 448 2^e = 0.875 2^(e + 9)
+    e = torch.where(amax > 0, e, torch.full_like(e, -100)).clamp(min=-100)
+    v = torch.where(finite, blocks, torch.zeros_like(blocks)) * torch.exp2(-e.float())[:, :, None]
+    codes = v.to(torch.float8_e4m3fn).view(torch.uint8)
+    tiny = ((codes & 0x7F) == 0) & (blocks != 0)
+    codes = torch.where(tiny, torch.where(blocks < 0, 0x81, 0x01).to(torch.uint8), codes)
+    codes = torch.where(finite, codes, torch.full_like(codes, 0x7F))
+    return codes.view(m, nb * 32)[:, :c].contiguous(), (e + 127).to(torch.uint8)
+
+
+def _decode(codes, exps):
+    scale = torch.exp2(exps.float() - 127.0).repeat_interleave(32, dim=1)[:, :codes.shape[1]]
+    return codes.view(torch.float8_e4m3fn).float() * scale
+
+
+def _ids(case, g):
+    """the adapter of every row, -1 for none: whole frames (runs of rows) or any order"""
+    m, count, none = case["m"], case["adapters"], case["none"]
+    if case["order"] == "frames":
+        frames = min(m, max(8, count))
+        order = torch.randperm(frames, generator=g, device="cuda") % count
+        gone = torch.rand(frames, generator=g, device="cuda") < none
+        order = torch.where(gone, torch.full_like(order, -1), order)
+        row = torch.arange(m, device="cuda") * frames // m
+        return order[row].to(torch.int32)
+    ids = torch.randint(0, count, (m,), generator=g, device="cuda")
+    gone = torch.rand(m, generator=g, device="cuda") < none
+    return torch.where(gone, torch.full_like(ids, -1), ids).to(torch.int32)
+
+
+def _inputs(case, seed):
+    g = _gen(seed)
+    op, m, t = case["op"], case["m"], _T[case["type"]]
+    if op == "keep":
+        return {"x": _activations(m, case["c"], case["relu"], g).to(t)}
+    if op == "wgrad8":
+        codes, exps = _encode(_activations(m, case["k"], True, g))
+        return {"dy": _gradients(m, case["n"], g).to(t), "codes": codes, "exps": exps}
+    k, n, r, count = case["k"], case["n"], case["rank"], case["adapters"]
+    s = {"ids": _ids(case, g),
+         "a": (torch.randn(count, r, k, generator=g, device="cuda") / math.sqrt(k)).to(t),
+         "b": (torch.randn(count, n, r, generator=g, device="cuda") * 0.1).to(t),
+         "scales": 0.5 + torch.rand(count, generator=g, device="cuda")}
+    if op == "adapt":
+        s["x"] = _activations(m, k, True, g).to(t)
+        s["base"] = torch.randn(m, n, generator=g, device="cuda").to(t)
+        return s
+    s["dy"] = _gradients(m, n, g).to(t)
+    s["base"] = _gradients(m, k, g).to(t)
+    x = _activations(m, k, True, g).to(t)
+    s["t"] = torch.zeros(m, r, device="cuda")                      # A_a x, as the forward pass kept it
+    for i in range(count):
+        rows = torch.nonzero(s["ids"] == i)[:, 0]
+        s["t"][rows] = x[rows].float() @ s["a"][i].float().t()
+    if case["x"] == "e4m3":
+        s["codes"], s["exps"] = _encode(x)
+    else:
+        s["x"] = x
+    return s
+
+
+def prepare(case, seed):
+    s = _inputs(case, seed)
+    s["case"] = case
+    if own:
+        if "codes" in s:
+            from jmodt_amd.ops.rows8 import Rows8
+            s["kept"] = Rows8.from_codes(s["codes"], s["exps"])    # the kept tensor, as the forward pass left it
+        if "ids" in s and not case.get("plan"):
+            from jmodt_amd.ops.adapters import AdapterPlan
+            s["plan"] = AdapterPlan(s["ids"], case["adapters"])    # one plan for all layers of a step
+    return s
+
+
+# ------------------------------------------------------------------------------------------------------------------- one pass
+def run(s):
+    return (_run_own if own else _run_plain)(s, s["case"])
+
+
+def _run_own(s, case):
+    from jmodt_amd.ops import adapters, rows8
+    op = case["op"]
+    if op == "keep":
+        kept = rows8.checkpoint_rows(s["x"])
+        return rows8.restore_rows(kept, s["x"].dtype), kept.exps
+    if op == "wgrad8":
+        return rows8.linear_wgrad8(s["dy"], s["kept"])
+    if op == "adapt":
+        plan = adapters.AdapterPlan(s["ids"], case["adapters"]) if case["plan"] else s["plan"]
+        if case["t"]:
+            return adapters.adapter_forward(s["base"], s["x"], s["a"], s["b"], s["scales"], plan, want_t=True)
+        return adapters.adapter_forward(s["base"], s["x"], s["a"], s["b"], s["scales"], plan)
+    x = s["kept"] if case["x"] == "e4m3" else s["x"]
+    return adapters.adapter_grad(s["dy"], x, s["t"], s["a"], s["b"], s["scales"], s["plan"], base=s["base"])
+
+
+def _run_plain(s, case):
+    op = case["op"]
+    if op == "keep":
+        codes, exps = _encode(s["x"])
+        return _decode(codes, exps).to(s["x"].dtype), exps
+    if op == "wgrad8":
+        dy = s["dy"].float()
+        return dy.t() @ _decode(s["codes"], s["exps"]), dy.sum(dim=0)
+    a, b, scales, ids = s["a"], s["b"], s["scales"], s["ids"]
+    if op == "adapt":
+        out = s["base"].float()
+        t = torch.zeros(case["m"], case["rank"], device=out.device)
+        for i in range(case["adapters"]):
+            rows = torch.nonzero(ids == i)[:, 0]
+            low = s["x"][rows].float() @ a[i].float().t()
+            t[rows] = low
+            out[rows] += scales[i] * (low @ b[i].float().t())
+        out = out.to(s["base"].dtype)
+        return (out, t) if case["t"] else out
+    x = _decode(s["codes"], s["exps"]) if case["x"] == "e4m3" else s["x"].float()
+    dy, dx = s["dy"].float(), s["base"].float()
+    da, db = torch.zeros(a.shape, device=dx.device), torch.zeros(b.shape, device=dx.device)
+    for i in range(case["adapters"]):
+        rows = torch.nonzero(ids == i)[:, 0]
+        d = dy[rows]
+        u = scales[i] * (d @ b[i].float())
+        dx[rows] += u @ a[i].float()
+        da[i] = u.t() @ x[rows]
+        db[i] = scales[i] * (d.t() @ s["t"][rows])
+    return dx.to(s["base"].dtype), da.to(a.dtype), db.to(b.dtype)
+
+
+# ------------------------------------------------------------------------------------------------------------------- 64 bits
+def _exact_values(codes, exps):
+    """the values that the codes stand for, from the bits: (-1)^s 2^(E - 7) (1 + M / 8), E = 0: 2^-6 M / 8, S.1111.111: NaN"""
+    c = codes.to(torch.int64)
+    expo, man = (c >> 3) & 15, (c & 7).double()
+    v = torch.where(expo > 0, torch.ldexp(1.0 + man / 8.0, (expo - 7).double()), torch.ldexp(man / 8.0, torch.full_like(man, -6.0)))
+    v = torch.where((c & 127) == 127, torch.full_like(v, math.nan), v)
+    v = torch.where(c >= 128, -v, v)
+    block = torch.arange(codes.shape[1], device=codes.device) // 32
+    return torch.ldexp(v, (exps.to(torch.int64) - 127).double()[:, block])
+
+
+def _exact_keep(x):
+    x = x.double()
+    m, c = x.shape
+    out = torch.empty_like(x)
+    exps = torch.empty(m, -(-c // 32), dtype=torch.uint8, device=x.device)
+    for j in range(exps.shape[1]):
+        part = x[:, 32 * j:32 * j + 32]
+        fin = torch.isfinite(part)
+        top = torch.where(fin, part.abs(), torch.zeros_like(part)).max(dim=1).values
+        e = torch.full_like(top, -100.0)
+        some = top > 0
+        guess = torch.floor(torch.log2(torch.where(some, top, torch.ones_like(top)))) - 10.0
+        for _ in range(4):                                         # the smallest power of two that holds the block
+            guess = torch.where(top > 448.0 * torch.exp2(guess), guess + 1.0, guess)
+        e = torch.where(some, torch.maximum(guess, e), e)
+        step = torch.exp2(e)[:, None]
+        v = torch.where(fin, part, torch.zeros_like(part)) / step
+        mag = v.abs()
+        unit = torch.exp2(torch.floor(torch.log2(mag.clamp(min=2.0 ** -6))) - 3.0)     # the distance of two e4m3 values there
+        q = torch.round(mag / unit) * unit                         # (torch.round: ties to even)
+        q = torch.where((q == 0) & (part != 0), torch.full_like(q, 2.0 ** -9), q)
+        val = torch.where(part < 0, -q, q) * step
+        out[:, 32 * j:32 * j + 32] = torch.where(fin, val, torch.full_like(val, math.nan))
+        exps[:, j] = (e + 127.0).to(torch.uint8)
+    return out, exps
+
+
+def exact(case, seed):
+    s = _inputs(case, seed)
+    op = case["op"]
+    if op == "keep":
+        return _exact_keep(s["x"])
+    if op == "wgrad8":
+        dy = s["dy"].double()
+        return torch.mm(dy.t().contiguous(), _exact_values(s["codes"], s["exps"])), dy.sum(dim=0)
+    a, b, scales = s["a"].double(), s["b"].double(), s["scales"].double()
+    ids = s["ids"].to(torch.int64)
+    m, r, count = case["m"], case["rank"], case["adapters"]
+    member = [(ids == i).double()[:, None] for i in range(count)]  # (rows of other adapters count zero times)
+    if op == "adapt":
+        x = s["x"].double()
+        low = torch.zeros(m, r, dtype=torch.float64, device=x.device)
+        out = s["base"].double()
+        for i in range(count):
+            part = torch.mm(x, a[i].t().contiguous()) * member[i]
+            low += part
+            out += torch.mm(part, b[i].t().contiguous()) * scales[i]
+        return (out, low) if case["t"] else out
+    x = _exact_values(s["codes"], s["exps"]) if case["x"] == "e4m3" else s["x"].double()
+    dy, t, dx = s["dy"].double(), s["t"].double(), s["base"].double()
+    da, db = torch.empty_like(a), torch.empty_like(b)
+    for i in range(count):
+        d = dy * member[i]
+        u = torch.mm(d, b[i]) * scales[i]
+        dx += torch.mm(u, a[i])
+        da[i] = torch.mm(u.t().contiguous(), x)
+        db[i] = torch.mm(d.t().contiguous(), t) * scales[i]
+    return dx, da, db
