@@ -9,6 +9,8 @@ measured and rejected, kept for the A/B scripts).  The product library contains 
 One translation unit per op family, compiled in parallel, linked into ONE shared library with a
 flat C ABI (include/jmodt_hip.h).  -ffp-contract=off: the kernels spell out every fused
 operation they want (see oracle/jmodt_oracle.c header for the floating-point conventions).
+-packed-fp32-ops: no v_pk_add / mul / fma_f32 — some forms of the packed fp32 instructions have given wrong results on this
+hardware now and then; the scalar forms have the same rounding.  (hipcc's host pass does not know the feature and says so.)
 """
 import os
 import subprocess
@@ -24,7 +26,8 @@ LIB = os.path.join(HERE, "libjmodt_hip.so")
 OBJ_DIR = os.path.join(HERE, "build")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math",
-         "-fvisibility=hidden", "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function", "-DJM_BUILDING"]
+         "-fvisibility=hidden", "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function", "-DJM_BUILDING",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _mtime(p):

@@ -49,7 +49,7 @@ conv3x3_rgb_kernel(int H, int W, int cout, int cg, int ng, const float* __restri
     float* T = lds + (size_t)wave * 64 * ld;
     // tap-outer: all cg (<= 32) accumulators of the lane's pixel stay in registers; one tap's cg weights are cg
     // consecutive floats of the tap-major array = wide scalar loads (s_load_dwordx8 / x16) into the SGPR operands of
-    // v_pk_fma_f32 (two channels per instruction); uniform addresses: weights and bias through the scalar cache
+    // the FMAs; uniform addresses: weights and bias through the scalar cache
     auto run = [&](auto NQ_) __attribute__((always_inline)) {
         constexpr int NQ = decltype(NQ_)::value;                 // float4 groups of output channels: cg = 4 NQ
         f32x2 acc[2 * NQ];

@@ -196,10 +196,9 @@ fps_regs2_kernel(int n, int m, int bs, int bs_log2, int R, int J, int recipJ, co
         }
         float best = -1.f;
         if constexpr (PTS % 2 == 0) {
-            // packed fp32 (v_pk_add/mul/fma_f32): two points per instruction.  Every component is
-            // the same IEEE operation sequence as the scalar path (sub, mul, fma, fma), so results
-            // are bit-identical; a wave64 packed op costs ~4 issue cycles against ~3 for a plain
-            // VALU op, i.e. 1.5x the distance throughput.
+            // two points per step.  Every component is the same IEEE operation sequence as the one-point path (sub, mul, fma,
+            // fma), so results are bit-identical; the build turns the packed fp32 instructions off (csrc/build.py), the pairs
+            // are two scalar chains.
             const f32x2 cx = {x1, x1}, cy = {y1, y1}, cz = {z1, z1};
 #pragma unroll
             for (int i = 0; i < PTS; i += 2) {

@@ -6,11 +6,11 @@
 // input features: rows = (centre, sample), row input = xyz[idx] - centre (pointnet2_utils.py:259-262), three
 // 1x1 conv + folded BN + ReLU layers, max over the samples.  7.5 GFLOP for 1.57 M rows at batch 8.
 //
-// Why not the matrix cores: fp32 MFMA and packed fp32 VALU (v_pk_fma_f32) have the SAME peak on this chip (157 TFLOP/s), and
+// Why not the matrix cores: the fp32 MFMA and the fp32 VALU peaks are close on this chip, and
 // with contraction lengths of 3, 16 and 32 the MFMA route pays for its operand layout instead of computing: the general
 // kernel (sa_mlp_kernel: gather waves -> LDS tiles -> 32x32x2 MFMAs with K padded to 16, 256 registers, 44 of them
 // spilled) takes 0.19 ms per scale = 0.12 of the peak.  Here a LANE owns a row: the three layers are straight-line
-// v_pk_fma_f32 on registers (two output channels per instruction, the input broadcast into both halves), the weights are
+// FMAs on registers (pairs of output channels, the input broadcast into both), the weights are
 // wave-uniform and come through the SCALAR cache straight into the SGPR operand of the FMA (s_load_dwordx4.. of the k-major
 // copy jm_sa_mlp_pack appends to small layers; as vector registers from LDS they push hipcc into thousands of spills: the
 // weights of a fully unrolled layer do not fit next to its accumulators), the max over a centre's 16 / 32 samples is 4 / 5
@@ -165,7 +165,7 @@ sa_xyz_valu_kernel(SaXyzParams p) {
     }
 
     // One layer for a chunk of 16 output channels: acc[r][8] (pairs) += in[r][kk] * Wt[kk][n0 .. n0 + 15] over kk < KIN; the
-    // addresses are uniform, so the weights are scalar loads into SGPRs (the SGPR operand of v_pk_fma_f32)
+    // addresses are uniform, so the weights are scalar loads into SGPRs (the SGPR operand of the FMA)
     auto chunk16 = [&](auto KIN_, auto IN_, const f32x2 (*in)[decltype(IN_)::value], bool relu_in, wptr Wt, int ldw,
                        wptr bias, int n0, f32x2 (&acc)[ROWS][8]) __attribute__((always_inline)) {
         constexpr int KIN = decltype(KIN_)::value;
