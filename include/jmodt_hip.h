@@ -789,6 +789,46 @@ int jm_fold_bn_multi(int n, const float* const* w, float* const* wf, const int* 
 int jm_fold_bn_multi_grad(int n, const float* const* dwf, const float* const* w, float* const* dw, const int* rows, const int* cols,
                           const int* soff, const float* s, float* ds, jm_stream_t stream);
 
+/* ------------------------------------------------------------------ rows kept in 8 bits (csrc/rows8.hip) -------- */
+#define JM_F32 0    /* element types of the entries below */
+#define JM_BF16 1
+#define JM_F16 2
+/* x (m, c), rows ldx apart -> e4m3 codes (m, c) in rows of ldc bytes (a multiple of 16, >= c; the bytes behind c are written as zero up to
+ * the next multiple of 16) and one scale byte per 32 channels, exps (m, ceil(c / 32)).  Per block: amax = the largest finite |x|, 2^e the
+ * smallest power of two with amax <= 448 2^e and e >= -100 (amax = 0: e = -100), byte = e + 127, code = x / 2^e to the nearest e4m3
+ * value, ties to even; a value that is not zero never becomes zero (it takes the smallest code of its sign), one that is not finite
+ * becomes NaN.  codes: 16-byte aligned; x: aligned to its element. */
+int jm_rows8_pack(int m, int c, int type, const void* x, long long ldx, unsigned char* codes, int ldc, unsigned char* exps, jm_stream_t stream);
+/* the values that the codes stand for, rounded once to the type (float32 and bfloat16 hold them exactly) */
+int jm_rows8_restore(int m, int c, int type, const unsigned char* codes, int ldc, const unsigned char* exps, void* out, long long ldo, jm_stream_t stream);
+/* out (m, c) = (kept value > 0) ? dy : 0: the gradient through a ReLU whose output was kept; out may be dy */
+int jm_rows8_relu_mask(int m, int c, const float* dy, int ldd, const unsigned char* codes, int ldc, float* out, int ldo, jm_stream_t stream);
+/* dw (n, k) = dy (m, n)^T X (m, k) with X kept (codes, exps), dbias (n) = column sums of dy (NULL: skipped).  Sums in float32, in a
+ * fixed order.  ws: >= jm_rows8_wgrad_workspace_bytes, 16-byte aligned. */
+size_t jm_rows8_wgrad_workspace_bytes(int m, int n, int k);
+int jm_rows8_linear_wgrad(int m, int n, int k, int type, const void* dy, long long lddy, const unsigned char* codes, int ldc, const unsigned char* exps,
+                          float* dw, long long lddw, float* dbias, void* ws, size_t ws_bytes, jm_stream_t stream);
+
+/* ------------------------------------------------------------------ low-rank adapters (csrc/adapters.hip) -------- */
+#define JM_ADAPTER_MAX_RANK 128
+/* The rows of every adapter, in device memory: ids (m) names the adapter of each row; a value outside 0 .. adapters - 1 is a row
+ * without one.  plan: jm_adapter_plan_elems(m, adapters) int32, 16-byte aligned; adapters <= 1023. */
+size_t jm_adapter_plan_elems(int m, int adapters);
+int jm_adapter_plan(int m, int adapters, const int* ids, int* plan, jm_stream_t stream);
+/* out[r] = base[r] + scales[a] b_a (a_a x[r]), a_a (rank, k), b_a (n, rank), a = the adapter of row r; rows without one: out = base.
+ * base NULL: zero; base == out (and ldb == ldo): in place.  t (m, rank) float32 = a_a x[r] (rows without an adapter: 0), or NULL.
+ * plan: jm_adapter_plan's for the same m and adapters. */
+int jm_adapter_forward(int m, int k, int n, int rank, int adapters, int type, const void* x, long long ldx, const void* a, const void* b,
+                       const float* scales, const int* plan, const void* base, long long ldb, void* out, long long ldo, float* t, jm_stream_t stream);
+/* dx[r] = base[r] + scales[a] a_a^T (b_a^T dy[r]) (base NULL: zero; base == dx: in place); da_a = scales[a] sum (b_a^T dy[r]) x[r]^T,
+ * db_a = scales[a] sum dy[r] t[r]^T over the rows of a (none: zero), float32 sums in a fixed order, rounded once.  x: rows of the
+ * type, or NULL with the kept form (codes, exps) of jm_rows8_pack.  ws: 16-byte aligned. */
+size_t jm_adapter_grad_workspace_bytes(int m, int k, int n, int rank, int adapters, int type);
+int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const void* dy, long long lddy, const void* x, long long ldx,
+                    const unsigned char* codes, int ldc, const unsigned char* exps, const float* t, const void* a, const void* b, const float* scales,
+                    const int* plan, const void* base, long long ldb, void* dx, long long lddx, void* da, void* db, void* ws, size_t ws_bytes,
+                    jm_stream_t stream);
+
 #pragma GCC visibility pop
 #ifdef __cplusplus
 }
