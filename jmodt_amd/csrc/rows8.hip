@@ -143,94 +143,271 @@ rows8_relu_mask_kernel(long long items, int c, int groups, const float* dy, int 
 }
 
 // ------------------------------------------------------------------------------------------------ weight gradient from kept rows
-// dW (n, k) = dY (m, n)^T X (m, k), db (n) = column sums of dY.  Workgroup = a 64 x 64 tile of dW over one split of the rows, 32 rows of
-// both operands at a time through LDS as float32, four waves of 16 x 64, 16 x 16 x 4 float32 products; the splits' partial tiles are
-// added in split order by the second kernel (no float atomics: the same bits every time).
-constexpr int W8_T = 64, W8_R = 32, W8_LD = W8_T + 4;
+// dW (n, k) = dY (m, n)^T X (m, k), db (n) = column sums of dY.
+//
+// On the bf16 matrix pipe although dW is a float32 result: a kept value is exact in bfloat16, and a gradient is the sum of bfloat16
+// pieces without any rounding — a float32 value of three (24 significant bits = 8 + 8 + 8, cut off, not rounded), a float16 value of two, a
+// bfloat16 value of one — so every product is exact and only the float32 additions round, as on the float32 pipe, at a third of sixteen
+// times its rate.
+//
+// Workgroup = a 128 x 128 tile of dW over one split of the rows, 64 rows at a time.  A thread fetches 8 rows x 4 columns of both
+// operands (the next 64 rows' while this one's are multiplied), cuts and converts them, and stores 8 rows of one column as 16 bytes: the
+// contraction index becomes the fast one on the way into LDS, and a matrix operand (8 rows of a column) is one 16-byte read.  In LDS column
+// 4 i + q of a tile sits in slot 32 q + i: writes and reads of a wave are contiguous.  Four waves of 64 x 64 (2 x 2 products of
+// 32 x 32 x 16), two workgroups a CU: one stores while the other multiplies.
+// The splits' partial tiles are added in split order by the second kernel (no float atomics: the same bits every time).
+constexpr int W8_T = 128, W8_R = 64, W8_SLAB = W8_R * W8_T;          // (elements of one operand piece in LDS)
 
 struct Wgrad8 {
-    int m, n, k, splits, rows_per;       // rows_per: rows of a split
+    int m, n, k, splits, rows_per;       // rows_per: rows of a split, a multiple of W8_R
     const void* dy; long long lddy;
     const unsigned char* codes; int ldc; const unsigned char* exps; int blocks;
     float *dw, *db;                      // (splits, n, k) and (splits, n) partials, or the results when splits == 1
     long long lddw;
 };
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// four consecutive columns of a row.  The columns of a group that lies outside the matrix are whatever lies inside (they only reach
+// outputs that are never stored); a group that straddles the edge (`ragged`, widths that are no multiple of 4) is read from width - 4 and shifted
+template <int TY> struct Quad;
+template <> struct Quad<JM_F32> {
+    f32x4 v;
+    __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(&v, p, 16); }
+    __device__ __forceinline__ void shift(int n) {
+        if (n & 1) { v[0] = v[1]; v[1] = v[2]; v[2] = v[3]; }
+        if (n & 2) { v[0] = v[2]; v[1] = v[3]; }
+    }
+    __device__ __forceinline__ void zero() { v = f32x4{0.f, 0.f, 0.f, 0.f}; }
+    __device__ __forceinline__ float get(int q) const { return v[q]; }
+};
+template <int TY> struct Quad16 {
+    unsigned long long v;
+    __device__ __forceinline__ void load(const typename Elem<TY>::T* p) { __builtin_memcpy(&v, p, 8); }
+    __device__ __forceinline__ void shift(int n) { v >>= 16 * n; }
+    __device__ __forceinline__ void zero() { v = 0; }
+    __device__ __forceinline__ unsigned bits(int q) const { return (unsigned)(v >> (16 * q)) & 0xffffu; }
+    __device__ __forceinline__ float get(int q) const {
+        const unsigned short h = (unsigned short)bits(q);
+        typename Elem<TY>::T t;
+        __builtin_memcpy(&t, &h, 2);
+        return (float)t;
+    }
+};
+template <> struct Quad<JM_BF16> : Quad16<JM_BF16> {};
+template <> struct Quad<JM_F16> : Quad16<JM_F16> {};
+
+// the upper halves of two words as one: (hi half of a) | (hi half of b) << 16
+__device__ __forceinline__ unsigned pack_hi(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
 template <int TY>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 rows8_wgrad_kernel(Wgrad8 p) {
     typedef typename Elem<TY>::T T;
-    __shared__ float Ys[W8_R][W8_LD], Xs[W8_R][W8_LD];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, i = lane & 15, g = lane >> 4;
-    const int tk = (p.k + W8_T - 1) / W8_T;
-    const int n0 = (int)(blockIdx.x / tk) * W8_T, k0 = (int)(blockIdx.x % tk) * W8_T;
-    const long long r_begin = (long long)blockIdx.y * p.rows_per, r_end = min((long long)p.m, r_begin + p.rows_per);
-    const T* dy = (const T*)p.dy;
-    f32x4 acc[4];
+    constexpr int P = TY == JM_F32 ? 3 : (TY == JM_F16 ? 2 : 1);                  // pieces of a gradient
+    typedef __bf16 frag_t __attribute__((ext_vector_type(8)));
+    typedef float f32x16 __attribute__((ext_vector_type(16)));
+    __shared__ __attribute__((aligned(16))) unsigned short lds[(P + 1) * W8_SLAB];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // workgroups are dealt to the 8 XCDs in turn: the tiles of one split, which read the same rows, stay on one of them
+    const int tk = (p.k + W8_T - 1) / W8_T, tiles = ((p.n + W8_T - 1) / W8_T) * tk;
+    const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
+    const int split = (local / tiles) * 8 + xcd, tile = local % tiles;
+    if (split >= p.splits) return;
+    const int n0 = (tile / tk) * W8_T, k0 = (tile % tk) * W8_T;
+    const long long r_begin = (long long)split * p.rows_per, r_end = min((long long)p.m, r_begin + p.rows_per);
+
+    // fetch: rows 8 oct .. + 7 of the 64, columns 4 l .. + 3 of both tiles
+    const int l = lane & 31, oct = wave * 2 + (lane >> 5);
+    const int cy = n0 + 4 * l, cx = min(k0 + 4 * l, p.ldc - 4);
+    const int ylast = p.n - 4;                               // (n < 4: element by element below)
+    const int ysh = (ylast >= 0 && cy < p.n) ? max(0, cy - ylast) : 0;
+    const bool ragged = (p.n & 3) != 0 && n0 + W8_T > p.n;
+    const T* dyp = (const T*)p.dy + (ylast >= 0 ? min(cy, ylast) : 0);
+    const unsigned char* xp = p.codes + cx;
+    const unsigned char* ep = p.exps + min(cx / R8_BLOCK, p.blocks - 1);
+    Quad<TY> y[8];
+    unsigned x[8];
+    unsigned e[8];
+    auto fetch = [&](long long r) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float bsum = 0.f;
-    const int col = tid & 63, r0 = tid >> 6;
+        for (int q = 0; q < 8; ++q) {
+            const long long row = min(r + 8 * oct + q, (long long)p.m - 1);
+            if (p.n >= 4) {
+                y[q].load(dyp + row * p.lddy);
+            } else {
+                T t[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) t[c] = dyp[row * p.lddy + min(c, p.n - 1)];
+                y[q].load(t);
+            }
+            x[q] = *reinterpret_cast<const unsigned*>(xp + row * p.ldc);
+            e[q] = ep[row * p.blocks];
+        }
+    };
+    float bs[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool do_bias = p.db != nullptr && k0 == 0;
+    auto stage = [&](long long r) __attribute__((always_inline)) {
+        if (r + W8_R > r_end) {                              // rows behind the split count as zeros on both sides
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (r + 8 * oct + q >= r_end) { y[q].zero(); x[q] = 0u; e[q] = 127u; }
+        }
+        if (ragged) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) y[q].shift(ysh);
+        }
+        if (do_bias) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) bs[c] += y[q].get(c);
+        }
+        u32x4* Y = reinterpret_cast<u32x4*>(lds) + oct * W8_T + l;          // 16 bytes = 8 rows of a slot
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            u32x4 w[P];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                if constexpr (TY == JM_BF16) {
+                    w[0][h] = y[2 * h].bits(c) | (y[2 * h + 1].bits(c) << 16);
+                } else {
+                    unsigned a = __float_as_uint(y[2 * h].get(c)), b = __float_as_uint(y[2 * h + 1].get(c));
+#pragma unroll
+                    for (int s = 0; s < P; ++s) {
+                        w[s][h] = pack_hi(a, b);
+                        if (s + 1 < P) {
+                            // what the cut left; of an infinity nothing (inf - inf would be NaN), of a NaN a NaN
+                            const float fa = __uint_as_float(a), fb = __uint_as_float(b);
+                            const float ra = fa - __uint_as_float(a & 0xffff0000u), rb = fb - __uint_as_float(b & 0xffff0000u);
+                            a = __builtin_isinf(fa) ? 0u : __float_as_uint(ra);
+                            b = __builtin_isinf(fb) ? 0u : __float_as_uint(rb);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < P; ++s) Y[s * (W8_SLAB / 8) + c * 32] = w[s];
+        }
+        // kept values: codes of a row share a scale within the four columns
+        unsigned v0[8], v1[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const float sc = __uint_as_float(e[q] << 23);
+            const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x[q], sc, false);
+            const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x[q], sc, true);
+            __builtin_memcpy(&v0[q], &lo, 4);
+            __builtin_memcpy(&v1[q], &hi, 4);
+        }
+        u32x4* X = reinterpret_cast<u32x4*>(lds + P * W8_SLAB) + oct * W8_T + l;
+        u32x4 w0, w1, w2, w3;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            w0[h] = __builtin_amdgcn_perm(v0[2 * h + 1], v0[2 * h], 0x05040100u);
+            w1[h] = pack_hi(v0[2 * h], v0[2 * h + 1]);
+            w2[h] = __builtin_amdgcn_perm(v1[2 * h + 1], v1[2 * h], 0x05040100u);
+            w3[h] = pack_hi(v1[2 * h], v1[2 * h + 1]);
+        }
+        X[0] = w0; X[32] = w1; X[64] = w2; X[96] = w3;
+    };
+
+    const int wn = wave >> 1, wk = wave & 1, lr = lane & 31, lk = lane >> 5;
+    f32x16 acc[2][2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[a][b][q] = 0.f;
+    if (r_begin < r_end) fetch(r_begin);
     for (long long r = r_begin; r < r_end; r += W8_R) {
+        stage(r);
         __syncthreads();
+        if (r + W8_R < r_end) fetch(r + W8_R);
+        const u32x4* Y = reinterpret_cast<const u32x4*>(lds);
+        const u32x4* X = reinterpret_cast<const u32x4*>(lds + P * W8_SLAB);
 #pragma unroll
-        for (int q = 0; q < W8_R / 4; ++q) {
-            const long long row = r + r0 + 4 * q;
-            const bool ok = row < r_end;
-            Ys[r0 + 4 * q][col] = (ok && n0 + col < p.n) ? (float)dy[row * p.lddy + n0 + col] : 0.f;
-            float x = 0.f;
-            if (ok && k0 + col < p.k)
-                x = __builtin_amdgcn_cvt_pk_f32_fp8((int)p.codes[row * p.ldc + k0 + col], false)[0] *
-                    exp2i((int)p.exps[row * p.blocks + (k0 + col) / R8_BLOCK] - 127);
-            Xs[r0 + 4 * q][col] = x;
+        for (int s = 0; s < W8_R / 16; ++s) {
+            const int at = (2 * s + lk) * W8_T + lr;
+            frag_t xb[2], ya[P][2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) xb[b] = __builtin_bit_cast(frag_t, X[at + (2 * wk + b) * 32]);
+#pragma unroll
+            for (int c = 0; c < P; ++c)
+#pragma unroll
+                for (int a = 0; a < 2; ++a) ya[c][a] = __builtin_bit_cast(frag_t, Y[c * (W8_SLAB / 8) + at + (2 * wn + a) * 32]);
+#pragma unroll
+            for (int c = P - 1; c >= 0; --c)
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ya[c][a], xb[b], acc[a][b], 0, 0, 0);
         }
         __syncthreads();
-        if (k0 == 0 && wave == 0)
-            for (int q = 0; q < W8_R; ++q) bsum += Ys[q][col];
+    }
+
+    float* dw = p.dw + (p.splits > 1 ? (size_t)split * p.n * p.k : 0);
+    const int k = k0 + 4 * lr + 2 * wk;
 #pragma unroll
-        for (int q = 0; q < W8_R; q += 4) {
-            const float a = Ys[q + g][wave * 16 + i];
+    for (int a = 0; a < 2; ++a)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, Xs[q + g][j * 16 + i], acc[j], 0, 0, 0);
+        for (int q = 0; q < 16; ++q) {
+            const int n = n0 + 4 * ((q & 3) + 8 * (q >> 2) + 4 * lk) + 2 * wn + a;
+            if (n < p.n) {
+                float* d = dw + (size_t)n * p.lddw + k;
+                if (k < p.k) d[0] = acc[a][0][q];
+                if (k + 1 < p.k) d[1] = acc[a][1][q];
+            }
+        }
+    if (do_bias) {                                           // the eight row groups' sums, in order
+        f32x4* red = reinterpret_cast<f32x4*>(lds);
+        red[oct * 32 + l] = f32x4{bs[0], bs[1], bs[2], bs[3]};
+        __syncthreads();
+        if (tid < 32) {
+            f32x4 s = red[tid];
+            for (int o = 1; o < 8; ++o) s += red[o * 32 + tid];
+            float* db = p.db + (p.splits > 1 ? (size_t)split * p.n : 0);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (n0 + 4 * tid + c < p.n) db[n0 + 4 * tid + c] = s[c];
         }
     }
-    float* dw = p.dw + (p.splits > 1 ? (size_t)blockIdx.y * p.n * p.k : 0);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int n = n0 + wave * 16 + 4 * g + q, k = k0 + j * 16 + i;
-            if (n < p.n && k < p.k) dw[(size_t)n * p.lddw + k] = acc[j][q];
-        }
-    if (k0 == 0 && wave == 0 && p.db != nullptr && n0 + col < p.n) p.db[(p.splits > 1 ? (size_t)blockIdx.y * p.n : 0) + n0 + col] = bsum;
 }
 
-// out[i] = the sum of the splits' partials in split order: items 0 .. n k - 1 are dW, then n of db
+// out = the sum of the splits' partials: items 0 .. n k - 1 are dW, then n of db.  A workgroup takes 64 items; its four waves sum every
+// fourth split (four chains each: the loads of consecutive splits are in flight together) and are added in wave order.
 __global__ void __launch_bounds__(256)
 rows8_wgrad_reduce_kernel(int n, int k, int splits, const float* __restrict__ part_w, const float* __restrict__ part_b, float* __restrict__ dw,
                           long long lddw, float* __restrict__ db) {
+    __shared__ float red[4][64];
     const long long nk = (long long)n * k;
-    const long long i = blockIdx.x * 256ll + threadIdx.x;
-    if (i >= nk + (db ? n : 0)) return;
-    const bool w = i < nk;
-    const float* src = w ? part_w + i : part_b + (i - nk);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long i = blockIdx.x * 64ll + lane;
+    const bool w = i < nk, ok = i < nk + (db ? n : 0);
+    const float* src = w ? part_w + i : part_b + (ok ? i - nk : 0);
     const size_t step = w ? (size_t)nk : (size_t)n;
     float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-    int t = 0;
-    for (; t + 4 <= splits; t += 4) {
-        s0 += src[(size_t)t * step];       s1 += src[(size_t)(t + 1) * step];
-        s2 += src[(size_t)(t + 2) * step]; s3 += src[(size_t)(t + 3) * step];
+    if (ok) {
+        int t = wave;
+        for (; t + 12 < splits; t += 16) {
+            s0 += src[(size_t)t * step];       s1 += src[(size_t)(t + 4) * step];
+            s2 += src[(size_t)(t + 8) * step]; s3 += src[(size_t)(t + 12) * step];
+        }
+        for (; t < splits; t += 4) s0 += src[(size_t)t * step];
     }
-    for (; t < splits; ++t) s0 += src[(size_t)t * step];
-    const float s = (s0 + s1) + (s2 + s3);
+    red[wave][lane] = (s0 + s1) + (s2 + s3);
+    __syncthreads();
+    if (wave > 0 || !ok) return;
+    const float s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
     if (w) dw[(i / k) * lddw + i % k] = s;
     else db[i - nk] = s;
 }
 
+// splits of the rows: two workgroups for every CU, at least 128 rows (two steps) each
 static int wgrad8_splits(int m, int n, int k) {
     const long long tiles = (long long)divup(n, W8_T) * divup(k, W8_T);
-    long long s = (1024 + tiles - 1) / tiles;
-    const int cap = imax(1, m / 256);
+    long long s = (512 + tiles - 1) / tiles;
+    const int cap = imax(1, m / 128);
     if (s > cap) s = cap;
     return (int)s;
 }
@@ -300,18 +477,20 @@ int jm_rows8_linear_wgrad(int m, int n, int k, int type, const void* dy, long lo
     }
     hipStream_t s = (hipStream_t)stream;
     Wgrad8 p{};
-    p.m = m; p.n = n; p.k = k; p.splits = splits; p.rows_per = divup(divup(m, splits), W8_R) * W8_R;
+    p.m = m; p.n = n; p.k = k; p.splits = splits; p.rows_per = m > 0 ? ((m - 1) / splits / W8_R + 1) * W8_R : W8_R;
     p.dy = dy; p.lddy = lddy; p.codes = codes; p.ldc = ldc; p.exps = exps; p.blocks = divup(k, R8_BLOCK);
     float* part_b = (float*)ws + (size_t)splits * n * k;
     if (splits > 1) { p.dw = (float*)ws; p.lddw = k; p.db = dbias ? part_b : nullptr; }
     else { p.dw = dw; p.lddw = lddw; p.db = dbias; }
-    const dim3 grid((unsigned)(divup(n, W8_T) * divup(k, W8_T)), (unsigned)splits), block(256);
+    const long long wgs = (long long)divup(n, W8_T) * divup(k, W8_T) * (divup(splits, 8) * 8);
+    JM_REQUIRE(wgs <= 0x7fffffffll, "rows8_linear_wgrad: n %d, k %d", n, k);
+    const dim3 grid((unsigned)wgs), block(256);
     if (type == JM_F32) hipLaunchKernelGGL((rows8_wgrad_kernel<JM_F32>), grid, block, 0, s, p);
     else if (type == JM_BF16) hipLaunchKernelGGL((rows8_wgrad_kernel<JM_BF16>), grid, block, 0, s, p);
     else hipLaunchKernelGGL((rows8_wgrad_kernel<JM_F16>), grid, block, 0, s, p);
     if (splits > 1) {
         const long long items = (long long)n * k + (dbias ? n : 0);
-        hipLaunchKernelGGL(rows8_wgrad_reduce_kernel, dim3((unsigned)((items + 255) / 256)), block, 0, s, n, k, splits, (const float*)ws,
+        hipLaunchKernelGGL(rows8_wgrad_reduce_kernel, dim3((unsigned)((items + 63) / 64)), block, 0, s, n, k, splits, (const float*)ws,
                            (const float*)part_b, dw, lddw, dbias);
     }
     return check_launch("rows8_linear_wgrad");
