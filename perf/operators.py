@@ -235,11 +235,14 @@ def _run_own(s, case):
         return rows8.linear_wgrad8(s["dy"], s["kept"])
     if op == "adapt":
         plan = adapters.AdapterPlan(s["ids"], case["adapters"]) if case["plan"] else s["plan"]
-        if case["t"]:
-            return adapters.adapter_forward(s["base"], s["x"], s["a"], s["b"], s["scales"], plan, want_t=True)
-        return adapters.adapter_forward(s["base"], s["x"], s["a"], s["b"], s["scales"], plan)
+        return adapters.adapter_forward(s["base"], s["x"], s["a"], s["b"], s["scales"], plan, out=_over(s, case), want_t=case["t"])
     x = s["kept"] if case["x"] == "e4m3" else s["x"]
-    return adapters.adapter_grad(s["dy"], x, s["t"], s["a"], s["b"], s["scales"], s["plan"], base=s["base"])
+    return adapters.adapter_grad(s["dy"], x, s["t"], s["a"], s["b"], s["scales"], s["plan"], base=s["base"], out=_over(s, case))
+
+
+def _over(s, case):
+    """float32: base itself, updated in place as the plain form does (there base.float() is base); else a new tensor"""
+    return s["base"] if case["type"] == "f32" else None
 
 
 def _run_plain(s, case):
