@@ -9,10 +9,11 @@
 // t, u and every sum are float32; base + s B t is rounded once.
 //
 // The rows of an adapter are found by a plan in device memory (a stable counting sort of the rows by adapter, built by three small
-// kernels, one for up to PL_ROWS rows; the host never learns the counts): tiles of 16 rows and chunks of AD_CHUNK rows, each of one
+// kernels, one for up to PL_ROWS rows; the host never learns the counts): tiles of 16 or 32 rows and chunks of AD_CHUNK rows, each of one
 // adapter.
 #include "jm_elem.h"
 #include "jm_rows.h"
+#include <type_traits>
 
 namespace jm {
 
@@ -20,7 +21,9 @@ namespace jm {
 constexpr int PL_ROWS = 4096;        // rows of a counting block
 constexpr int PL_THREADS = 1024;
 constexpr int PL_MAX_ADAPTERS = 1023;        // + the rows without an adapter: one counter a thread
-constexpr int AD_TILE = 16;          // rows of a tile
+constexpr int AD_WIDE_ROWS = 16384;
+// rows of a tile: 16 while that leaves CUs idle, 32 where there are enough tiles (A and B are read once a tile)
+static __host__ __device__ __forceinline__ int ad_tile(int m) { return m < AD_WIDE_ROWS ? 16 : 32; }
 constexpr int AD_CHUNK = 1024;       // rows of a chunk (weight gradients)
 constexpr int AD_MAX_ROWS = 1 << 30, AD_MAX_WIDTH = 1 << 20;        // tile counts, grids and per-adapter element counts stay in range
 
@@ -31,7 +34,7 @@ struct PlanLayout {                  // offsets in ints; header: [0] tiles, [1] 
 static PlanLayout plan_layout(int m, int adapters) {
     PlanLayout l;
     l.blocks = divup(m, PL_ROWS);
-    l.max_tiles = divup(m, AD_TILE) + (adapters + 1 < m ? adapters + 1 : m);
+    l.max_tiles = divup(m, ad_tile(m)) + (adapters + 1 < m ? adapters + 1 : m);
     l.max_chunks = divup(m, AD_CHUNK) + (adapters < m ? adapters : m);
     l.order = 4;
     l.tiles = align_up(l.order + (size_t)m, 4);
@@ -68,10 +71,10 @@ __device__ __forceinline__ void plan_scan3(int (&v)[3], int (*wave_tot)[3]) {
 
 // bucket counts -> starts, and the tables of tiles and chunks.  `count`: this thread's bucket count (thread = bucket).
 // first[b] = {row start, first tile, first chunk} of bucket b, first[adapters + 1] = the totals.
-__device__ void plan_tables(int count, int adapters, int (*first)[3], int (*wave_tot)[3], int* __restrict__ plan, size_t o_tiles, size_t o_chunks,
+__device__ void plan_tables(int count, int adapters, int tile_rows, int (*first)[3], int (*wave_tot)[3], int* __restrict__ plan, size_t o_tiles, size_t o_chunks,
                             size_t o_chunk_first) {
     const int b = threadIdx.x;
-    int v[3] = {count, (count + AD_TILE - 1) / AD_TILE, b < adapters ? (count + AD_CHUNK - 1) / AD_CHUNK : 0};
+    int v[3] = {count, (count + tile_rows - 1) / tile_rows, b < adapters ? (count + AD_CHUNK - 1) / AD_CHUNK : 0};
     const int mine[3] = {v[0], v[1], v[2]};
     plan_scan3(v, wave_tot);
     if (b <= adapters)
@@ -91,8 +94,8 @@ __device__ void plan_tables(int count, int adapters, int (*first)[3], int (*wave
             const int mid = (lo + hi + 1) >> 1;
             if (first[mid][1] <= t) lo = mid; else hi = mid - 1;
         }
-        const int start = first[lo][0] + (t - first[lo][1]) * AD_TILE;
-        *reinterpret_cast<int4*>(plan + o_tiles + 4 * (size_t)t) = make_int4(lo < adapters ? lo : -1, start, min(AD_TILE, first[lo + 1][0] - start), 0);
+        const int start = first[lo][0] + (t - first[lo][1]) * tile_rows;
+        *reinterpret_cast<int4*>(plan + o_tiles + 4 * (size_t)t) = make_int4(lo < adapters ? lo : -1, start, min(tile_rows, first[lo + 1][0] - start), 0);
     }
     for (int t = b; t < nc; t += PL_THREADS) {
         int lo = 0, hi = adapters - 1;
@@ -156,7 +159,7 @@ adapter_plan_count_kernel(int m, int adapters, const int* __restrict__ ids, int*
     for (int r = threadIdx.x; r < rows; r += PL_THREADS) atomicAdd(&cnt[plan_bucket(ids, row0 + r, adapters)], 1);
     __syncthreads();
     if constexpr (WHOLE) {
-        plan_tables(cnt[threadIdx.x], adapters, first, wave_tot, plan, o_tiles, o_chunks, o_chunk_first);
+        plan_tables(cnt[threadIdx.x], adapters, ad_tile(m), first, wave_tot, plan, o_tiles, o_chunks, o_chunk_first);
         __syncthreads();
         if ((int)threadIdx.x <= adapters) cnt[threadIdx.x] = first[threadIdx.x][0];
         plan_scatter(ids, 0, rows, adapters, cnt, wcnt, plan + o_order);
@@ -167,13 +170,13 @@ adapter_plan_count_kernel(int m, int adapters, const int* __restrict__ ids, int*
 
 // the blocks' counts -> every block's first place of every bucket (in place), and the tables
 __global__ void __launch_bounds__(PL_THREADS)
-adapter_plan_tables_kernel(int blocks, int adapters, int* __restrict__ plan, size_t o_tiles, size_t o_chunks, size_t o_chunk_first, size_t o_hist) {
+adapter_plan_tables_kernel(int m, int blocks, int adapters, int* __restrict__ plan, size_t o_tiles, size_t o_chunks, size_t o_chunk_first, size_t o_hist) {
     __shared__ int first[PL_THREADS + 2][3], wave_tot[16][3];
     const int b = threadIdx.x;
     int total = 0;
     if (b <= adapters)
         for (int k = 0; k < blocks; ++k) total += plan[o_hist + (size_t)k * (adapters + 1) + b];
-    plan_tables(total, adapters, first, wave_tot, plan, o_tiles, o_chunks, o_chunk_first);
+    plan_tables(total, adapters, ad_tile(m), first, wave_tot, plan, o_tiles, o_chunks, o_chunk_first);
     if (b <= adapters) {
         int at = first[b][0];
         for (int k = 0; k < blocks; ++k) {
@@ -207,128 +210,264 @@ struct Adapt {
     int copy;                            // base and out are not the same rows: rows without an adapter are copied
 };
 
-// A wave owns a tile of 16 rows.  First t (rank x 16 rows) = A x^T over k, 32 elements a step, both operands straight from memory into
-// the registers of the 16 x 16 products; t crosses the lanes through LDS; then out (n x 16 rows), 64 channels at a time: the rows of B
-// are permuted so that a lane ends up with 16 consecutive channels of its row.
+// 16 consecutive channels of a row
+template <int TY>
+struct Run16 {
+    typedef typename Elem<TY>::T T;
+    typedef typename Elem<TY>::V8 V8;
+    V8 v[2];
+    __device__ __forceinline__ void load(const T* p, int n) {
+        if (n >= 16) { v[0] = load8<V8>(p); v[1] = load8<V8>(p + 8); }
+        else { v[0] = load8_upto<V8>(p, n); v[1] = load8_upto<V8>(p + 8, n - 8); }
+    }
+    __device__ __forceinline__ void store(T* p, int n) const {
+        if (n >= 16) { store8(p, v[0]); store8(p + 8, v[1]); return; }
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (e < n) p[e] = v[e >> 3][e & 7];
+    }
+};
+
+// A workgroup owns a tile of 16 MB rows of one adapter (and every gridDim.y-th group of four 64-channel blocks of out: with few rows the
+// workgroups of one tile each make t again, which costs less than a CU left idle).
+//   1  t (rank x rows) = A x^T: the four waves take a quarter of k each, 32 elements a step, both operands straight from memory into the
+//      registers of the 16 x 16 products (lane: 8 consecutive elements of one row), UK steps in flight; the quarters are added through LDS.
+//   2  out (channels x rows) = base + s B t^T: a wave takes 64 channels; the rows of B are permuted so that a lane ends up with 16
+//      consecutive channels of its row, which it reads from base and writes to out.
 // t enters the second product as the sum of two values of the 16-bit type (16 significant bits in bfloat16, 22 in float16, where the
-// row is scaled by a power of two first: t may leave float16's range although out does not); as it is in float32.
-template <int TY, int RB>
-__global__ void __launch_bounds__(64)
+// row is scaled by a power of two first: t may leave float16's range although out does not); as it is in float32.  With a rank of up
+// to 16 both values share one product: the contraction is 32 long, [hi | lo] times [B | B].
+template <int TY, int RB, int MB>
+__global__ void __launch_bounds__(256)
 adapter_rows_kernel(Adapt p) {
     typedef typename Elem<TY>::T T;
     typedef typename Elem<TY>::V8 V8;
-    constexpr int RS = (RB * 16 + 31) / 32;              // 32-wide steps over the rank
-    constexpr int LD = RS * 32 + 4;
-    __shared__ __attribute__((aligned(16))) float ts[16][LD];
+    constexpr int RP = RB * 16, LD = RP + 4, ROWS = 16 * MB;
+    constexpr int UK = (TY == JM_F32 ? 4 : 8) / (RB < 2 ? 1 : (RB < 8 ? RB / 2 * MB : 8 / (TY == JM_F32 ? 2 : 1)));
+    constexpr bool PAIR = TY != JM_F32 && RB == 1;       // hi and lo in one contraction
+    constexpr int RS = TY == JM_F32 ? RB : (RB + 1) / 2; // contraction steps over the rank: 16 long in float32, 32 otherwise
+    __shared__ __attribute__((aligned(16))) float ts[2][ROWS][LD];
     if ((int)blockIdx.x >= p.plan[0]) return;
     const int4 tile = *reinterpret_cast<const int4*>(p.plan + p.o_tiles + 4 * (size_t)blockIdx.x);
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ad = tile.x, count = tile.z;
-    const bool live = i < count;
-    const size_t row = (size_t)p.plan[p.o_order + tile.y + min(i, count - 1)];
-    const T* base = p.base ? (const T*)p.base + row * p.ldb : nullptr;
-    T* out = (T*)p.out + row * p.ldo;
+    const int* order = p.plan + p.o_order + tile.y;
+    size_t row[MB];
+    bool live[MB];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+        live[mb] = mb * 16 + i < count;
+        row[mb] = (size_t)order[min(mb * 16 + i, count - 1)];
+    }
+    const int nblocks = (p.n + 63) / 64;
+    const T* const base = (const T*)p.base;
+    T* const out = (T*)p.out;
     if (ad < 0) {                                        // rows without an adapter
-        if (!live) return;
         if (p.copy)
-            for (int c = g; c < p.n; c += 4) out[c] = base ? base[c] : (T)0.f;
-        if (p.t)
-            for (int c = g; c < p.rank; c += 4) p.t[row * p.rank + c] = 0.f;
+            for (int nb = blockIdx.y * 4 + wave; nb < nblocks; nb += gridDim.y * 4)
+#pragma unroll
+                for (int mb = 0; mb < MB; ++mb)
+                    if (live[mb]) {
+                        const int c = nb * 64 + 16 * g;
+                        Run16<TY> v;
+                        if (base) v.load(base + row[mb] * p.ldb + c, p.n - c);
+                        else
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) v.v[e >> 3][e & 7] = (T)0.f;
+                        v.store(out + row[mb] * p.ldo + c, p.n - c);
+                    }
+        if (p.t && blockIdx.y == 0)
+            for (int e = threadIdx.x; e < count * p.rank; e += 256) p.t[(size_t)order[e / p.rank] * p.rank + e % p.rank] = 0.f;
         return;
     }
-    const T* x = (const T*)p.x + row * p.ldx;
     const T* A = (const T*)p.a + (size_t)ad * p.rank * p.k;
     const T* B = (const T*)p.b + (size_t)ad * p.n * p.rank;
     const float scale = p.scales[ad];
 
-    f32x4 acc[RB];
+    {
+        const T *xr[MB], *ar[RB];
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) acc[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < p.k; k0 += 32) {
-        const int kk = k0 + 8 * g, left = p.k - kk;
-        const V8 xv = load8_upto<V8>(x + kk, left);
+        for (int mb = 0; mb < MB; ++mb) xr[mb] = (const T*)p.x + row[mb] * p.ldx + 8 * g;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            const V8 av = load8_upto<V8>(A + (size_t)min(rb * 16 + i, p.rank - 1) * p.k + kk, left);
-            acc[rb] = mma16(acc[rb], av, xv);            // D: column = row i of the tile, rows = rank index 4 g + q
-        }
-    }
-    // rank indices beyond the rank hold copies of the last one: zeroed, so that the second product contracts zeros there
+        for (int rb = 0; rb < RB; ++rb) ar[rb] = A + (size_t)min(rb * 16 + i, p.rank - 1) * p.k + 8 * g;
+        f32x4 acc[MB][RB];
 #pragma unroll
-    for (int rb = 0; rb < 2 * RS; ++rb) {
-        f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (rb < RB)
+        for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = rb * 16 + 4 * g + q < p.rank ? acc[rb < RB ? rb : 0][q] : 0.f;
-        *reinterpret_cast<f32x4*>(&ts[i][rb * 16 + 4 * g]) = v;
-    }
-    __syncthreads();
-    if (p.t && live)
-        for (int c = g; c < p.rank; c += 4) p.t[row * p.rank + c] = ts[i][c];
-
-    float back = scale;
-    V8 hi[RS], lo[RS];
-    float fit = 1.f;
-    if constexpr (TY == JM_F16) {
-        float top = 0.f;
+            for (int rb = 0; rb < RB; ++rb) acc[mb][rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const int nk = (p.k + 31) / 32, per = (nk + 3) / 4;
+        int s = wave * per;
+        const int s_end = min(nk, s + per), s_full = min(s_end, p.k / 32);
+        auto batch = [&](auto n_) __attribute__((always_inline)) {
+            constexpr int U = decltype(n_)::value;
+            V8 xv[U][MB], av[U][RB];
 #pragma unroll
-        for (int s = 0; s < RS; ++s)
+            for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(ts[i][s * 32 + 8 * g + e]));
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 126);      // the row's values become less than 2
-        fit = __uint_as_float((unsigned)(127 - ex) << 23);
-        back = scale * __uint_as_float((unsigned)(127 + ex) << 23);
-    }
+                for (int mb = 0; mb < MB; ++mb) xv[u][mb] = load8<V8>(xr[mb] + 32 * (s + u));
 #pragma unroll
-    for (int s = 0; s < RS; ++s)
+                for (int rb = 0; rb < RB; ++rb) av[u][rb] = load8<V8>(ar[rb] + 32 * (s + u));
+            }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float v = ts[i][s * 32 + 8 * g + e] * fit;
-            const T h = (T)v;
-            hi[s][e] = h;
-            if constexpr (TY != JM_F32) lo[s][e] = (T)(fabsf((float)h) < __builtin_inff() ? v - (float)h : 0.f);
-        }
-
-    for (int n0 = 0; n0 < p.n; n0 += 64) {
-        f32x4 d[4];
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            d[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            const T* Br = B + (size_t)min(n0 + (i >> 2) * 16 + j * 4 + (i & 3), p.n - 1) * p.rank;
+                for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-            for (int s = 0; s < RS; ++s) {
-                const int r0 = s * 32 + 8 * g;
-                const V8 bv = load8_upto<V8>(Br + r0, p.rank - r0);
-                d[j] = mma16(d[j], bv, hi[s]);
-                if constexpr (TY != JM_F32) d[j] = mma16(d[j], bv, lo[s]);
+                    for (int rb = 0; rb < RB; ++rb) acc[mb][rb] = mma16(acc[mb][rb], av[u][rb], xv[u][mb]);
+            s += U;
+        };
+        while (s + UK <= s_full) batch(std::integral_constant<int, UK>{});
+        if constexpr (UK > 4) { if (s + 4 <= s_full) batch(std::integral_constant<int, 4>{}); }
+        if constexpr (UK > 2) { if (s + 2 <= s_full) batch(std::integral_constant<int, 2>{}); }
+        if constexpr (UK > 1) { if (s + 1 <= s_full) batch(std::integral_constant<int, 1>{}); }
+        for (; s < s_end; ++s) {
+            const int left = p.k - 32 * s - 8 * g;
+            V8 xv[MB];
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) xv[mb] = load8_upto<V8>(xr[mb] + 32 * s, left);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const V8 av = load8_upto<V8>(ar[rb] + 32 * s, left);
+#pragma unroll
+                for (int mb = 0; mb < MB; ++mb) acc[mb][rb] = mma16(acc[mb][rb], av, xv[mb]);
             }
         }
-        if (live) {
+        // D: column = row i of the block, rows = rank index 4 g + q
+        if (wave < 2)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int c = n0 + 16 * g + 4 * j + q;
-                    if (c < p.n) out[c] = (T)((base ? (float)base[c] : 0.f) + back * d[j][q]);
+                for (int rb = 0; rb < RB; ++rb) *reinterpret_cast<f32x4*>(&ts[wave][mb * 16 + i][rb * 16 + 4 * g]) = acc[mb][rb];
+        __syncthreads();
+        if (wave >= 2)
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    f32x4* q = reinterpret_cast<f32x4*>(&ts[wave - 2][mb * 16 + i][rb * 16 + 4 * g]);
+                    *q = *q + acc[mb][rb];
+                }
+        __syncthreads();
+    }
+    if (p.t && blockIdx.y == 0)
+        for (int e = threadIdx.x; e < count * p.rank; e += 256) {
+            const int r = e / p.rank, c = e - r * p.rank;
+            p.t[(size_t)order[r] * p.rank + c] = ts[0][r][c] + ts[1][r][c];
+        }
+    if (blockIdx.y * 4 + wave >= nblocks) return;
+
+    // this lane's part of t; rank indices beyond the rank (copies of the last one) are zeros
+    auto tval = [&](int mb, int r) { return r < p.rank ? ts[0][mb * 16 + i][r] + ts[1][mb * 16 + i][r] : 0.f; };
+    float back[MB];
+    f32x4 t32[TY == JM_F32 ? MB : 1][RS];
+    V8 hi[MB][RS], lo[MB][RS];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+        back[mb] = scale;
+        if constexpr (TY == JM_F32) {
+#pragma unroll
+            for (int s = 0; s < RS; ++s)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t32[mb][s][e] = tval(mb, s * 16 + 4 * g + e);
+        } else {
+            float v[RS][8], fit = 1.f, top = 0.f;
+#pragma unroll
+            for (int s = 0; s < RS; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[s][e] = tval(mb, PAIR ? 8 * (g & 1) + e : s * 32 + 8 * g + e);
+                    top = fmaxf(top, fabsf(v[s][e]));
+                }
+            if constexpr (TY == JM_F16) {
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const int ex = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 126);      // the row's values become less than 4
+                fit = __uint_as_float((unsigned)(127 - ex) << 23);
+                back[mb] = scale * __uint_as_float((unsigned)(127 + ex) << 23);
+            }
+#pragma unroll
+            for (int s = 0; s < RS; ++s)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float f = v[s][e] * fit;
+                    const T h = (T)f;
+                    const T r = (T)(fabsf((float)h) < __builtin_inff() ? f - (float)h : 0.f);
+                    hi[mb][s][e] = (PAIR && g >= 2) ? r : h;
+                    lo[mb][s][e] = r;
                 }
         }
     }
+
+    for (int nb = blockIdx.y * 4 + wave; nb < nblocks; nb += gridDim.y * 4) {
+        const int n0 = nb * 64, c = n0 + 16 * g;
+        Run16<TY> bv[MB];
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+            if (base) bv[mb].load(base + row[mb] * p.ldb + c, p.n - c);
+            else
+#pragma unroll
+                for (int e = 0; e < 16; ++e) bv[mb].v[e >> 3][e & 7] = (T)0.f;
+        }
+        f32x4 d[MB][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const T* Br = B + (size_t)min(n0 + (i >> 2) * 16 + j * 4 + (i & 3), p.n - 1) * p.rank;
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) d[mb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < RS; ++s) {
+                if constexpr (TY == JM_F32) {
+                    const int r0 = s * 16 + 4 * g;
+                    f32x4 b4;
+                    if (r0 + 4 <= p.rank) __builtin_memcpy(&b4, Br + r0, 16);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) b4[e] = r0 + e < p.rank ? Br[r0 + e] : 0.f;
+#pragma unroll
+                    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) d[mb][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(b4[e], t32[mb][s][e], d[mb][j], 0, 0, 0);
+                } else {
+                    const int r0 = PAIR ? 8 * (g & 1) : s * 32 + 8 * g;
+                    const V8 b8 = load8_upto<V8>(Br + r0, p.rank - r0);
+#pragma unroll
+                    for (int mb = 0; mb < MB; ++mb) {
+                        d[mb][j] = mma16(d[mb][j], b8, hi[mb][s]);
+                        if constexpr (!PAIR) d[mb][j] = mma16(d[mb][j], b8, lo[mb][s]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+            if (live[mb]) {
+                Run16<TY> o;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o.v[e >> 3][e & 7] = (T)((float)bv[mb].v[e >> 3][e & 7] + back[mb] * d[mb][e >> 2][e & 3]);
+                o.store(out + row[mb] * p.ldo + c, p.n - c);
+            }
+    }
 }
 
-// (count, rows, cols) -> (count, cols, rows)
+// (adapters, rank, k) -> (adapters, k, rank) and (adapters, n, rank) -> (adapters, rank, n): blockIdx.x walks the 32 x 32 tiles of both
 template <typename T>
 __global__ void __launch_bounds__(256)
-adapter_transpose_kernel(int rows, int cols, const T* __restrict__ src, T* __restrict__ dst) {
+adapter_transpose_kernel(int rank, int k, int n, const T* __restrict__ a, T* __restrict__ at, const T* __restrict__ b, T* __restrict__ bt) {
     __shared__ T tile[32][33];
-    const size_t off = (size_t)blockIdx.z * rows * cols;
-    const int c0 = blockIdx.x * 32, r0 = blockIdx.y * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int tr = (rank + 31) / 32, ta = ((k + 31) / 32) * tr;
+    const bool isA = (int)blockIdx.x < ta;
+    const int id = isA ? blockIdx.x : blockIdx.x - ta;
+    const int rows = isA ? rank : n, cols = isA ? k : rank;
+    const int r0 = (isA ? id % tr : id / tr) * 32, c0 = (isA ? id / tr : id % tr) * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const size_t off = (size_t)blockIdx.y * rows * cols;
+    const T* src = (isA ? a : b) + off;
+    T* dst = (isA ? at : bt) + off;
     for (int q = ty; q < 32; q += 8)
-        if (r0 + q < rows && c0 + tx < cols) tile[q][tx] = src[off + (size_t)(r0 + q) * cols + c0 + tx];
+        if (r0 + q < rows && c0 + tx < cols) tile[q][tx] = src[(size_t)(r0 + q) * cols + c0 + tx];
     __syncthreads();
     for (int q = ty; q < 32; q += 8)
-        if (c0 + q < cols && r0 + tx < rows) dst[off + (size_t)(c0 + q) * rows + r0 + tx] = tile[tx][q];
+        if (c0 + q < cols && r0 + tx < rows) dst[(size_t)(c0 + q) * rows + r0 + tx] = tile[tx][q];
 }
 
 // ------------------------------------------------------------------------------------------------ gradients of A and B
@@ -356,19 +495,37 @@ __device__ __forceinline__ f32x4 grad_load4(const AdaptGrad& p, const void* src,
         const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
         v = f32x4{lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
     } else {
-        const typename Elem<TY>::T* q = (const typename Elem<TY>::T*)src + row * ld + c;
+        typedef typename Elem<TY>::T T;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        const T* q = (const T*)src + row * ld + c;
+        T4 r;
+        if (c + 4 <= width) {
+            __builtin_memcpy(&r, q, sizeof(T4));
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = c + e < width ? (float)q[e] : 0.f;
+            for (int e = 0; e < 4; ++e) {
+                T t = (T)0.f;
+                if (c + e < width) t = q[e];
+                r[e] = t;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)r[e];
     }
     return v;
 }
 
 // Workgroup = (chunk of one adapter's rows) x (64 channels of x, then of dy) x (64 rank indices); its four waves take every fourth group
-// of four rows, 16 x 16 x 4 float32 products of T (t or u: rank) with X (channels), and add their tiles in wave order through LDS.
+// of four rows, 16 x 16 x 4 float32 products of T (t or u: rank) with X (channels), UR groups in flight, and add their tiles in wave
+// order through LDS.
 template <int TY, bool KEPT, int RB>
 __global__ void __launch_bounds__(256)
 adapter_wgrad_kernel(AdaptGrad p) {
-    __shared__ f32x4 red[3][RB * 4][64];
+    constexpr int UR = 8;
+    __shared__ union {
+        f32x4 red[3][RB * 4][64];
+        int order[AD_CHUNK];
+    } sh;
     if ((int)blockIdx.x >= p.plan[1]) return;
     const int4 chunk = *reinterpret_cast<const int4*>(p.plan + p.o_chunks + 4 * (size_t)blockIdx.x);
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
@@ -376,26 +533,43 @@ adapter_wgrad_kernel(AdaptGrad p) {
     const bool isA = (int)blockIdx.y < tk;
     const int c0 = (isA ? (int)blockIdx.y : (int)blockIdx.y - tk) * 64, width = isA ? p.k : p.n, r0 = blockIdx.z * 64;
     const float* T = isA ? p.u : p.t;
+    for (int q = threadIdx.x; q < chunk.z; q += 256) sh.order[q] = p.plan[p.o_order + chunk.y + q];
+    __syncthreads();
     f32x4 acc[RB][4];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[rb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int q = wave * 4; q < chunk.z; q += 16) {
-        const bool ok = q + g < chunk.z;
-        const size_t row = (size_t)p.plan[p.o_order + chunk.y + min(q + g, chunk.z - 1)];
-        f32x4 xv;
-        if (isA) xv = grad_load4<TY, KEPT>(p, p.x, p.ldx, row, c0 + 4 * i, width);
-        else xv = grad_load4<TY, false>(p, p.dy, p.lddy, row, c0 + 4 * i, width);
+    auto body = [&](auto kept_, const void* src, long long ld) __attribute__((always_inline)) {
+        constexpr bool K8 = decltype(kept_)::value;
+        for (int q0 = wave * 4; q0 < chunk.z; q0 += 16 * UR) {
+            f32x4 xv[UR];
+            float tv[UR][RB];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) xv[e] = ok ? xv[e] : 0.f;
+            for (int u = 0; u < UR; ++u) {               // (rows beyond the chunk: the last one, counted as zeros)
+                const size_t row = (size_t)sh.order[min(q0 + 16 * u + g, chunk.z - 1)];
+                xv[u] = grad_load4<TY, K8>(p, src, ld, row, c0 + 4 * i, width);
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            const float tv = ok ? T[row * p.rank + min(r0 + rb * 16 + i, p.rank - 1)] : 0.f;
+                for (int rb = 0; rb < RB; ++rb) tv[u][rb] = T[row * p.rank + min(r0 + rb * 16 + i, p.rank - 1)];
+            }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[rb][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(tv, xv[j], acc[rb][j], 0, 0, 0);
+            for (int u = 0; u < UR; ++u) {
+                const bool ok = q0 + 16 * u + g < chunk.z;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) xv[u][e] = ok ? xv[u][e] : 0.f;
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    const float t = ok ? tv[u][rb] : 0.f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[rb][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(t, xv[u][j], acc[rb][j], 0, 0, 0);
+                }
+            }
         }
-    }
+    };
+    if (KEPT && isA) body(std::integral_constant<bool, KEPT>{}, nullptr, 0);
+    else body(std::false_type{}, isA ? p.x : p.dy, isA ? p.ldx : p.lddy);
+    __syncthreads();
+    auto& red = sh.red;
     if (wave > 0)
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
@@ -434,8 +608,14 @@ adapter_wgrad_reduce_kernel(AdaptGrad p) {
     if (e >= per) return;
     const int c_begin = p.plan[p.o_chunk_first + ad], c_end = p.plan[p.o_chunk_first + ad + 1];
     float s = 0.f;
-    for (int c = c_begin; c < c_end; ++c) s += p.part[(size_t)c * per + e];
-    s *= p.scales[ad];
+    float s1 = 0.f, s2 = 0.f, s3 = 0.f;                  // four chains: the loads of consecutive chunks are in flight together
+    int c = c_begin;
+    for (; c + 4 <= c_end; c += 4) {
+        s += p.part[(size_t)c * per + e];        s1 += p.part[(size_t)(c + 1) * per + e];
+        s2 += p.part[(size_t)(c + 2) * per + e]; s3 += p.part[(size_t)(c + 3) * per + e];
+    }
+    for (; c < c_end; ++c) s += p.part[(size_t)c * per + e];
+    s = ((s + s1) + (s2 + s3)) * p.scales[ad];
     const int na = p.rank * p.k;
     if (c_begin == c_end) s = 0.f;
     if (e < na) ((T*)p.da)[(size_t)ad * na + e] = (T)s;
@@ -444,18 +624,25 @@ adapter_wgrad_reduce_kernel(AdaptGrad p) {
 
 static size_t elem_size(int type) { return type == JM_F32 ? 4 : 2; }
 
+template <int TY, int RB>
+static void launch_rows(const Adapt& p, dim3 grid, hipStream_t s) {
+    if (ad_tile(p.m) == 16) hipLaunchKernelGGL((adapter_rows_kernel<TY, RB, 1>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((adapter_rows_kernel<TY, RB, 2>), grid, dim3(256), 0, s, p);
+}
 template <int TY>
-static void launch_rows(const Adapt& p, int tiles, hipStream_t s) {
-    const dim3 grid((unsigned)tiles), block(64);
-    if (p.rank <= 16) hipLaunchKernelGGL((adapter_rows_kernel<TY, 1>), grid, block, 0, s, p);
-    else if (p.rank <= 32) hipLaunchKernelGGL((adapter_rows_kernel<TY, 2>), grid, block, 0, s, p);
-    else if (p.rank <= 64) hipLaunchKernelGGL((adapter_rows_kernel<TY, 4>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((adapter_rows_kernel<TY, 8>), grid, block, 0, s, p);
+static void launch_rows(const Adapt& p, dim3 grid, hipStream_t s) {
+    if (p.rank <= 16) launch_rows<TY, 1>(p, grid, s);
+    else if (p.rank <= 32) launch_rows<TY, 2>(p, grid, s);
+    else if (p.rank <= 64) launch_rows<TY, 4>(p, grid, s);
+    else launch_rows<TY, 8>(p, grid, s);
 }
 static void launch_rows(int type, const Adapt& p, int tiles, hipStream_t s) {
-    if (type == JM_F32) launch_rows<JM_F32>(p, tiles, s);
-    else if (type == JM_BF16) launch_rows<JM_BF16>(p, tiles, s);
-    else launch_rows<JM_F16>(p, tiles, s);
+    // few tiles: several workgroups a tile, as far as there are channel blocks and idle CUs
+    const int y = imax(1, (int)((long long)divup(p.n, 256) < 256 / tiles ? divup(p.n, 256) : 256 / tiles));
+    const dim3 grid((unsigned)tiles, (unsigned)y);
+    if (type == JM_F32) launch_rows<JM_F32>(p, grid, s);
+    else if (type == JM_BF16) launch_rows<JM_BF16>(p, grid, s);
+    else launch_rows<JM_F16>(p, grid, s);
 }
 
 template <int TY, bool KEPT>
@@ -507,7 +694,7 @@ int jm_adapter_plan(int m, int adapters, const int* ids, int* plan, jm_stream_t 
     }
     hipLaunchKernelGGL((adapter_plan_count_kernel<false>), dim3((unsigned)l.blocks), dim3(PL_THREADS), 0, s, m, adapters, ids, plan, l.order, l.tiles, l.chunks,
                        l.chunk_first, l.hist);
-    hipLaunchKernelGGL(adapter_plan_tables_kernel, dim3(1), dim3(PL_THREADS), 0, s, l.blocks, adapters, plan, l.tiles, l.chunks, l.chunk_first, l.hist);
+    hipLaunchKernelGGL(adapter_plan_tables_kernel, dim3(1), dim3(PL_THREADS), 0, s, m, l.blocks, adapters, plan, l.tiles, l.chunks, l.chunk_first, l.hist);
     hipLaunchKernelGGL(adapter_plan_scatter_kernel, dim3((unsigned)l.blocks), dim3(PL_THREADS), 0, s, m, adapters, ids, plan, l.order, l.hist);
     return check_launch("adapter_plan");
 }
@@ -553,14 +740,12 @@ int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const
     q.o_chunk_first = l.chunk_first; q.x = x; q.ldx = ldx; q.codes = codes; q.ldc = ldc; q.exps = exps; q.blocks = divup(k, 32);
     q.dy = dy; q.lddy = lddy; q.t = t; q.u = (const float*)(w + gl.u); q.scales = scales; q.part = (float*)(w + gl.part); q.da = da; q.db = db;
     if (m > 0) {
-        const dim3 ga((unsigned)divup(k, 32), (unsigned)divup(rank, 32), (unsigned)adapters), gb((unsigned)divup(rank, 32), (unsigned)divup(n, 32), (unsigned)adapters);
+        const dim3 gt((unsigned)((divup(k, 32) + divup(n, 32)) * divup(rank, 32)), (unsigned)adapters);
         if (type == JM_F32) {
-            hipLaunchKernelGGL((adapter_transpose_kernel<float>), ga, dim3(256), 0, s, rank, k, (const float*)a, (float*)(w + gl.at));
-            hipLaunchKernelGGL((adapter_transpose_kernel<float>), gb, dim3(256), 0, s, n, rank, (const float*)b, (float*)(w + gl.bt));
+            hipLaunchKernelGGL((adapter_transpose_kernel<float>), gt, dim3(256), 0, s, rank, k, n, (const float*)a, (float*)(w + gl.at), (const float*)b, (float*)(w + gl.bt));
         } else {
             typedef unsigned short u16;
-            hipLaunchKernelGGL((adapter_transpose_kernel<u16>), ga, dim3(256), 0, s, rank, k, (const u16*)a, (u16*)(w + gl.at));
-            hipLaunchKernelGGL((adapter_transpose_kernel<u16>), gb, dim3(256), 0, s, n, rank, (const u16*)b, (u16*)(w + gl.bt));
+            hipLaunchKernelGGL((adapter_transpose_kernel<u16>), gt, dim3(256), 0, s, rank, k, n, (const u16*)a, (u16*)(w + gl.at), (const u16*)b, (u16*)(w + gl.bt));
         }
         Adapt p{};
         p.m = m; p.k = n; p.n = k; p.rank = rank; p.plan = plan; p.o_order = l.order; p.o_tiles = l.tiles; p.x = dy; p.ldx = lddy;
