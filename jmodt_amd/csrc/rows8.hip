@@ -12,10 +12,12 @@
 // 1.03 bytes per element instead of 4 (float32) or 2.
 #include "jm_elem.h"
 #include "jm_rows.h"
+#include <type_traits>
 
 namespace jm {
 
 constexpr int R8_BLOCK = 32;         // channels per scale
+constexpr int R8_MAX_ROWS = 1 << 30;        // (row counters of the weight gradient are 32 bits wide)
 constexpr int R8_EMIN = -100;        // least scale exponent: 2^e and the smallest code 2^(e - 9) stay normal in float32 and bfloat16
 
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }      // -126 <= e <= 127
@@ -200,7 +202,7 @@ template <> struct Quad<JM_F16> : Quad16<JM_F16> {};
 // the upper halves of two words as one: (hi half of a) | (hi half of b) << 16
 __device__ __forceinline__ unsigned pack_hi(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-template <int TY>
+template <int TY, bool SMALL>
 __global__ void __launch_bounds__(256, 2)
 rows8_wgrad_kernel(Wgrad8 p) {
     typedef typename Elem<TY>::T T;
@@ -215,43 +217,57 @@ rows8_wgrad_kernel(Wgrad8 p) {
     const int split = (local / tiles) * 8 + xcd, tile = local % tiles;
     if (split >= p.splits) return;
     const int n0 = (tile / tk) * W8_T, k0 = (tile % tk) * W8_T;
-    const long long r_begin = (long long)split * p.rows_per, r_end = min((long long)p.m, r_begin + p.rows_per);
+    const int r_begin = min((long long)split * p.rows_per, (long long)p.m), r_end = min(p.m, r_begin + p.rows_per);
 
     // fetch: rows 8 oct .. + 7 of the 64, columns 4 l .. + 3 of both tiles
     const int l = lane & 31, oct = wave * 2 + (lane >> 5);
     const int cy = n0 + 4 * l, cx = min(k0 + 4 * l, p.ldc - 4);
-    const int ylast = p.n - 4;                               // (n < 4: element by element below)
-    const int ysh = (ylast >= 0 && cy < p.n) ? max(0, cy - ylast) : 0;
-    const bool ragged = (p.n & 3) != 0 && n0 + W8_T > p.n;
-    const T* dyp = (const T*)p.dy + (ylast >= 0 ? min(cy, ylast) : 0);
+    const int ylast = p.n - 4;
+    const int ysh = (!SMALL && cy < p.n) ? max(0, cy - ylast) : 0;
+    const bool ragged = !SMALL && (p.n & 3) != 0 && n0 + W8_T > p.n;
+    const T* dyp = (const T*)p.dy + (SMALL ? 0 : min(cy, ylast));
     const unsigned char* xp = p.codes + cx;
     const unsigned char* ep = p.exps + min(cx / R8_BLOCK, p.blocks - 1);
-    Quad<TY> y[8];
-    unsigned x[8];
-    unsigned e[8];
-    auto fetch = [&](long long r) __attribute__((always_inline)) {
+    struct Rows {
+        Quad<TY> y[8];
+        unsigned x[8], e[8];
+    };
+    Rows rows[2];
+    // the last octet of the matrix is read from row m - 8 on: rows before its own first one count as zeros (stage)
+    auto first_row = [&](int r) { return SMALL ? r + 8 * oct : min(r + 8 * oct, p.m - 8); };
+    auto fetch = [&](Rows& d, int r) __attribute__((always_inline)) {
+        const int at = first_row(r);
+        const T* py = dyp + (long long)at * p.lddy;
+        const unsigned char* px = xp + (long long)at * p.ldc;
+        const unsigned char* pe = ep + (long long)at * p.blocks;
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-            const long long row = min(r + 8 * oct + q, (long long)p.m - 1);
-            if (p.n >= 4) {
-                y[q].load(dyp + row * p.lddy);
-            } else {
+            if constexpr (SMALL) {                           // fewer than 8 rows or 4 columns: element by element
+                const long long row = min(at + q, p.m - 1);
                 T t[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) t[c] = dyp[row * p.lddy + min(c, p.n - 1)];
-                y[q].load(t);
+                for (int c = 0; c < 4; ++c) t[c] = dyp[row * p.lddy + min(cy + c, p.n - 1)];
+                d.y[q].load(t);
+                d.x[q] = *reinterpret_cast<const unsigned*>(xp + row * p.ldc);
+                d.e[q] = ep[row * p.blocks];
+            } else {
+                d.y[q].load(py + q * p.lddy);
+                d.x[q] = *reinterpret_cast<const unsigned*>(px + q * (long long)p.ldc);
+                d.e[q] = pe[q * (long long)p.blocks];
             }
-            x[q] = *reinterpret_cast<const unsigned*>(xp + row * p.ldc);
-            e[q] = ep[row * p.blocks];
         }
     };
     float bs[4] = {0.f, 0.f, 0.f, 0.f};
     const bool do_bias = p.db != nullptr && k0 == 0;
-    auto stage = [&](long long r) __attribute__((always_inline)) {
-        if (r + W8_R > r_end) {                              // rows behind the split count as zeros on both sides
+    auto stage = [&](Rows& d, int r) __attribute__((always_inline)) {
+        Quad<TY>(&y)[8] = d.y;
+        unsigned(&x)[8] = d.x;
+        unsigned(&e)[8] = d.e;
+        if (r + W8_R > r_end) {                              // rows outside this step's own count as zeros on both sides
+            const int at = first_row(r);
 #pragma unroll
             for (int q = 0; q < 8; ++q)
-                if (r + 8 * oct + q >= r_end) { y[q].zero(); x[q] = 0u; e[q] = 127u; }
+                if (at + q >= r_end || at + q < r + 8 * oct) { y[q].zero(); x[q] = 0u; e[q] = 127u; }
         }
         if (ragged) {
 #pragma unroll
@@ -263,32 +279,45 @@ rows8_wgrad_kernel(Wgrad8 p) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) bs[c] += y[q].get(c);
         }
+        // an infinity leaves no rest (inf - inf would be NaN), a NaN leaves a NaN: looked for once for the whole wave
+        bool inf_seen = false;
+        if constexpr (P > 1) {
+            float z = 0.f;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) z = __builtin_fmaf(y[q].get(c), 0.f, z);
+            inf_seen = __ballot(z != z) != 0ull;
+        }
         u32x4* Y = reinterpret_cast<u32x4*>(lds) + oct * W8_T + l;          // 16 bytes = 8 rows of a slot
+        auto cut = [&](auto special_) __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            u32x4 w[P];
+            for (int c = 0; c < 4; ++c) {
+                u32x4 w[P];
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                if constexpr (TY == JM_BF16) {
-                    w[0][h] = y[2 * h].bits(c) | (y[2 * h + 1].bits(c) << 16);
-                } else {
-                    unsigned a = __float_as_uint(y[2 * h].get(c)), b = __float_as_uint(y[2 * h + 1].get(c));
+                for (int h = 0; h < 4; ++h) {
+                    if constexpr (TY == JM_BF16) {
+                        w[0][h] = y[2 * h].bits(c) | (y[2 * h + 1].bits(c) << 16);
+                    } else {
+                        unsigned a = __float_as_uint(y[2 * h].get(c)), b = __float_as_uint(y[2 * h + 1].get(c));
 #pragma unroll
-                    for (int s = 0; s < P; ++s) {
-                        w[s][h] = pack_hi(a, b);
-                        if (s + 1 < P) {
-                            // what the cut left; of an infinity nothing (inf - inf would be NaN), of a NaN a NaN
-                            const float fa = __uint_as_float(a), fb = __uint_as_float(b);
-                            const float ra = fa - __uint_as_float(a & 0xffff0000u), rb = fb - __uint_as_float(b & 0xffff0000u);
-                            a = __builtin_isinf(fa) ? 0u : __float_as_uint(ra);
-                            b = __builtin_isinf(fb) ? 0u : __float_as_uint(rb);
+                        for (int s = 0; s < P; ++s) {
+                            w[s][h] = pack_hi(a, b);
+                            if (s + 1 < P) {
+                                const float fa = __uint_as_float(a), fb = __uint_as_float(b);
+                                const float ra = fa - __uint_as_float(a & 0xffff0000u), rb = fb - __uint_as_float(b & 0xffff0000u);
+                                a = (decltype(special_)::value && __builtin_isinf(fa)) ? 0u : __float_as_uint(ra);
+                                b = (decltype(special_)::value && __builtin_isinf(fb)) ? 0u : __float_as_uint(rb);
+                            }
                         }
                     }
                 }
-            }
 #pragma unroll
-            for (int s = 0; s < P; ++s) Y[s * (W8_SLAB / 8) + c * 32] = w[s];
-        }
+                for (int s = 0; s < P; ++s) Y[s * (W8_SLAB / 8) + c * 32] = w[s];
+            }
+        };
+        if (P > 1 && inf_seen) cut(std::true_type{});
+        else cut(std::false_type{});
         // kept values: codes of a row share a scale within the four columns
         unsigned v0[8], v1[8];
 #pragma unroll
@@ -319,11 +348,10 @@ rows8_wgrad_kernel(Wgrad8 p) {
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[a][b][q] = 0.f;
-    if (r_begin < r_end) fetch(r_begin);
-    for (long long r = r_begin; r < r_end; r += W8_R) {
-        stage(r);
+    auto step = [&](Rows& d, int r) __attribute__((always_inline)) {
+        stage(d, r);
         __syncthreads();
-        if (r + W8_R < r_end) fetch(r + W8_R);
+        if (r + 2 * W8_R < r_end) fetch(d, r + 2 * W8_R);    // two steps ahead
         const u32x4* Y = reinterpret_cast<const u32x4*>(lds);
         const u32x4* X = reinterpret_cast<const u32x4*>(lds + P * W8_SLAB);
 #pragma unroll
@@ -344,6 +372,12 @@ rows8_wgrad_kernel(Wgrad8 p) {
                     for (int b = 0; b < 2; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ya[c][a], xb[b], acc[a][b], 0, 0, 0);
         }
         __syncthreads();
+    };
+    if (r_begin < r_end) fetch(rows[0], r_begin);
+    if (r_begin + W8_R < r_end) fetch(rows[1], r_begin + W8_R);
+    for (int r = r_begin; r < r_end; r += 2 * W8_R) {
+        step(rows[0], r);
+        if (r + W8_R < r_end) step(rows[1], r + W8_R);
     }
 
     float* dw = p.dw + (p.splits > 1 ? (size_t)split * p.n * p.k : 0);
@@ -467,7 +501,7 @@ size_t jm_rows8_wgrad_workspace_bytes(int m, int n, int k) {
 
 int jm_rows8_linear_wgrad(int m, int n, int k, int type, const void* dy, long long lddy, const unsigned char* codes, int ldc, const unsigned char* exps,
                           float* dw, long long lddw, float* dbias, void* ws, size_t ws_bytes, jm_stream_t stream) {
-    JM_REQUIRE(m >= 0 && n > 0 && k > 0 && type >= JM_F32 && type <= JM_F16 && dw, "rows8_linear_wgrad: m %d, n %d, k %d, type %d", m, n, k, type);
+    JM_REQUIRE(m >= 0 && m <= R8_MAX_ROWS && n > 0 && k > 0 && type >= JM_F32 && type <= JM_F16 && dw, "rows8_linear_wgrad: m %d, n %d, k %d, type %d", m, n, k, type);
     JM_REQUIRE(lddy >= n && ldc >= k && ldc % 16 == 0 && lddw >= k, "rows8_linear_wgrad: lddy %lld, ldc %d, lddw %lld for n %d, k %d", lddy, ldc, lddw, n, k);
     JM_REQUIRE(m == 0 || (dy && codes && exps && ((uintptr_t)codes & 15) == 0), "rows8_linear_wgrad: NULL or unaligned buffers");
     const int splits = m > 0 ? wgrad8_splits(m, n, k) : 1;
@@ -485,9 +519,9 @@ int jm_rows8_linear_wgrad(int m, int n, int k, int type, const void* dy, long lo
     const long long wgs = (long long)divup(n, W8_T) * divup(k, W8_T) * (divup(splits, 8) * 8);
     JM_REQUIRE(wgs <= 0x7fffffffll, "rows8_linear_wgrad: n %d, k %d", n, k);
     const dim3 grid((unsigned)wgs), block(256);
-    if (type == JM_F32) hipLaunchKernelGGL((rows8_wgrad_kernel<JM_F32>), grid, block, 0, s, p);
-    else if (type == JM_BF16) hipLaunchKernelGGL((rows8_wgrad_kernel<JM_BF16>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((rows8_wgrad_kernel<JM_F16>), grid, block, 0, s, p);
+    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, p); };
+    if (m >= 8 && n >= 4) run(type == JM_F32 ? rows8_wgrad_kernel<JM_F32, false> : (type == JM_BF16 ? rows8_wgrad_kernel<JM_BF16, false> : rows8_wgrad_kernel<JM_F16, false>));
+    else run(type == JM_F32 ? rows8_wgrad_kernel<JM_F32, true> : (type == JM_BF16 ? rows8_wgrad_kernel<JM_BF16, true> : rows8_wgrad_kernel<JM_F16, true>));
     if (splits > 1) {
         const long long items = (long long)n * k + (dbias ? n : 0);
         hipLaunchKernelGGL(rows8_wgrad_reduce_kernel, dim3((unsigned)((items + 63) / 64)), block, 0, s, n, k, splits, (const float*)ws,
