@@ -158,10 +158,10 @@ rows8_relu_mask_kernel(long long items, int c, int groups, const float* dy, int 
 // 4 i + q of a tile sits in slot 32 q + i: writes and reads of a wave are contiguous.  Four waves of 64 x 64 (2 x 2 products of
 // 32 x 32 x 16), two workgroups a CU: one stores while the other multiplies.
 // The splits' partial tiles are added in split order by the second kernel (no float atomics: the same bits every time).
-constexpr int W8_T = 128, W8_R = 64, W8_SLAB = W8_R * W8_T;          // (elements of one operand piece in LDS)
+constexpr int W8_SLAB = 8192;          // elements of one operand piece of a step: 64 rows x 128 columns or 128 x 64
 
 struct Wgrad8 {
-    int m, n, k, splits, rows_per;       // rows_per: rows of a split, a multiple of W8_R
+    int m, n, k, splits, rows_per;       // rows_per: rows of a split, a multiple of a step's
     const void* dy; long long lddy;
     const unsigned char* codes; int ldc; const unsigned char* exps; int blocks;
     float *dw, *db;                      // (splits, n, k) and (splits, n) partials, or the results when splits == 1
@@ -202,10 +202,11 @@ template <> struct Quad<JM_F16> : Quad16<JM_F16> {};
 // the upper halves of two words as one: (hi half of a) | (hi half of b) << 16
 __device__ __forceinline__ unsigned pack_hi(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-template <int TY, bool SMALL>
+template <int TY, bool SMALL, int W8_T>
 __global__ void __launch_bounds__(256, 2)
 rows8_wgrad_kernel(Wgrad8 p) {
     typedef typename Elem<TY>::T T;
+    constexpr int W8_R = W8_SLAB / W8_T, G = W8_T / 4, BL = W8_T / 64;          // rows of a step; column groups; 32-wide blocks of a wave a side
     constexpr int P = TY == JM_F32 ? 3 : (TY == JM_F16 ? 2 : 1);                  // pieces of a gradient
     typedef __bf16 frag_t __attribute__((ext_vector_type(8)));
     typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -220,7 +221,7 @@ rows8_wgrad_kernel(Wgrad8 p) {
     const int r_begin = min((long long)split * p.rows_per, (long long)p.m), r_end = min(p.m, r_begin + p.rows_per);
 
     // fetch: rows 8 oct .. + 7 of the 64, columns 4 l .. + 3 of both tiles
-    const int l = lane & 31, oct = wave * 2 + (lane >> 5);
+    const int l = tid % G, oct = tid / G;
     const int cy = n0 + 4 * l, cx = min(k0 + 4 * l, p.ldc - 4);
     const int ylast = p.n - 4;
     const int ysh = (!SMALL && cy < p.n) ? max(0, cy - ylast) : 0;
@@ -313,7 +314,7 @@ rows8_wgrad_kernel(Wgrad8 p) {
                     }
                 }
 #pragma unroll
-                for (int s = 0; s < P; ++s) Y[s * (W8_SLAB / 8) + c * 32] = w[s];
+                for (int s = 0; s < P; ++s) Y[s * (W8_SLAB / 8) + c * G] = w[s];
             }
         };
         if (P > 1 && inf_seen) cut(std::true_type{});
@@ -337,15 +338,15 @@ rows8_wgrad_kernel(Wgrad8 p) {
             w2[h] = __builtin_amdgcn_perm(v1[2 * h + 1], v1[2 * h], 0x05040100u);
             w3[h] = pack_hi(v1[2 * h], v1[2 * h + 1]);
         }
-        X[0] = w0; X[32] = w1; X[64] = w2; X[96] = w3;
+        X[0] = w0; X[G] = w1; X[2 * G] = w2; X[3 * G] = w3;
     };
 
     const int wn = wave >> 1, wk = wave & 1, lr = lane & 31, lk = lane >> 5;
-    f32x16 acc[2][2];
+    f32x16 acc[BL][BL];
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < BL; ++a)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < BL; ++b)
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[a][b][q] = 0.f;
     auto step = [&](Rows& d, int r) __attribute__((always_inline)) {
@@ -357,19 +358,19 @@ rows8_wgrad_kernel(Wgrad8 p) {
 #pragma unroll
         for (int s = 0; s < W8_R / 16; ++s) {
             const int at = (2 * s + lk) * W8_T + lr;
-            frag_t xb[2], ya[P][2];
+            frag_t xb[BL], ya[P][BL];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) xb[b] = __builtin_bit_cast(frag_t, X[at + (2 * wk + b) * 32]);
+            for (int b = 0; b < BL; ++b) xb[b] = __builtin_bit_cast(frag_t, X[at + (BL * wk + b) * 32]);
 #pragma unroll
             for (int c = 0; c < P; ++c)
 #pragma unroll
-                for (int a = 0; a < 2; ++a) ya[c][a] = __builtin_bit_cast(frag_t, Y[c * (W8_SLAB / 8) + at + (2 * wn + a) * 32]);
+                for (int a = 0; a < BL; ++a) ya[c][a] = __builtin_bit_cast(frag_t, Y[c * (W8_SLAB / 8) + at + (BL * wn + a) * 32]);
 #pragma unroll
             for (int c = P - 1; c >= 0; --c)
 #pragma unroll
-                for (int a = 0; a < 2; ++a)
+                for (int a = 0; a < BL; ++a)
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ya[c][a], xb[b], acc[a][b], 0, 0, 0);
+                    for (int b = 0; b < BL; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ya[c][a], xb[b], acc[a][b], 0, 0, 0);
         }
         __syncthreads();
     };
@@ -381,25 +382,27 @@ rows8_wgrad_kernel(Wgrad8 p) {
     }
 
     float* dw = p.dw + (p.splits > 1 ? (size_t)split * p.n * p.k : 0);
-    const int k = k0 + 4 * lr + 2 * wk;
+    auto column = [&](int slot) { return 4 * (slot % G) + slot / G; };
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < BL; ++a)
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-            const int n = n0 + 4 * ((q & 3) + 8 * (q >> 2) + 4 * lk) + 2 * wn + a;
+            const int n = n0 + column((BL * wn + a) * 32 + (q & 3) + 8 * (q >> 2) + 4 * lk);
             if (n < p.n) {
-                float* d = dw + (size_t)n * p.lddw + k;
-                if (k < p.k) d[0] = acc[a][0][q];
-                if (k + 1 < p.k) d[1] = acc[a][1][q];
+#pragma unroll
+                for (int b = 0; b < BL; ++b) {
+                    const int k = k0 + column((BL * wk + b) * 32 + lr);
+                    if (k < p.k) dw[(size_t)n * p.lddw + k] = acc[a][b][q];
+                }
             }
         }
-    if (do_bias) {                                           // the eight row groups' sums, in order
+    if (do_bias) {                                           // the row groups' sums, in order
         f32x4* red = reinterpret_cast<f32x4*>(lds);
-        red[oct * 32 + l] = f32x4{bs[0], bs[1], bs[2], bs[3]};
+        red[oct * G + l] = f32x4{bs[0], bs[1], bs[2], bs[3]};
         __syncthreads();
-        if (tid < 32) {
+        if (tid < G) {
             f32x4 s = red[tid];
-            for (int o = 1; o < 8; ++o) s += red[o * 32 + tid];
+            for (int o = 1; o < 256 / G; ++o) s += red[o * G + tid];
             float* db = p.db + (p.splits > 1 ? (size_t)split * p.n : 0);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
@@ -408,42 +411,56 @@ rows8_wgrad_kernel(Wgrad8 p) {
     }
 }
 
-// out = the sum of the splits' partials: items 0 .. n k - 1 are dW, then n of db.  A workgroup takes 64 items; its four waves sum every
-// fourth split (four chains each: the loads of consecutive splits are in flight together) and are added in wave order.
-__global__ void __launch_bounds__(256)
+// out = the sum of the splits' partials: items 0 .. n k - 1 are dW, then n of db.  A workgroup takes 32 items (a cache line of every
+// partial); its 16 groups of 32 lanes sum every 16th split on four chains, the groups are added in order through LDS.
+__global__ void __launch_bounds__(512)
 rows8_wgrad_reduce_kernel(int n, int k, int splits, const float* __restrict__ part_w, const float* __restrict__ part_b, float* __restrict__ dw,
                           long long lddw, float* __restrict__ db) {
-    __shared__ float red[4][64];
+    __shared__ float red[16][32];
     const long long nk = (long long)n * k;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long i = blockIdx.x * 64ll + lane;
+    const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
+    const long long i = blockIdx.x * 32ll + lane;
     const bool w = i < nk, ok = i < nk + (db ? n : 0);
     const float* src = w ? part_w + i : part_b + (ok ? i - nk : 0);
     const size_t step = w ? (size_t)nk : (size_t)n;
     float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
     if (ok) {
-        int t = wave;
-        for (; t + 12 < splits; t += 16) {
-            s0 += src[(size_t)t * step];       s1 += src[(size_t)(t + 4) * step];
-            s2 += src[(size_t)(t + 8) * step]; s3 += src[(size_t)(t + 12) * step];
+        int t = grp;
+        for (; t + 48 < splits; t += 64) {
+            s0 += src[(size_t)t * step];        s1 += src[(size_t)(t + 16) * step];
+            s2 += src[(size_t)(t + 32) * step]; s3 += src[(size_t)(t + 48) * step];
         }
-        for (; t < splits; t += 4) s0 += src[(size_t)t * step];
+        for (; t < splits; t += 16) s0 += src[(size_t)t * step];
     }
-    red[wave][lane] = (s0 + s1) + (s2 + s3);
+    red[grp][lane] = (s0 + s1) + (s2 + s3);
     __syncthreads();
-    if (wave > 0 || !ok) return;
-    const float s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+    if (grp > 0 || !ok) return;
+    float s = red[0][lane];
+#pragma unroll
+    for (int g = 1; g < 16; ++g) s += red[g][lane];
     if (w) dw[(i / k) * lddw + i % k] = s;
     else db[i - nk] = s;
 }
 
-// splits of the rows: two workgroups for every CU, at least 128 rows (two steps) each
-static int wgrad8_splits(int m, int n, int k) {
-    const long long tiles = (long long)divup(n, W8_T) * divup(k, W8_T);
-    long long s = (512 + tiles - 1) / tiles;
-    const int cap = imax(1, m / 128);
-    if (s > cap) s = cap;
-    return (int)s;
+// Tiles of 128 x 128 halve what is read from the L2 and feed the matrix pipe best, but there have to be enough of them: with at least 4096
+// (tile, 64 rows) steps and both sides wider than 64 (65536 x 256 x 256: 47 us against 52; 16384 x 1024 x 1024: 144 against 338); 64 x 64
+// otherwise (65536 x 64 x 64: 13 us against 18; 4096 x 512 x 512: 26 against 33).  Splits: up to two workgroups a CU; what a split saves
+// in steps (about 1.5 us each where the CU has nothing else to do) is weighed against the partials it writes and the second kernel reads.
+struct Wgrad8Plan { int tile, splits; };
+static Wgrad8Plan wgrad8_plan(int m, int n, int k) {
+    Wgrad8Plan p;
+    const bool wide = n > 64 && k > 64 && (long long)divup(n, 128) * divup(k, 128) * (m / 64) >= 4096;
+    p.tile = wide ? 128 : 64;
+    const int steps = imax(1, m / (W8_SLAB / p.tile));
+    const long long tiles = (long long)divup(n, p.tile) * divup(k, p.tile);
+    p.splits = 1;
+    float best = 1.5f * (float)steps;
+    for (long long s = 512 / tiles; s > 1; s /= 2) {
+        const int t = (int)(s > 256 ? 256 : (s > steps ? steps : s));
+        const float us = 1.5f * (float)divup(steps, t) + 3.f + 2.f * (float)t * (float)n * (float)k * 1e-6f;
+        if (t > 1 && us < best) { best = us; p.splits = t; }
+    }
+    return p;
 }
 
 }  // namespace jm
@@ -495,7 +512,7 @@ int jm_rows8_relu_mask(int m, int c, const float* dy, int ldd, const unsigned ch
 
 size_t jm_rows8_wgrad_workspace_bytes(int m, int n, int k) {
     if (m <= 0 || n <= 0 || k <= 0) return 0;
-    const size_t s = (size_t)wgrad8_splits(m, n, k);
+    const size_t s = (size_t)wgrad8_plan(m, n, k).splits;
     return s > 1 ? s * ((size_t)n * (size_t)k + (size_t)n) * sizeof(float) : 0;
 }
 
@@ -504,27 +521,34 @@ int jm_rows8_linear_wgrad(int m, int n, int k, int type, const void* dy, long lo
     JM_REQUIRE(m >= 0 && m <= R8_MAX_ROWS && n > 0 && k > 0 && type >= JM_F32 && type <= JM_F16 && dw, "rows8_linear_wgrad: m %d, n %d, k %d, type %d", m, n, k, type);
     JM_REQUIRE(lddy >= n && ldc >= k && ldc % 16 == 0 && lddw >= k, "rows8_linear_wgrad: lddy %lld, ldc %d, lddw %lld for n %d, k %d", lddy, ldc, lddw, n, k);
     JM_REQUIRE(m == 0 || (dy && codes && exps && ((uintptr_t)codes & 15) == 0), "rows8_linear_wgrad: NULL or unaligned buffers");
-    const int splits = m > 0 ? wgrad8_splits(m, n, k) : 1;
+    const Wgrad8Plan plan = wgrad8_plan(m, n, k);
+    const int splits = plan.splits, step = W8_SLAB / plan.tile;
     if (splits > 1 && (!ws || ws_bytes < jm_rows8_wgrad_workspace_bytes(m, n, k))) {
         set_error("rows8_linear_wgrad: workspace of %zu bytes, need %zu", ws_bytes, jm_rows8_wgrad_workspace_bytes(m, n, k));
         return JM_EWORKSPACE;
     }
     hipStream_t s = (hipStream_t)stream;
     Wgrad8 p{};
-    p.m = m; p.n = n; p.k = k; p.splits = splits; p.rows_per = m > 0 ? ((m - 1) / splits / W8_R + 1) * W8_R : W8_R;
+    p.m = m; p.n = n; p.k = k; p.splits = splits; p.rows_per = m > 0 ? ((m - 1) / splits / step + 1) * step : step;
     p.dy = dy; p.lddy = lddy; p.codes = codes; p.ldc = ldc; p.exps = exps; p.blocks = divup(k, R8_BLOCK);
     float* part_b = (float*)ws + (size_t)splits * n * k;
     if (splits > 1) { p.dw = (float*)ws; p.lddw = k; p.db = dbias ? part_b : nullptr; }
     else { p.dw = dw; p.lddw = lddw; p.db = dbias; }
-    const long long wgs = (long long)divup(n, W8_T) * divup(k, W8_T) * (divup(splits, 8) * 8);
+    const long long wgs = (long long)divup(n, plan.tile) * divup(k, plan.tile) * (divup(splits, 8) * 8);
     JM_REQUIRE(wgs <= 0x7fffffffll, "rows8_linear_wgrad: n %d, k %d", n, k);
     const dim3 grid((unsigned)wgs), block(256);
     auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, p); };
-    if (m >= 8 && n >= 4) run(type == JM_F32 ? rows8_wgrad_kernel<JM_F32, false> : (type == JM_BF16 ? rows8_wgrad_kernel<JM_BF16, false> : rows8_wgrad_kernel<JM_F16, false>));
-    else run(type == JM_F32 ? rows8_wgrad_kernel<JM_F32, true> : (type == JM_BF16 ? rows8_wgrad_kernel<JM_BF16, true> : rows8_wgrad_kernel<JM_F16, true>));
+    auto pick = [&](auto small_, auto tile_) {
+        constexpr bool S = decltype(small_)::value;
+        constexpr int W = decltype(tile_)::value;
+        run(type == JM_F32 ? rows8_wgrad_kernel<JM_F32, S, W> : (type == JM_BF16 ? rows8_wgrad_kernel<JM_BF16, S, W> : rows8_wgrad_kernel<JM_F16, S, W>));
+    };
+    if (m < 8 || n < 4) pick(std::true_type{}, std::integral_constant<int, 64>{});
+    else if (plan.tile == 64) pick(std::false_type{}, std::integral_constant<int, 64>{});
+    else pick(std::false_type{}, std::integral_constant<int, 128>{});
     if (splits > 1) {
         const long long items = (long long)n * k + (dbias ? n : 0);
-        hipLaunchKernelGGL(rows8_wgrad_reduce_kernel, dim3((unsigned)((items + 63) / 64)), block, 0, s, n, k, splits, (const float*)ws,
+        hipLaunchKernelGGL(rows8_wgrad_reduce_kernel, dim3((unsigned)((items + 31) / 32)), dim3(512), 0, s, n, k, splits, (const float*)ws,
                            (const float*)part_b, dw, lddw, dbias);
     }
     return check_launch("rows8_linear_wgrad");
