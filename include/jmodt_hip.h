@@ -794,20 +794,23 @@ int jm_fold_bn_multi_grad(int n, const float* const* dwf, const float* const* w,
 #define JM_BF16 1
 #define JM_F16 2
 /* x (m, c), rows ldx apart -> e4m3 codes (m, c) in rows of ldc bytes (a multiple of 16, >= c; the bytes behind c are written as zero up to
- * the next multiple of 16) and one scale byte per 32 channels, exps (m, ceil(c / 32)).  Per block: amax = the largest finite |x|, 2^e the
+ * the next multiple of 16) and one scale byte per row and 32 channels, exps (ceil(c / 32), m) with
+ * block rows of lde bytes (a multiple of 16, >= m).  Per block: amax = the largest finite |x|, 2^e the
  * smallest power of two with amax <= 448 2^e and e >= -100 (amax = 0: e = -100), byte = e + 127, code = x / 2^e to the nearest e4m3
  * value, ties to even; a value that is not zero never becomes zero (it takes the smallest code of its sign), one that is not finite
- * becomes NaN.  codes: 16-byte aligned; x: aligned to its element. */
-int jm_rows8_pack(int m, int c, int type, const void* x, long long ldx, unsigned char* codes, int ldc, unsigned char* exps, jm_stream_t stream);
+ * becomes NaN.  codes, exps: 16-byte aligned; x: aligned to its element. */
+int jm_rows8_pack(int m, int c, int type, const void* x, long long ldx, unsigned char* codes, int ldc, unsigned char* exps, int lde,
+                  jm_stream_t stream);
 /* the values that the codes stand for, rounded once to the type (float32 and bfloat16 hold them exactly) */
-int jm_rows8_restore(int m, int c, int type, const unsigned char* codes, int ldc, const unsigned char* exps, void* out, long long ldo, jm_stream_t stream);
+int jm_rows8_restore(int m, int c, int type, const unsigned char* codes, int ldc, const unsigned char* exps, int lde, void* out, long long ldo,
+                     jm_stream_t stream);
 /* out (m, c) = (kept value > 0) ? dy : 0: the gradient through a ReLU whose output was kept; out may be dy */
 int jm_rows8_relu_mask(int m, int c, const float* dy, int ldd, const unsigned char* codes, int ldc, float* out, int ldo, jm_stream_t stream);
 /* dw (n, k) = dy (m, n)^T X (m, k) with X kept (codes, exps), dbias (n) = column sums of dy (NULL: skipped).  Sums in float32, in a
- * fixed order.  ws: >= jm_rows8_wgrad_workspace_bytes, 16-byte aligned. */
+ * fixed order; lddy <= 2^22.  ws: >= jm_rows8_wgrad_workspace_bytes, 16-byte aligned. */
 size_t jm_rows8_wgrad_workspace_bytes(int m, int n, int k);
 int jm_rows8_linear_wgrad(int m, int n, int k, int type, const void* dy, long long lddy, const unsigned char* codes, int ldc, const unsigned char* exps,
-                          float* dw, long long lddw, float* dbias, void* ws, size_t ws_bytes, jm_stream_t stream);
+                          int lde, float* dw, long long lddw, float* dbias, void* ws, size_t ws_bytes, jm_stream_t stream);
 
 /* ------------------------------------------------------------------ low-rank adapters (csrc/adapters.hip) -------- */
 #define JM_ADAPTER_MAX_RANK 128
@@ -825,7 +828,7 @@ int jm_adapter_forward(int m, int k, int n, int rank, int adapters, int type, co
  * type, or NULL with the kept form (codes, exps) of jm_rows8_pack.  ws: 16-byte aligned. */
 size_t jm_adapter_grad_workspace_bytes(int m, int k, int n, int rank, int adapters, int type);
 int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const void* dy, long long lddy, const void* x, long long ldx,
-                    const unsigned char* codes, int ldc, const unsigned char* exps, const float* t, const void* a, const void* b, const float* scales,
+                    const unsigned char* codes, int ldc, const unsigned char* exps, int lde, const float* t, const void* a, const void* b, const float* scales,
                     const int* plan, const void* base, long long ldb, void* dx, long long lddx, void* da, void* db, void* ws, size_t ws_bytes,
                     jm_stream_t stream);
 

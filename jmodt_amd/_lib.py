@@ -222,16 +222,16 @@ SIGNATURES = {
     "jm_fold_bn_multi": (_I, [_I, _P, _P, _P, _P, _P, _P, _P]),
     "jm_fold_bn_multi_grad": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "jm_rows_sigmoid": (_I, [_I, _P, _I, _P, _P]),
-    "jm_rows8_pack": (_I, [_I, _I, _I, _P, _L, _P, _I, _P, _P]),
-    "jm_rows8_restore": (_I, [_I, _I, _I, _P, _I, _P, _P, _L, _P]),
+    "jm_rows8_pack": (_I, [_I, _I, _I, _P, _L, _P, _I, _P, _I, _P]),
+    "jm_rows8_restore": (_I, [_I, _I, _I, _P, _I, _P, _I, _P, _L, _P]),
     "jm_rows8_relu_mask": (_I, [_I, _I, _P, _I, _P, _I, _P, _I, _P]),
     "jm_rows8_wgrad_workspace_bytes": (_Z, [_I, _I, _I]),
-    "jm_rows8_linear_wgrad": (_I, [_I, _I, _I, _I, _P, _L, _P, _I, _P, _P, _L, _P, _P, _Z, _P]),
+    "jm_rows8_linear_wgrad": (_I, [_I, _I, _I, _I, _P, _L, _P, _I, _P, _I, _P, _L, _P, _P, _Z, _P]),
     "jm_adapter_plan_elems": (_Z, [_I, _I]),
     "jm_adapter_plan": (_I, [_I, _I, _P, _P, _P]),
     "jm_adapter_forward": (_I, [_I] * 6 + [_P, _L, _P, _P, _P, _P, _P, _L, _P, _L, _P, _P]),
     "jm_adapter_grad_workspace_bytes": (_Z, [_I] * 6),
-    "jm_adapter_grad": (_I, [_I] * 6 + [_P, _L, _P, _L, _P, _I, _P, _P, _P, _P, _P, _P, _P, _L, _P, _L, _P, _P, _P, _Z, _P]),
+    "jm_adapter_grad": (_I, [_I] * 6 + [_P, _L, _P, _L, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _L, _P, _L, _P, _P, _P, _Z, _P]),
     "jm_rows_gate_backward": (_I, [_I, _I, _I, _P, _I, _P, _I, _P, _P, _I, _P, _P, _P, _I, _P]),
 }
 

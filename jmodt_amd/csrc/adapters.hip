@@ -475,7 +475,7 @@ struct AdaptGrad {
     int m, k, n, rank, adapters;
     const int* plan; size_t o_order, o_chunks, o_chunk_first;
     const void* x; long long ldx;
-    const unsigned char* codes; int ldc; const unsigned char* exps; int blocks;      // x kept in 8 bits (x NULL)
+    const unsigned char* codes; int ldc; const unsigned char* exps; int lde;      // x kept in 8 bits (x NULL)
     const void* dy; long long lddy;
     const float *t, *u;                  // (m, rank)
     const float* scales;
@@ -488,7 +488,7 @@ template <int TY, bool KEPT>
 __device__ __forceinline__ f32x4 grad_load4(const AdaptGrad& p, const void* src, long long ld, size_t row, int c, int width) {
     f32x4 v;
     if (KEPT) {
-        const float s = __uint_as_float((unsigned)p.exps[row * p.blocks + min(c, width - 1) / 32] << 23);       // scale bytes: 27 .. 247
+        const float s = __uint_as_float((unsigned)p.exps[(size_t)(min(c, width - 1) / 32) * p.lde + row] << 23);       // scale bytes: 27 .. 247
         unsigned w = 0;
         if (c < width) w = *reinterpret_cast<const unsigned*>(p.codes + row * p.ldc + c);
         const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
@@ -719,12 +719,12 @@ size_t jm_adapter_grad_workspace_bytes(int m, int k, int n, int rank, int adapte
 }
 
 int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const void* dy, long long lddy, const void* x, long long ldx,
-                    const unsigned char* codes, int ldc, const unsigned char* exps, const float* t, const void* a, const void* b, const float* scales,
+                    const unsigned char* codes, int ldc, const unsigned char* exps, int lde, const float* t, const void* a, const void* b, const float* scales,
                     const int* plan, const void* base, long long ldb, void* dx, long long lddx, void* da, void* db, void* ws, size_t ws_bytes,
                     jm_stream_t stream) {
     if (int e = adapter_check("adapter_grad", m, k, n, rank, adapters, type)) return e;
     JM_REQUIRE(lddy >= n && lddx >= k && (!base || ldb >= k), "adapter_grad: lddy %lld, ldb %lld, lddx %lld for k %d, n %d", lddy, ldb, lddx, k, n);
-    JM_REQUIRE(x ? ldx >= k : (m == 0 || (codes && exps && ldc >= k && ldc % 16 == 0 && ((uintptr_t)codes & 15) == 0)),
+    JM_REQUIRE(x ? ldx >= k : (m == 0 || (codes && exps && ldc >= k && ldc % 16 == 0 && lde >= m && lde % 16 == 0 && (((uintptr_t)codes | (uintptr_t)exps) & 15) == 0)),
                "adapter_grad: x or its kept rows are needed (ldx %lld, ldc %d, k %d)", ldx, ldc, k);
     JM_REQUIRE(a && b && scales && plan && da && db && (m == 0 || (dy && t && dx)), "adapter_grad: NULL buffers");
     const GradLayout gl = grad_layout(m, k, n, rank, adapters, type);
@@ -737,7 +737,7 @@ int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const
     char* w = (char*)ws;
     AdaptGrad q{};
     q.m = m; q.k = k; q.n = n; q.rank = rank; q.adapters = adapters; q.plan = plan; q.o_order = l.order; q.o_chunks = l.chunks;
-    q.o_chunk_first = l.chunk_first; q.x = x; q.ldx = ldx; q.codes = codes; q.ldc = ldc; q.exps = exps; q.blocks = divup(k, 32);
+    q.o_chunk_first = l.chunk_first; q.x = x; q.ldx = ldx; q.codes = codes; q.ldc = ldc; q.exps = exps; q.lde = lde;
     q.dy = dy; q.lddy = lddy; q.t = t; q.u = (const float*)(w + gl.u); q.scales = scales; q.part = (float*)(w + gl.part); q.da = da; q.db = db;
     if (m > 0) {
         const dim3 gt((unsigned)((divup(k, 32) + divup(n, 32)) * divup(rank, 32)), (unsigned)adapters);

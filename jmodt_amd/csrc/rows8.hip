@@ -4,6 +4,7 @@
 // Format.  A row tensor X (m, c) is kept as e4m3 codes (m, ldc) plus one scale byte per 32 consecutive channels of a row:
 //     amax  = the largest finite |x| of the block;  2^e = the smallest power of two with amax <= 448 2^e, e >= -100 (empty block: -100)
 //     code  = x / 2^e rounded to the nearest e4m3 value, ties to even;  scale byte = e + 127
+// (the scale bytes of one block of channels lie together, (blocks, lde >= m): the scales of many rows are one load for the weight gradient)
 // with two exceptions: a value that is not zero never becomes zero (it takes the smallest code of its sign, 2^-9 2^e, so that the sign
 // pattern — a ReLU's mask — survives), and a value that is not finite becomes the NaN code (e4m3 has no infinity).
 // Why e4m3 with power-of-two scales: the division is exact, so the codes are a defined rounding of the input (half a step, 2^-4
@@ -18,6 +19,7 @@ namespace jm {
 
 constexpr int R8_BLOCK = 32;         // channels per scale
 constexpr int R8_MAX_ROWS = 1 << 30;        // (row counters of the weight gradient are 32 bits wide)
+constexpr long long R8_MAX_LD = 1 << 22;      // (128 rows of it are addressed by 32-bit offsets there)
 constexpr int R8_EMIN = -100;        // least scale exponent: 2^e and the smallest code 2^(e - 9) stay normal in float32 and bfloat16
 
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }      // -126 <= e <= 127
@@ -33,7 +35,7 @@ __device__ __forceinline__ int r8_exponent(unsigned amax_bits) {
 // by memory.  Threads walk (row, 8 channels) in memory order.
 template <int TY>
 __global__ void __launch_bounds__(256)
-rows8_pack_kernel(long long items, int c, int groups, const typename Elem<TY>::T* __restrict__ x, long long ldx, unsigned char* __restrict__ codes,
+rows8_pack_kernel(int lde, long long items, int c, int groups, const typename Elem<TY>::T* __restrict__ x, long long ldx, unsigned char* __restrict__ codes,
                   int ldc, unsigned char* __restrict__ exps) {
     typedef typename Elem<TY>::V8 V8;
     for (long long it = blockIdx.x * 256ll + threadIdx.x; it < items; it += gridDim.x * 256ll) {
@@ -82,7 +84,7 @@ rows8_pack_kernel(long long items, int c, int groups, const typename Elem<TY>::T
             w[h] = u;
         }
         if (grp * 8 < ldc) *reinterpret_cast<uint2*>(codes + row * ldc + grp * 8) = make_uint2(w[0], w[1]);
-        if ((grp & 3) == 0) exps[row * (groups >> 2) + (grp >> 2)] = (unsigned char)(e2 + 127);
+        if ((grp & 3) == 0) exps[(size_t)(grp >> 2) * lde + row] = (unsigned char)(e2 + 127);
     }
 }
 
@@ -94,11 +96,10 @@ __device__ __forceinline__ void r8_decode4(unsigned w, float scale, float (&v)[4
 
 template <int TY>
 __global__ void __launch_bounds__(256)
-rows8_restore_kernel(long long items, int c, int groups, const unsigned char* __restrict__ codes, int ldc, const unsigned char* __restrict__ exps,
+rows8_restore_kernel(int lde, long long items, int c, int groups, const unsigned char* __restrict__ codes, int ldc, const unsigned char* __restrict__ exps,
                      typename Elem<TY>::T* __restrict__ out, long long ldo) {
     typedef typename Elem<TY>::T T;
     typedef typename Elem<TY>::V8 V8;
-    const int blocks = (c + R8_BLOCK - 1) / R8_BLOCK;
     for (long long it = blockIdx.x * 256ll + threadIdx.x; it < items; it += gridDim.x * 256ll) {
         long long row;
         int grp;
@@ -110,7 +111,7 @@ rows8_restore_kernel(long long items, int c, int groups, const unsigned char* __
             grp = (int)(it - row * groups);
         }
         const uint2 w = *reinterpret_cast<const uint2*>(codes + row * ldc + grp * 8);
-        const float scale = exp2i((int)exps[row * blocks + (grp >> 2)] - 127);
+        const float scale = exp2i((int)exps[(size_t)(grp >> 2) * lde + row] - 127);
         float v[8];
         r8_decode4(w.x, scale, *reinterpret_cast<float (*)[4]>(&v[0]));
         r8_decode4(w.y, scale, *reinterpret_cast<float (*)[4]>(&v[4]));
@@ -152,18 +153,23 @@ rows8_relu_mask_kernel(long long items, int c, int groups, const float* dy, int 
 // bfloat16 value of one — so every product is exact and only the float32 additions round, as on the float32 pipe, at a third of sixteen
 // times its rate.
 //
-// Workgroup = a 128 x 128 tile of dW over one split of the rows, 64 rows at a time.  A thread fetches 8 rows x 4 columns of both
-// operands (the next 64 rows' while this one's are multiplied), cuts and converts them, and stores 8 rows of one column as 16 bytes: the
-// contraction index becomes the fast one on the way into LDS, and a matrix operand (8 rows of a column) is one 16-byte read.  In LDS column
-// 4 i + q of a tile sits in slot 32 q + i: writes and reads of a wave are contiguous.  Four waves of 64 x 64 (2 x 2 products of
-// 32 x 32 x 16), two workgroups a CU: one stores while the other multiplies.
-// The splits' partial tiles are added in split order by the second kernel (no float atomics: the same bits every time).
+// Workgroup = a 128 x 128 (64 x 64) tile of dW over one split of the rows, 64 (128) rows a step.  A thread fetches 8 rows x 4 columns of both
+// operands, cuts and converts them, and stores 8 rows of one column as 16 bytes: the contraction index becomes the fast one on the way
+// into LDS, and a matrix operand (8 rows of a column) is one 16-byte read.  In LDS column 4 i + q of a tile sits in slot (T / 4) q + i:
+// writes and reads of a wave are contiguous.
+// Two groups of four waves take the steps in turn: while one cuts and stores its step (about 250 vector instructions a wave in float32),
+// the other multiplies its own (48 matrix instructions of 32 x 32 x 16 a wave) and asks for its next rows between them; their sums are
+// added through LDS at the end, so a CU writes one partial tile.  The splits' partials are added in split order by the second kernel (no
+// float atomics: the same bits every time).
+// Measured (float32 / bfloat16 gradients, both kernels): 65536 x 256 x 256 39 / 27 us, 131072 x 512 x 512 230 / 103 us — 0.9 and 0.67
+// PFLOP/s on the bf16 pipe, where a library product of 8192^3 reaches 1.2; 512 x 512 x 512 9 / 7 us.  Bound by the two phases' own latencies
+// (LDS, barrier) more than by any one unit: the matrix pipe is busy half of the time in float32.
 constexpr int W8_SLAB = 8192;          // elements of one operand piece of a step: 64 rows x 128 columns or 128 x 64
 
 struct Wgrad8 {
     int m, n, k, splits, rows_per;       // rows_per: rows of a split, a multiple of a step's
     const void* dy; long long lddy;
-    const unsigned char* codes; int ldc; const unsigned char* exps; int blocks;
+    const unsigned char* codes; int ldc; const unsigned char* exps; int lde, blocks;
     float *dw, *db;                      // (splits, n, k) and (splits, n) partials, or the results when splits == 1
     long long lddw;
 };
@@ -184,13 +190,17 @@ template <> struct Quad<JM_F32> {
     __device__ __forceinline__ float get(int q) const { return v[q]; }
 };
 template <int TY> struct Quad16 {
-    unsigned long long v;
-    __device__ __forceinline__ void load(const typename Elem<TY>::T* p) { __builtin_memcpy(&v, p, 8); }
-    __device__ __forceinline__ void shift(int n) { v >>= 16 * n; }
-    __device__ __forceinline__ void zero() { v = 0; }
-    __device__ __forceinline__ unsigned bits(int q) const { return (unsigned)(v >> (16 * q)) & 0xffffu; }
+    unsigned v[2];
+    __device__ __forceinline__ void load(const typename Elem<TY>::T* p) { __builtin_memcpy(v, p, 8); }
+    __device__ __forceinline__ void shift(int n) {
+        if (n & 1) { v[0] = (v[0] >> 16) | (v[1] << 16); v[1] >>= 16; }
+        if (n & 2) v[0] = v[1];
+    }
+    __device__ __forceinline__ void zero() { v[0] = v[1] = 0u; }
+    template <typename V2> __device__ __forceinline__ void set(const V2& w) { v[0] = w[0]; v[1] = w[1]; }
+    __device__ __forceinline__ unsigned word(int q) const { return v[q >> 1]; }
     __device__ __forceinline__ float get(int q) const {
-        const unsigned short h = (unsigned short)bits(q);
+        const unsigned short h = (unsigned short)(v[q >> 1] >> (16 * (q & 1)));
         typename Elem<TY>::T t;
         __builtin_memcpy(&t, &h, 2);
         return (float)t;
@@ -201,22 +211,26 @@ template <> struct Quad<JM_F16> : Quad16<JM_F16> {};
 
 // the upper halves of two words as one: (hi half of a) | (hi half of b) << 16
 __device__ __forceinline__ unsigned pack_hi(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+__device__ __forceinline__ unsigned pack_lo(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 
 template <int TY, bool SMALL, int W8_T>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(512, 1)
 rows8_wgrad_kernel(Wgrad8 p) {
     typedef typename Elem<TY>::T T;
     constexpr int W8_R = W8_SLAB / W8_T, G = W8_T / 4, BL = W8_T / 64;          // rows of a step; column groups; 32-wide blocks of a wave a side
     constexpr int P = TY == JM_F32 ? 3 : (TY == JM_F16 ? 2 : 1);                  // pieces of a gradient
     typedef __bf16 frag_t __attribute__((ext_vector_type(8)));
     typedef float f32x16 __attribute__((ext_vector_type(16)));
-    __shared__ __attribute__((aligned(16))) unsigned short lds[(P + 1) * W8_SLAB];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    // workgroups are dealt to the 8 XCDs in turn: the tiles of one split, which read the same rows, stay on one of them
-    const int tk = (p.k + W8_T - 1) / W8_T, tiles = ((p.n + W8_T - 1) / W8_T) * tk;
-    const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
-    const int split = (local / tiles) * 8 + xcd, tile = local % tiles;
-    if (split >= p.splits) return;
+    extern __shared__ __attribute__((aligned(16))) unsigned short lds_all[];
+    constexpr int BUF = (P + 1) * W8_SLAB;                   // one step's operands; two buffers
+    const int grp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int tid = threadIdx.x & 255, lane = tid & 63, wave = tid >> 6;
+    // workgroups are dealt to the 8 XCDs in turn: each XCD takes an eighth of the (split, tile) list, so that the tiles of one split, which
+    // read the same rows, share an L2
+    const int tk = (p.k + W8_T - 1) / W8_T, tiles = ((p.n + W8_T - 1) / W8_T) * tk, total = tiles * p.splits;
+    const int item = (int)(blockIdx.x & 7) * ((total + 7) / 8) + (int)(blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= (total + 7) / 8 || item >= total) return;
+    const int split = item / tiles, tile = item % tiles;
     const int n0 = (tile / tk) * W8_T, k0 = (tile % tk) * W8_T;
     const int r_begin = min((long long)split * p.rows_per, (long long)p.m), r_end = min(p.m, r_begin + p.rows_per);
 
@@ -226,116 +240,119 @@ rows8_wgrad_kernel(Wgrad8 p) {
     const int ylast = p.n - 4;
     const int ysh = (!SMALL && cy < p.n) ? max(0, cy - ylast) : 0;
     const bool ragged = !SMALL && (p.n & 3) != 0 && n0 + W8_T > p.n;
-    const T* dyp = (const T*)p.dy + (SMALL ? 0 : min(cy, ylast));
-    const unsigned char* xp = p.codes + cx;
-    const unsigned char* ep = p.exps + min(cx / R8_BLOCK, p.blocks - 1);
+    const int ycol = min(cy, max(ylast, 0));
     struct Rows {
         Quad<TY> y[8];
-        unsigned x[8], e[8];
+        unsigned x[8];
+        unsigned long long e;                                // the rows' scales
     };
-    Rows rows[2];
-    // the last octet of the matrix is read from row m - 8 on: rows before its own first one count as zeros (stage)
-    auto first_row = [&](int r) { return SMALL ? r + 8 * oct : min(r + 8 * oct, p.m - 8); };
-    auto fetch = [&](Rows& d, int r) __attribute__((always_inline)) {
-        const int at = first_row(r);
-        const T* py = dyp + (long long)at * p.lddy;
-        const unsigned char* px = xp + (long long)at * p.ldc;
-        const unsigned char* pe = ep + (long long)at * p.blocks;
+    Rows rows;
+    const unsigned char* const ep = p.exps + (size_t)min(cx / R8_BLOCK, p.blocks - 1) * p.lde;
+    const unsigned yo = ((unsigned)(8 * oct) * (unsigned)p.lddy + (unsigned)ycol) * (unsigned)sizeof(T), xo = (unsigned)(8 * oct) * (unsigned)p.ldc + (unsigned)cx;
+    // rows q0 .. q1 - 1 of the lane's eight of the step at row r; rows behind the split are read as zeros (bounds of the buffers)
+    auto fetch = [&](Rows& d, int r, int q0, int q1) __attribute__((always_inline)) {
+        const int left = min(W8_R, r_end - r);
+        if (q0 == 0) d.e = *reinterpret_cast<const unsigned long long*>(ep + min(r + 8 * oct, p.lde - 8));
+        const unsigned char* xr = p.codes + (long long)r * p.ldc;
+        const auto xbuf = __builtin_amdgcn_make_buffer_rsrc((void*)xr, 0, (unsigned)left * (unsigned)p.ldc, 0x00020000);
+        const T* yr = (const T*)p.dy + (long long)r * p.lddy;
+        const auto ybuf = __builtin_amdgcn_make_buffer_rsrc((void*)yr, 0, ((unsigned)(left - 1) * (unsigned)p.lddy + (unsigned)p.n) * (unsigned)sizeof(T), 0x00020000);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-            if constexpr (SMALL) {                           // fewer than 8 rows or 4 columns: element by element
-                const long long row = min(at + q, p.m - 1);
+            if (q < q0 || q >= q1) continue;
+            d.x[q] = __builtin_amdgcn_raw_buffer_load_b32(xbuf, xo, q * p.ldc, 0);
+            if constexpr (SMALL) {                           // fewer than 4 columns, or rows that are not aligned to 4 bytes
+                const T* dy = yr + (long long)min(8 * oct + q, left - 1) * p.lddy;
                 T t[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) t[c] = dyp[row * p.lddy + min(cy + c, p.n - 1)];
+                for (int c = 0; c < 4; ++c) t[c] = dy[min(cy + c, p.n - 1)];
                 d.y[q].load(t);
-                d.x[q] = *reinterpret_cast<const unsigned*>(xp + row * p.ldc);
-                d.e[q] = ep[row * p.blocks];
+                if (8 * oct + q >= left) d.y[q].zero();
+            } else if constexpr (TY == JM_F32) {
+                d.y[q].v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ybuf, yo, q * (int)p.lddy * 4, 0));
             } else {
-                d.y[q].load(py + q * p.lddy);
-                d.x[q] = *reinterpret_cast<const unsigned*>(px + q * (long long)p.ldc);
-                d.e[q] = pe[q * (long long)p.blocks];
+                d.y[q].set(__builtin_amdgcn_raw_buffer_load_b64(ybuf, yo, q * (int)p.lddy * 2, 0));
             }
         }
     };
     float bs[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool do_bias = p.db != nullptr && k0 == 0;
-    auto stage = [&](Rows& d, int r) __attribute__((always_inline)) {
+    // the bias sums of a split's rows: step i is the tile column i mod tk's, so that no workgroup has all of them (one split: its first column's)
+    const int kt = tile % tk;
+    const bool do_bias = p.db != nullptr && (p.splits > 1 || kt == 0);
+    // before a step's rows are staged: rows behind the split count as zeros on both sides, columns that straddle the edge, the bias sums.
+    // Returns whether the wave holds an infinity (looked for once: its rest must be nothing, inf - inf would be NaN; a NaN's rest is a NaN).
+    auto prepare = [&](Rows& d, int r) __attribute__((always_inline)) -> bool {
         Quad<TY>(&y)[8] = d.y;
-        unsigned(&x)[8] = d.x;
-        unsigned(&e)[8] = d.e;
-        if (r + W8_R > r_end) {                              // rows outside this step's own count as zeros on both sides
-            const int at = first_row(r);
+        if (r + W8_R > r_end) {                              // (the scales behind the matrix are not written: any power of two for the zeros there)
 #pragma unroll
             for (int q = 0; q < 8; ++q)
-                if (at + q >= r_end || at + q < r + 8 * oct) { y[q].zero(); x[q] = 0u; e[q] = 127u; }
+                if (r + 8 * oct + q >= r_end) d.e = (d.e & ~(0xffull << (8 * q))) | (127ull << (8 * q));
         }
         if (ragged) {
 #pragma unroll
             for (int q = 0; q < 8; ++q) y[q].shift(ysh);
         }
-        if (do_bias) {
+        if (do_bias && (p.splits == 1 || ((r - r_begin) / W8_R) % tk == kt)) {
 #pragma unroll
             for (int q = 0; q < 8; ++q)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) bs[c] += y[q].get(c);
         }
-        // an infinity leaves no rest (inf - inf would be NaN), a NaN leaves a NaN: looked for once for the whole wave
-        bool inf_seen = false;
         if constexpr (P > 1) {
-            float z = 0.f;
+            float top = 0.f;
 #pragma unroll
             for (int q = 0; q < 8; ++q)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) z = __builtin_fmaf(y[q].get(c), 0.f, z);
-            inf_seen = __ballot(z != z) != 0ull;
+                for (int c = 0; c < 4; c += 2) asm("v_max3_f32 %0, |%1|, |%2|, %0" : "+v"(top) : "v"(y[q].get(c)), "v"(y[q].get(c + 1)));
+            return __ballot(top == __builtin_inff()) != 0ull;
         }
+        return false;
+    };
+    auto stage = [&](auto special_, Rows& d, unsigned short* lds) __attribute__((always_inline)) {
+        Quad<TY>(&y)[8] = d.y;
         u32x4* Y = reinterpret_cast<u32x4*>(lds) + oct * W8_T + l;          // 16 bytes = 8 rows of a slot
-        auto cut = [&](auto special_) __attribute__((always_inline)) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                u32x4 w[P];
+        for (int c = 0; c < 4; ++c) {
+            u32x4 w[P];
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    if constexpr (TY == JM_BF16) {
-                        w[0][h] = y[2 * h].bits(c) | (y[2 * h + 1].bits(c) << 16);
-                    } else {
-                        unsigned a = __float_as_uint(y[2 * h].get(c)), b = __float_as_uint(y[2 * h + 1].get(c));
+            for (int h = 0; h < 4; ++h) {
+                if constexpr (TY == JM_BF16) {
+                    w[0][h] = (c & 1) ? pack_hi(y[2 * h].word(c), y[2 * h + 1].word(c)) : pack_lo(y[2 * h].word(c), y[2 * h + 1].word(c));
+                } else {
+                    unsigned a = __float_as_uint(y[2 * h].get(c)), b = __float_as_uint(y[2 * h + 1].get(c));
 #pragma unroll
-                        for (int s = 0; s < P; ++s) {
-                            w[s][h] = pack_hi(a, b);
-                            if (s + 1 < P) {
-                                const float fa = __uint_as_float(a), fb = __uint_as_float(b);
-                                const float ra = fa - __uint_as_float(a & 0xffff0000u), rb = fb - __uint_as_float(b & 0xffff0000u);
-                                a = (decltype(special_)::value && __builtin_isinf(fa)) ? 0u : __float_as_uint(ra);
-                                b = (decltype(special_)::value && __builtin_isinf(fb)) ? 0u : __float_as_uint(rb);
-                            }
+                    for (int s = 0; s < P; ++s) {
+                        w[s][h] = pack_hi(a, b);
+                        if (s + 1 < P) {
+                            const float fa = __uint_as_float(a), fb = __uint_as_float(b);
+                            const float ra = fa - __uint_as_float(a & 0xffff0000u), rb = fb - __uint_as_float(b & 0xffff0000u);
+                            a = (decltype(special_)::value && __builtin_isinf(fa)) ? 0u : __float_as_uint(ra);
+                            b = (decltype(special_)::value && __builtin_isinf(fb)) ? 0u : __float_as_uint(rb);
                         }
                     }
                 }
-#pragma unroll
-                for (int s = 0; s < P; ++s) Y[s * (W8_SLAB / 8) + c * G] = w[s];
             }
-        };
-        if (P > 1 && inf_seen) cut(std::true_type{});
-        else cut(std::false_type{});
+#pragma unroll
+            for (int s = 0; s < P; ++s) Y[s * (W8_SLAB / 8) + c * G] = w[s];
+        }
         // kept values: codes of a row share a scale within the four columns
         unsigned v0[8], v1[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-            const float sc = __uint_as_float(e[q] << 23);
-            const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x[q], sc, false);
-            const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x[q], sc, true);
+            const unsigned half = (unsigned)(d.e >> (q < 4 ? 0 : 32));
+            const float sc = __uint_as_float(((half >> (8 * (q & 3))) & 0xffu) << 23);
+            const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)d.x[q], sc, false);
+            const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)d.x[q], sc, true);
             __builtin_memcpy(&v0[q], &lo, 4);
             __builtin_memcpy(&v1[q], &hi, 4);
         }
-        u32x4* X = reinterpret_cast<u32x4*>(lds + P * W8_SLAB) + oct * W8_T + l;
+        u32x4* X = Y + P * (W8_SLAB / 8);
         u32x4 w0, w1, w2, w3;
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
-            w0[h] = __builtin_amdgcn_perm(v0[2 * h + 1], v0[2 * h], 0x05040100u);
+            w0[h] = pack_lo(v0[2 * h], v0[2 * h + 1]);
             w1[h] = pack_hi(v0[2 * h], v0[2 * h + 1]);
-            w2[h] = __builtin_amdgcn_perm(v1[2 * h + 1], v1[2 * h], 0x05040100u);
+            w2[h] = pack_lo(v1[2 * h], v1[2 * h + 1]);
             w3[h] = pack_hi(v1[2 * h], v1[2 * h + 1]);
         }
         X[0] = w0; X[G] = w1; X[2 * G] = w2; X[3 * G] = w3;
@@ -349,61 +366,113 @@ rows8_wgrad_kernel(Wgrad8 p) {
         for (int b = 0; b < BL; ++b)
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[a][b][q] = 0.f;
-    auto step = [&](Rows& d, int r) __attribute__((always_inline)) {
-        stage(d, r);
-        __syncthreads();
-        if (r + 2 * W8_R < r_end) fetch(d, r + 2 * W8_R);    // two steps ahead
+    // one step's products, and the next one's rows asked for in between: a load waits for its turn at the L1's port, and a wave that waits
+    // there in one go leaves the matrix pipe idle
+    auto multiply = [&](unsigned short* lds, Rows& d, int r) __attribute__((always_inline)) {
         const u32x4* Y = reinterpret_cast<const u32x4*>(lds);
-        const u32x4* X = reinterpret_cast<const u32x4*>(lds + P * W8_SLAB);
-#pragma unroll
-        for (int s = 0; s < W8_R / 16; ++s) {
+        const u32x4* X = Y + P * (W8_SLAB / 8);
+        frag_t xb[2][BL], ya[2][P][BL];
+        auto read = [&](int s) __attribute__((always_inline)) {
             const int at = (2 * s + lk) * W8_T + lr;
-            frag_t xb[BL], ya[P][BL];
 #pragma unroll
-            for (int b = 0; b < BL; ++b) xb[b] = __builtin_bit_cast(frag_t, X[at + (BL * wk + b) * 32]);
+            for (int b = 0; b < BL; ++b) xb[s & 1][b] = __builtin_bit_cast(frag_t, X[at + (BL * wk + b) * 32]);
 #pragma unroll
-            for (int c = 0; c < P; ++c)
+            for (int c = P - 1; c >= 0; --c)
 #pragma unroll
-                for (int a = 0; a < BL; ++a) ya[c][a] = __builtin_bit_cast(frag_t, Y[c * (W8_SLAB / 8) + at + (BL * wn + a) * 32]);
+                for (int a = 0; a < BL; ++a) ya[s & 1][c][a] = __builtin_bit_cast(frag_t, Y[c * (W8_SLAB / 8) + at + (BL * wn + a) * 32]);
+        };
+        constexpr int KS = W8_R / 16;
+        const bool more = r < r_end;
+        read(0);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if (s + 1 < KS) read(s + 1);                     // the next operands are on their way while these are multiplied
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int c = P - 1; c >= 0; --c)
 #pragma unroll
                 for (int a = 0; a < BL; ++a)
 #pragma unroll
-                    for (int b = 0; b < BL; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ya[c][a], xb[b], acc[a][b], 0, 0, 0);
+                    for (int b = 0; b < BL; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ya[s & 1][c][a], xb[s & 1][b], acc[a][b], 0, 0, 0);
+            if (more) fetch(d, r, s * 8 / KS, (s + 1) * 8 / KS);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        __syncthreads();
     };
-    if (r_begin < r_end) fetch(rows[0], r_begin);
-    if (r_begin + W8_R < r_end) fetch(rows[1], r_begin + W8_R);
-    for (int r = r_begin; r < r_end; r += 2 * W8_R) {
-        step(rows[0], r);
-        if (r + W8_R < r_end) step(rows[1], r + W8_R);
+    const int steps = (r_end - r_begin + W8_R - 1) / W8_R;
+    // group g takes the steps g, g + 2, ...; the barriers put one group's staging beside the other's products (2 turns + 1 for both;
+    // lds_barrier leaves loads in flight)
+    const int first = r_begin + grp * W8_R, turns = (steps + 1) / 2;
+    unsigned short* lds = lds_all + grp * BUF;
+    if (first < r_end) fetch(rows, first, 0, 8);
+    auto put = [&](int r) __attribute__((always_inline)) {
+        if (r >= r_end) return;
+        if (prepare(rows, r)) stage(std::true_type{}, rows, lds);
+        else stage(std::false_type{}, rows, lds);
+    };
+    if (grp == 0) {
+        put(first);
+        lds_barrier();
+        for (int t = 0; t < turns; ++t) {
+            multiply(lds, rows, first + (t + 1) * 2 * W8_R);
+            lds_barrier();
+            put(first + (t + 1) * 2 * W8_R);
+            lds_barrier();
+        }
+    } else {
+        lds_barrier();
+        for (int t = 0; t < turns; ++t) {
+            const int r = first + t * 2 * W8_R;
+            put(r);
+            lds_barrier();
+            if (r < r_end) multiply(lds, rows, r + 2 * W8_R);
+            lds_barrier();
+        }
+    }
+    float* red = reinterpret_cast<float*>(lds_all);
+    if (grp == 1) {
+#pragma unroll
+        for (int a = 0; a < BL; ++a)
+#pragma unroll
+            for (int b = 0; b < BL; ++b)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) red[((a * BL + b) * 16 + q) * 256 + tid] = acc[a][b][q];
+    }
+    __syncthreads();
+    if (grp == 0) {
+#pragma unroll
+        for (int a = 0; a < BL; ++a)
+#pragma unroll
+            for (int b = 0; b < BL; ++b)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) acc[a][b][q] += red[((a * BL + b) * 16 + q) * 256 + tid];
     }
 
     float* dw = p.dw + (p.splits > 1 ? (size_t)split * p.n * p.k : 0);
     auto column = [&](int slot) { return 4 * (slot % G) + slot / G; };
+    if (grp == 0) {
 #pragma unroll
-    for (int a = 0; a < BL; ++a)
+        for (int a = 0; a < BL; ++a)
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-            const int n = n0 + column((BL * wn + a) * 32 + (q & 3) + 8 * (q >> 2) + 4 * lk);
-            if (n < p.n) {
+            for (int q = 0; q < 16; ++q) {
+                const int n = n0 + column((BL * wn + a) * 32 + (q & 3) + 8 * (q >> 2) + 4 * lk);
+                if (n < p.n) {
 #pragma unroll
-                for (int b = 0; b < BL; ++b) {
-                    const int k = k0 + column((BL * wk + b) * 32 + lr);
-                    if (k < p.k) dw[(size_t)n * p.lddw + k] = acc[a][b][q];
+                    for (int b = 0; b < BL; ++b) {
+                        const int k = k0 + column((BL * wk + b) * 32 + lr);
+                        if (k < p.k) dw[(size_t)n * p.lddw + k] = acc[a][b][q];
+                    }
                 }
             }
-        }
+    }
     if (do_bias) {                                           // the row groups' sums, in order
-        f32x4* red = reinterpret_cast<f32x4*>(lds);
-        red[oct * G + l] = f32x4{bs[0], bs[1], bs[2], bs[3]};
+        f32x4* sums = reinterpret_cast<f32x4*>(lds_all);
         __syncthreads();
-        if (tid < G) {
-            f32x4 s = red[tid];
-            for (int o = 1; o < 256 / G; ++o) s += red[o * G + tid];
-            float* db = p.db + (p.splits > 1 ? (size_t)split * p.n : 0);
+        sums[threadIdx.x] = f32x4{bs[0], bs[1], bs[2], bs[3]};       // (oct * G + l)
+        __syncthreads();
+        if (grp == 0 && tid < G) {
+            f32x4 s = sums[tid];
+            for (int o = 1; o < 512 / G; ++o) s += sums[o * G + tid];
+            float* db = p.db + (p.splits > 1 ? ((size_t)split * tk + kt) * p.n : 0);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
                 if (n0 + 4 * tid + c < p.n) db[n0 + 4 * tid + c] = s[c];
@@ -414,7 +483,7 @@ rows8_wgrad_kernel(Wgrad8 p) {
 // out = the sum of the splits' partials: items 0 .. n k - 1 are dW, then n of db.  A workgroup takes 32 items (a cache line of every
 // partial); its 16 groups of 32 lanes sum every 16th split on four chains, the groups are added in order through LDS.
 __global__ void __launch_bounds__(512)
-rows8_wgrad_reduce_kernel(int n, int k, int splits, const float* __restrict__ part_w, const float* __restrict__ part_b, float* __restrict__ dw,
+rows8_wgrad_reduce_kernel(int n, int k, int splits_w, int splits_b, const float* __restrict__ part_w, const float* __restrict__ part_b, float* __restrict__ dw,
                           long long lddw, float* __restrict__ db) {
     __shared__ float red[16][32];
     const long long nk = (long long)n * k;
@@ -423,6 +492,7 @@ rows8_wgrad_reduce_kernel(int n, int k, int splits, const float* __restrict__ pa
     const bool w = i < nk, ok = i < nk + (db ? n : 0);
     const float* src = w ? part_w + i : part_b + (ok ? i - nk : 0);
     const size_t step = w ? (size_t)nk : (size_t)n;
+    const int splits = w ? splits_w : splits_b;
     float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
     if (ok) {
         int t = grp;
@@ -443,9 +513,10 @@ rows8_wgrad_reduce_kernel(int n, int k, int splits, const float* __restrict__ pa
 }
 
 // Tiles of 128 x 128 halve what is read from the L2 and feed the matrix pipe best, but there have to be enough of them: with at least 4096
-// (tile, 64 rows) steps and both sides wider than 64 (65536 x 256 x 256: 47 us against 52; 16384 x 1024 x 1024: 144 against 338); 64 x 64
-// otherwise (65536 x 64 x 64: 13 us against 18; 4096 x 512 x 512: 26 against 33).  Splits: up to two workgroups a CU; what a split saves
-// in steps (about 1.5 us each where the CU has nothing else to do) is weighed against the partials it writes and the second kernel reads.
+// (tile, 64 rows) steps and both sides wider than 64 (one form of this kernel, float32: 65536 x 256 x 256 47 us against 52, 16384 x 1024 x
+// 1024 144 against 338); 64 x 64 otherwise (65536 x 64 x 64: 13 us against 18; 4096 x 512 x 512: 26 against 33).  Splits: up to one
+// workgroup a CU; what a split saves in steps (about 1.5 us each where the CU has nothing else to do) is weighed against the partials it
+// writes and the second kernel reads.
 struct Wgrad8Plan { int tile, splits; };
 static Wgrad8Plan wgrad8_plan(int m, int n, int k) {
     Wgrad8Plan p;
@@ -455,7 +526,7 @@ static Wgrad8Plan wgrad8_plan(int m, int n, int k) {
     const long long tiles = (long long)divup(n, p.tile) * divup(k, p.tile);
     p.splits = 1;
     float best = 1.5f * (float)steps;
-    for (long long s = 512 / tiles; s > 1; s /= 2) {
+    for (long long s = 256 / tiles; s > 1; s /= 2) {
         const int t = (int)(s > 256 ? 256 : (s > steps ? steps : s));
         const float us = 1.5f * (float)divup(steps, t) + 3.f + 2.f * (float)t * (float)n * (float)k * 1e-6f;
         if (t > 1 && us < best) { best = us; p.splits = t; }
@@ -469,33 +540,37 @@ using namespace jm;
 
 extern "C" {
 
-int jm_rows8_pack(int m, int c, int type, const void* x, long long ldx, unsigned char* codes, int ldc, unsigned char* exps, jm_stream_t stream) {
+int jm_rows8_pack(int m, int c, int type, const void* x, long long ldx, unsigned char* codes, int ldc, unsigned char* exps, int lde,
+                  jm_stream_t stream) {
     JM_REQUIRE(m >= 0 && c > 0 && type >= JM_F32 && type <= JM_F16, "rows8_pack: m %d, c %d, type %d", m, c, type);
-    JM_REQUIRE(ldc >= c && ldc % 16 == 0 && ldx >= c, "rows8_pack: codes in rows of a multiple of 16 bytes (ldc %d, c %d, ldx %lld)", ldc, c, ldx);
+    JM_REQUIRE(ldc >= c && ldc % 16 == 0 && lde >= m && lde % 16 == 0 && ldx >= c, "rows8_pack: codes and scales in multiples of 16 bytes (ldc %d, c %d, lde %d, m %d, ldx %lld)", ldc,
+               c, lde, m, ldx);
     if (m == 0) return JM_OK;
-    JM_REQUIRE(x && codes && exps && ((uintptr_t)codes & 15) == 0, "rows8_pack: NULL or unaligned buffers");
+    JM_REQUIRE(x && codes && exps && (((uintptr_t)codes | (uintptr_t)exps) & 15) == 0, "rows8_pack: NULL or unaligned buffers");
     const int groups = divup(c, R8_BLOCK) * 4;
     const long long items = (long long)m * groups;
     const dim3 grid((unsigned)grid_for(items, 256, JM_EGRID)), block(256);
     hipStream_t s = (hipStream_t)stream;
-    if (type == JM_F32) hipLaunchKernelGGL((rows8_pack_kernel<JM_F32>), grid, block, 0, s, items, c, groups, (const float*)x, ldx, codes, ldc, exps);
-    else if (type == JM_BF16) hipLaunchKernelGGL((rows8_pack_kernel<JM_BF16>), grid, block, 0, s, items, c, groups, (const __bf16*)x, ldx, codes, ldc, exps);
-    else hipLaunchKernelGGL((rows8_pack_kernel<JM_F16>), grid, block, 0, s, items, c, groups, (const _Float16*)x, ldx, codes, ldc, exps);
+    if (type == JM_F32) hipLaunchKernelGGL((rows8_pack_kernel<JM_F32>), grid, block, 0, s, lde, items, c, groups, (const float*)x, ldx, codes, ldc, exps);
+    else if (type == JM_BF16) hipLaunchKernelGGL((rows8_pack_kernel<JM_BF16>), grid, block, 0, s, lde, items, c, groups, (const __bf16*)x, ldx, codes, ldc, exps);
+    else hipLaunchKernelGGL((rows8_pack_kernel<JM_F16>), grid, block, 0, s, lde, items, c, groups, (const _Float16*)x, ldx, codes, ldc, exps);
     return check_launch("rows8_pack");
 }
 
-int jm_rows8_restore(int m, int c, int type, const unsigned char* codes, int ldc, const unsigned char* exps, void* out, long long ldo, jm_stream_t stream) {
+int jm_rows8_restore(int m, int c, int type, const unsigned char* codes, int ldc, const unsigned char* exps, int lde, void* out, long long ldo,
+                     jm_stream_t stream) {
     JM_REQUIRE(m >= 0 && c > 0 && type >= JM_F32 && type <= JM_F16, "rows8_restore: m %d, c %d, type %d", m, c, type);
-    JM_REQUIRE(ldc >= c && ldc % 16 == 0 && ldo >= c, "rows8_restore: codes in rows of a multiple of 16 bytes (ldc %d, c %d, ldo %lld)", ldc, c, ldo);
+    JM_REQUIRE(ldc >= c && ldc % 16 == 0 && lde >= m && lde % 16 == 0 && ldo >= c, "rows8_restore: codes and scales in multiples of 16 bytes (ldc %d, c %d, lde %d, m %d, ldo %lld)",
+               ldc, c, lde, m, ldo);
     if (m == 0) return JM_OK;
-    JM_REQUIRE(codes && exps && out && ((uintptr_t)codes & 15) == 0, "rows8_restore: NULL or unaligned buffers");
+    JM_REQUIRE(codes && exps && out && (((uintptr_t)codes | (uintptr_t)exps) & 15) == 0, "rows8_restore: NULL or unaligned buffers");
     const int groups = divup(c, 8);
     const long long items = (long long)m * groups;
     const dim3 grid((unsigned)grid_for(items, 256, JM_EGRID)), block(256);
     hipStream_t s = (hipStream_t)stream;
-    if (type == JM_F32) hipLaunchKernelGGL((rows8_restore_kernel<JM_F32>), grid, block, 0, s, items, c, groups, codes, ldc, exps, (float*)out, ldo);
-    else if (type == JM_BF16) hipLaunchKernelGGL((rows8_restore_kernel<JM_BF16>), grid, block, 0, s, items, c, groups, codes, ldc, exps, (__bf16*)out, ldo);
-    else hipLaunchKernelGGL((rows8_restore_kernel<JM_F16>), grid, block, 0, s, items, c, groups, codes, ldc, exps, (_Float16*)out, ldo);
+    if (type == JM_F32) hipLaunchKernelGGL((rows8_restore_kernel<JM_F32>), grid, block, 0, s, lde, items, c, groups, codes, ldc, exps, (float*)out, ldo);
+    else if (type == JM_BF16) hipLaunchKernelGGL((rows8_restore_kernel<JM_BF16>), grid, block, 0, s, lde, items, c, groups, codes, ldc, exps, (__bf16*)out, ldo);
+    else hipLaunchKernelGGL((rows8_restore_kernel<JM_F16>), grid, block, 0, s, lde, items, c, groups, codes, ldc, exps, (_Float16*)out, ldo);
     return check_launch("rows8_restore");
 }
 
@@ -512,15 +587,16 @@ int jm_rows8_relu_mask(int m, int c, const float* dy, int ldd, const unsigned ch
 
 size_t jm_rows8_wgrad_workspace_bytes(int m, int n, int k) {
     if (m <= 0 || n <= 0 || k <= 0) return 0;
-    const size_t s = (size_t)wgrad8_plan(m, n, k).splits;
-    return s > 1 ? s * ((size_t)n * (size_t)k + (size_t)n) * sizeof(float) : 0;
+    const Wgrad8Plan p = wgrad8_plan(m, n, k);               // per split dW, then per split and tile column the bias sums
+    return p.splits > 1 ? (size_t)p.splits * ((size_t)n * (size_t)k + (size_t)divup(k, p.tile) * n) * sizeof(float) : 0;
 }
 
 int jm_rows8_linear_wgrad(int m, int n, int k, int type, const void* dy, long long lddy, const unsigned char* codes, int ldc, const unsigned char* exps,
-                          float* dw, long long lddw, float* dbias, void* ws, size_t ws_bytes, jm_stream_t stream) {
+                          int lde, float* dw, long long lddw, float* dbias, void* ws, size_t ws_bytes, jm_stream_t stream) {
     JM_REQUIRE(m >= 0 && m <= R8_MAX_ROWS && n > 0 && k > 0 && type >= JM_F32 && type <= JM_F16 && dw, "rows8_linear_wgrad: m %d, n %d, k %d, type %d", m, n, k, type);
-    JM_REQUIRE(lddy >= n && ldc >= k && ldc % 16 == 0 && lddw >= k, "rows8_linear_wgrad: lddy %lld, ldc %d, lddw %lld for n %d, k %d", lddy, ldc, lddw, n, k);
-    JM_REQUIRE(m == 0 || (dy && codes && exps && ((uintptr_t)codes & 15) == 0), "rows8_linear_wgrad: NULL or unaligned buffers");
+    JM_REQUIRE(lddy >= n && lddy <= R8_MAX_LD && ldc >= k && ldc <= R8_MAX_LD && ldc % 16 == 0 && lde >= m && lde % 16 == 0 && lddw >= k,
+               "rows8_linear_wgrad: lddy %lld, ldc %d, lde %d, lddw %lld for m %d, n %d, k %d", lddy, ldc, lde, lddw, m, n, k);
+    JM_REQUIRE(m == 0 || (dy && codes && exps && (((uintptr_t)codes | (uintptr_t)exps) & 15) == 0), "rows8_linear_wgrad: NULL or unaligned buffers");
     const Wgrad8Plan plan = wgrad8_plan(m, n, k);
     const int splits = plan.splits, step = W8_SLAB / plan.tile;
     if (splits > 1 && (!ws || ws_bytes < jm_rows8_wgrad_workspace_bytes(m, n, k))) {
@@ -530,25 +606,29 @@ int jm_rows8_linear_wgrad(int m, int n, int k, int type, const void* dy, long lo
     hipStream_t s = (hipStream_t)stream;
     Wgrad8 p{};
     p.m = m; p.n = n; p.k = k; p.splits = splits; p.rows_per = m > 0 ? ((m - 1) / splits / step + 1) * step : step;
-    p.dy = dy; p.lddy = lddy; p.codes = codes; p.ldc = ldc; p.exps = exps; p.blocks = divup(k, R8_BLOCK);
+    p.dy = dy; p.lddy = lddy; p.codes = codes; p.ldc = ldc; p.exps = exps; p.lde = lde; p.blocks = divup(k, R8_BLOCK);
     float* part_b = (float*)ws + (size_t)splits * n * k;
     if (splits > 1) { p.dw = (float*)ws; p.lddw = k; p.db = dbias ? part_b : nullptr; }
     else { p.dw = dw; p.lddw = lddw; p.db = dbias; }
-    const long long wgs = (long long)divup(n, plan.tile) * divup(k, plan.tile) * (divup(splits, 8) * 8);
+    const long long wgs = ((long long)divup(n, plan.tile) * divup(k, plan.tile) * splits + 7) / 8 * 8;
     JM_REQUIRE(wgs <= 0x7fffffffll, "rows8_linear_wgrad: n %d, k %d", n, k);
-    const dim3 grid((unsigned)wgs), block(256);
-    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, p); };
+    const dim3 grid((unsigned)wgs), block(512);
+    const unsigned lds = 2u * (type == JM_F32 ? 4u : (type == JM_F16 ? 3u : 2u)) * W8_SLAB * 2u;
+    auto run = [&](auto kernel) {
+        (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        hipLaunchKernelGGL(kernel, grid, block, lds, s, p);
+    };
     auto pick = [&](auto small_, auto tile_) {
         constexpr bool S = decltype(small_)::value;
         constexpr int W = decltype(tile_)::value;
         run(type == JM_F32 ? rows8_wgrad_kernel<JM_F32, S, W> : (type == JM_BF16 ? rows8_wgrad_kernel<JM_BF16, S, W> : rows8_wgrad_kernel<JM_F16, S, W>));
     };
-    if (m < 8 || n < 4) pick(std::true_type{}, std::integral_constant<int, 64>{});
+    if (n < 4 || (type != JM_F32 && (((uintptr_t)dy & 3) || (lddy & 1)))) pick(std::true_type{}, std::integral_constant<int, 64>{});
     else if (plan.tile == 64) pick(std::false_type{}, std::integral_constant<int, 64>{});
     else pick(std::false_type{}, std::integral_constant<int, 128>{});
     if (splits > 1) {
         const long long items = (long long)n * k + (dbias ? n : 0);
-        hipLaunchKernelGGL(rows8_wgrad_reduce_kernel, dim3((unsigned)((items + 31) / 32)), dim3(512), 0, s, n, k, splits, (const float*)ws,
+        hipLaunchKernelGGL(rows8_wgrad_reduce_kernel, dim3((unsigned)((items + 31) / 32)), dim3(512), 0, s, n, k, splits, splits * divup(k, plan.tile), (const float*)ws,
                            (const float*)part_b, dw, lddw, dbias);
     }
     return check_launch("rows8_linear_wgrad");

@@ -151,7 +151,7 @@ def adapter_grad(dy: torch.Tensor, x: Union[torch.Tensor, Rows8], t: torch.Tenso
     ws = torch.empty(((nbytes + 3) // 4,), dtype=_f32, device=dy.device)
     if not kept and m == 0:
         px = a.data_ptr()          # (an empty tensor has no address; nothing is read)
-    L.check(lib.jm_adapter_grad(m, k, n, rank, count, TYPES[dy.dtype], pdy, ldd, px, max(ldx, k), pc, ldc, pe, t.data_ptr(), a.data_ptr(), b.data_ptr(),
+    L.check(lib.jm_adapter_grad(m, k, n, rank, count, TYPES[dy.dtype], pdy, ldd, px, max(ldx, k), pc, ldc, pe, (m + 15) // 16 * 16, t.data_ptr(), a.data_ptr(), b.data_ptr(),
                                 scales.data_ptr(), plan.data.data_ptr(), pb, ldb, dx.data_ptr(), dx.stride(0) if m > 1 else k, da.data_ptr(), db.data_ptr(),
                                 ws.data_ptr(), nbytes, L.stream_ptr()), "adapter_grad")
     return dx, da, db

@@ -52,9 +52,14 @@ def _matrix(t, name: str, dtype: Optional[torch.dtype] = None) -> Tuple[int, int
     return t.data_ptr(), ld
 
 
+def _exps(m: int, c: int, device) -> torch.Tensor:
+    """(m, blocks of c) scale bytes, column by column in memory"""
+    return torch.empty(((c + BLOCK - 1) // BLOCK, (m + 15) // 16 * 16), dtype=_u8, device=device).t()[:m]
+
+
 class Rows8:
     """A kept row tensor: `codes` (rows, ld) uint8, ld = the channels rounded up to 16, zeros behind the channels; `exps`
-    (rows, ceil(channels / 32)) uint8, a block's scale is 2^(exps - 127); `shape` = (rows, channels)."""
+    (rows, ceil(channels / 32)) uint8, column by column in memory, a column padded to 16 rows; a block's scale is 2^(exps - 127); `shape` = (rows, channels)."""
     __slots__ = ("codes", "exps", "shape")
 
     def __init__(self, codes: torch.Tensor, exps: torch.Tensor, channels: int):
@@ -69,8 +74,10 @@ class Rows8:
                              f"got {tuple(codes.shape)} and {tuple(exps.shape)}")
         if codes.device != exps.device:
             raise RuntimeError(f"codes on {codes.device}, exps on {exps.device}")
-        if not (codes.is_contiguous() and exps.is_contiguous()) or codes.data_ptr() % 16:
-            raise RuntimeError("codes and exps must be contiguous, codes 16-byte aligned")
+        if not codes.is_contiguous() or codes.data_ptr() % 16:
+            raise RuntimeError("codes must be contiguous and 16-byte aligned")
+        if exps.data_ptr() % 16 or (m > 1 and exps.stride(0) != 1) or (exps.shape[1] > 1 and exps.stride(1) != (m + 15) // 16 * 16):
+            raise RuntimeError("exps must be (blocks, rows rounded up to 16) in memory: Rows8.from_codes lays them out")
         self.codes, self.exps, self.shape = codes, exps, (m, channels)
 
     @classmethod
@@ -81,7 +88,9 @@ class Rows8:
         m, c = codes.shape
         padded = torch.zeros((m, (c + 15) // 16 * 16), dtype=_u8, device=codes.device)
         padded[:, :c] = codes
-        return cls(padded, exps.contiguous(), c)
+        columns = _exps(m, c, codes.device)
+        columns.copy_(exps)
+        return cls(padded, columns, c)
 
     @property
     def device(self):
@@ -103,8 +112,8 @@ def checkpoint_rows(x: torch.Tensor) -> Rows8:
     px, ldx = _matrix(x, "x")
     m, c = x.shape
     codes = torch.empty((m, (c + 15) // 16 * 16), dtype=_u8, device=x.device)
-    exps = torch.empty((m, (c + BLOCK - 1) // BLOCK), dtype=_u8, device=x.device)
-    L.check(L.load().jm_rows8_pack(m, c, TYPES[x.dtype], px, ldx, codes.data_ptr(), codes.shape[1], exps.data_ptr(), L.stream_ptr()), "checkpoint_rows")
+    exps = _exps(m, c, x.device)
+    L.check(L.load().jm_rows8_pack(m, c, TYPES[x.dtype], px, ldx, codes.data_ptr(), codes.shape[1], exps.data_ptr(), (m + 15) // 16 * 16, L.stream_ptr()), "checkpoint_rows")
     return Rows8(codes, exps, c)
 
 
@@ -115,7 +124,7 @@ def restore_rows(x8: Rows8, dtype: torch.dtype = _f32) -> torch.Tensor:
         raise TypeError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     m, c = x8.shape
     out = torch.empty((m, c), dtype=dtype, device=x8.device)
-    L.check(L.load().jm_rows8_restore(m, c, TYPES[dtype], x8.codes.data_ptr(), x8.codes.shape[1], x8.exps.data_ptr(), out.data_ptr(), c, L.stream_ptr()),
+    L.check(L.load().jm_rows8_restore(m, c, TYPES[dtype], x8.codes.data_ptr(), x8.codes.shape[1], x8.exps.data_ptr(), (m + 15) // 16 * 16, out.data_ptr(), c, L.stream_ptr()),
             "restore_rows")
     return out
 
@@ -146,7 +155,7 @@ def linear_wgrad8(dy: torch.Tensor, x8: Rows8, want_bias: bool = True) -> Tuple[
     db = torch.empty((n,), dtype=_f32, device=dy.device) if want_bias else None
     nbytes = lib.jm_rows8_wgrad_workspace_bytes(m, n, k)
     ws = torch.empty((nbytes // 4,), dtype=_f32, device=dy.device) if nbytes else None
-    L.check(lib.jm_rows8_linear_wgrad(m, n, k, TYPES[dy.dtype], pdy, ldd, x8.codes.data_ptr(), x8.codes.shape[1], x8.exps.data_ptr(), dw.data_ptr(), k,
+    L.check(lib.jm_rows8_linear_wgrad(m, n, k, TYPES[dy.dtype], pdy, ldd, x8.codes.data_ptr(), x8.codes.shape[1], x8.exps.data_ptr(), (m + 15) // 16 * 16, dw.data_ptr(), k,
                                       db.data_ptr() if want_bias else None, ws.data_ptr() if ws is not None else None, nbytes, L.stream_ptr()),
             "linear_wgrad8")
     return dw, db

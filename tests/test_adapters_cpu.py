@@ -17,7 +17,7 @@ def test_host_tensors_are_refused():
     x = torch.randn(4, 8)
     with pytest.raises(RuntimeError):
         R8.checkpoint_rows(x)
-    k = R8.Rows8(torch.zeros(4, 16, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8), 8)
+    k = R8.Rows8.from_codes(torch.zeros(4, 8, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8))
     assert k.shape == (4, 8) and k.nbytes() == 68
     for call in (lambda: R8.restore_rows(k), lambda: R8.linear_wgrad8(x, k), lambda: R8.relu_mask8(x, k), lambda: AD.AdapterPlan(torch.zeros(4, dtype=torch.int32), 2)):
         with pytest.raises(RuntimeError):
@@ -25,23 +25,23 @@ def test_host_tensors_are_refused():
 
 
 @pytest.mark.parametrize("args", [dict(m=-1), dict(c=0), dict(type=3), dict(ldc=24), dict(ldc=0), dict(ldx=7), dict(x=None), dict(codes=None),
-                                  dict(codes=PTR + 4), dict(exps=None)])
+                                  dict(codes=PTR + 4), dict(exps=None), dict(lde=1), dict(lde=24)])
 def test_pack_refuses(args):
-    a = dict(m=2, c=8, type=0, x=PTR, ldx=8, codes=PTR, ldc=16, exps=PTR)
+    a = dict(m=2, c=8, type=0, x=PTR, ldx=8, codes=PTR, ldc=16, exps=PTR, lde=16)
     a.update(args)
     lib = L.load()
-    assert lib.jm_rows8_pack(a["m"], a["c"], a["type"], a["x"], a["ldx"], a["codes"], a["ldc"], a["exps"], None) == EINVAL
-    assert lib.jm_rows8_restore(a["m"], a["c"], a["type"], a["codes"], a["ldc"], a["exps"], a["x"], a["ldx"], None) == EINVAL
+    assert lib.jm_rows8_pack(a["m"], a["c"], a["type"], a["x"], a["ldx"], a["codes"], a["ldc"], a["exps"], a["lde"], None) == EINVAL
+    assert lib.jm_rows8_restore(a["m"], a["c"], a["type"], a["codes"], a["ldc"], a["exps"], a["lde"], a["x"], a["ldx"], None) == EINVAL
     assert b"rows8" in lib.jm_last_error()
 
 
 @pytest.mark.parametrize("args,code", [(dict(m=-1), EINVAL), (dict(n=0), EINVAL), (dict(k=0), EINVAL), (dict(type=-1), EINVAL), (dict(dw=None), EINVAL),
-                                       (dict(lddy=3), EINVAL), (dict(ldc=40), EINVAL), (dict(lddw=4), EINVAL), (dict(codes=PTR + 8), EINVAL),
+                                       (dict(lddy=3), EINVAL), (dict(ldc=40), EINVAL), (dict(lddw=4), EINVAL), (dict(codes=PTR + 8), EINVAL), (dict(lde=8), EINVAL), (dict(lddy=1 << 23), EINVAL),
                                        (dict(m=100000, ws=None), EWORKSPACE), (dict(m=100000, ws_bytes=8), EWORKSPACE)])
 def test_wgrad_refuses(args, code):
-    a = dict(m=4, n=4, k=8, type=0, dy=PTR, lddy=4, codes=PTR, ldc=16, exps=PTR, dw=PTR, lddw=8, db=PTR, ws=PTR, ws_bytes=0)
+    a = dict(m=4, n=4, k=8, type=0, dy=PTR, lddy=4, codes=PTR, ldc=16, exps=PTR, lde=1 << 20, dw=PTR, lddw=8, db=PTR, ws=PTR, ws_bytes=0)
     a.update(args)
-    assert L.load().jm_rows8_linear_wgrad(a["m"], a["n"], a["k"], a["type"], a["dy"], a["lddy"], a["codes"], a["ldc"], a["exps"], a["dw"], a["lddw"], a["db"],
+    assert L.load().jm_rows8_linear_wgrad(a["m"], a["n"], a["k"], a["type"], a["dy"], a["lddy"], a["codes"], a["ldc"], a["exps"], a["lde"], a["dw"], a["lddw"], a["db"],
                                           a["ws"], a["ws_bytes"], None) == code
 
 
@@ -56,10 +56,10 @@ def test_adapter_forward_refuses(args):
 
 
 @pytest.mark.parametrize("args,code", [(dict(rank=129), EINVAL), (dict(adapters=1024), EINVAL), (dict(lddy=3), EINVAL), (dict(lddx=7), EINVAL), (dict(ldx=7), EINVAL),
-                                       (dict(x=None, codes=None), EINVAL), (dict(x=None, ldc=8), EINVAL), (dict(t=None), EINVAL), (dict(da=None), EINVAL),
+                                       (dict(x=None, codes=None), EINVAL), (dict(x=None, ldc=8), EINVAL), (dict(x=None, lde=1), EINVAL), (dict(t=None), EINVAL), (dict(da=None), EINVAL),
                                        (dict(ws=None), EWORKSPACE), (dict(ws_bytes=16), EWORKSPACE)])
 def test_adapter_grad_refuses(args, code):
-    a = dict(m=2, k=8, n=4, rank=2, adapters=3, type=0, dy=PTR, lddy=4, x=PTR, ldx=8, codes=PTR, ldc=16, exps=PTR, t=PTR, a=PTR, b=PTR, scales=PTR, plan=PTR,
+    a = dict(m=2, k=8, n=4, rank=2, adapters=3, type=0, dy=PTR, lddy=4, x=PTR, ldx=8, codes=PTR, ldc=16, exps=PTR, lde=16, t=PTR, a=PTR, b=PTR, scales=PTR, plan=PTR,
              base=PTR, ldb=8, dx=PTR, lddx=8, da=PTR, db=PTR, ws=PTR, ws_bytes=100)
     a.update(args)
     assert L.load().jm_adapter_grad(*a.values(), None) == code
