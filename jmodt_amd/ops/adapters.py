@@ -43,65 +43,68 @@ def _weights(a, b, scales, plan, dtype, k: int, n: int, m: int):
     if not isinstance(plan, AdapterPlan):
         raise TypeError(f"plan: expected AdapterPlan, got {type(plan).__name__}")
     _on_device(plan.data, "plan")
-    for t, name in ((a, "a"), (b, "b")):
-        _on_device(t, name)
-        if t.dtype != dtype:
-            raise TypeError(f"{name} must be {dtype} like the rows, got {t.dtype}")
-        if t.dim() != 3 or not t.is_contiguous():
-            raise RuntimeError(f"{name} must be a contiguous 3-D tensor, got {tuple(t.shape)}")
-    count, rank = a.shape[0], a.shape[1]
-    if tuple(a.shape) != (count, rank, k) or tuple(b.shape) != (count, n, rank):
+    _on_device(a, "a")
+    _on_device(b, "b")
+    _on_device(scales, "scales")
+    if a.dtype != dtype or b.dtype != dtype:
+        raise TypeError(f"a and b must be {dtype} like the rows, got {a.dtype} and {b.dtype}")
+    if a.dim() != 3 or not a.is_contiguous() or b.dim() != 3 or not b.is_contiguous():
+        raise RuntimeError(f"a and b must be contiguous 3-D tensors, got {tuple(a.shape)} and {tuple(b.shape)}")
+    count, rank, ka = a.shape
+    if ka != k or b.shape != (count, n, rank):
         raise ValueError(f"a {tuple(a.shape)}, b {tuple(b.shape)}: expected (adapters, rank, {k}) and (adapters, {n}, rank)")
     if not 1 <= rank <= MAX_RANK:
         raise ValueError(f"rank {rank}; 1 .. {MAX_RANK} are supported")
-    if plan.adapters != count:
-        raise ValueError(f"a plan of {plan.adapters} adapters for {count}")
-    if plan.rows != m:
-        raise ValueError(f"a plan of {plan.rows} rows for {m}")
-    _on_device(scales, "scales")
-    if scales.dtype != _f32 or tuple(scales.shape) != (count,) or not scales.is_contiguous():
+    if plan.adapters != count or plan.rows != m:
+        raise ValueError(f"a plan of {plan.rows} rows and {plan.adapters} adapters for {m} and {count}")
+    if scales.dtype != _f32 or scales.shape != (count,) or not scales.is_contiguous():
         raise TypeError(f"scales must be a contiguous float32 tensor of ({count},), got {scales.dtype} {tuple(scales.shape)}")
     return rank, count
 
 
-def _span(t: torch.Tensor) -> Tuple[int, int]:
-    p, s = t.data_ptr(), t.element_size()
-    if t.numel() == 0:
-        return p, p
-    return p, p + s * (1 + sum((d - 1) * st for d, st in zip(t.shape, t.stride())))
+def _bytes(t: torch.Tensor) -> int:
+    """from the tensor's first byte to behind its last one"""
+    if t.is_contiguous():
+        return t.numel() * t.element_size()
+    return t.element_size() * (1 + sum((d - 1) * st for d, st in zip(t.shape, t.stride()))) if t.numel() else 0
 
 
-def _disjoint(out: torch.Tensor, other: torch.Tensor, name: str) -> None:
-    """refuses an output that shares elements with an input (columns beside each other in rows of one buffer are fine)"""
-    a0, a1 = _span(out)
-    b0, b1 = _span(other)
-    if a0 >= b1 or b0 >= a1:
+def _disjoint(p: int, size: int, out: torch.Tensor, other: torch.Tensor, name: str) -> None:
+    """refuses an output (`size` bytes at p) that shares elements with an input; columns beside each other in rows of one buffer are fine"""
+    q = other.data_ptr()
+    if q >= p + size or q + _bytes(other) <= p:
         return
-    if out.dim() == 2 and other.dim() == 2 and out.element_size() == other.element_size() and out.shape[0] > 1 and other.shape[0] > 1:
+    if other.dim() == 2 and out.element_size() == other.element_size() and out.shape[0] > 1 and other.shape[0] > 1:
         ld = out.stride(0)
         if ld == other.stride(0):
-            d = ((b0 - a0) // out.element_size()) % ld          # columns from out's first to other's first
+            d = ((q - p) // out.element_size()) % ld          # columns from out's first to other's first
             if d >= out.shape[1] and d + other.shape[1] <= ld:
                 return
     raise RuntimeError(f"out shares memory with {name}")
 
 
 def _result(base, out, m: int, n: int, like: torch.Tensor, others):
-    """(base address, base row stride, out): checks of base / out, out allocated when not given"""
+    """(base address, base row stride, out, its address, its row stride): checks of base / out, out allocated when not given"""
     pb, ldb = None, 0
     if base is not None:
-        pb, ldb = _matrix(base, "base", like.dtype)
-        if tuple(base.shape) != (m, n):
+        mb, nb, pb, ldb = _matrix(base, "base", like.dtype)
+        if mb != m or nb != n:
             raise ValueError(f"base {tuple(base.shape)}: expected ({m}, {n})")
     if out is None:
-        return pb, ldb, torch.empty((m, n), dtype=like.dtype, device=like.device)
-    _matrix(out, "out", like.dtype)
-    if tuple(out.shape) != (m, n):
-        raise ValueError(f"out {tuple(out.shape)}: expected ({m}, {n})")
-    same = base is not None and out.data_ptr() == base.data_ptr() and out.stride() == base.stride()
-    for t, name in others + ([(base, "base")] if base is not None and not same else []):
-        _disjoint(out, t, name)
-    return pb, ldb, out
+        out = torch.empty((m, n), dtype=like.dtype, device=like.device)
+        return pb, ldb, out, out.data_ptr(), n
+    if out is base:
+        po, ldo = pb, ldb
+    else:
+        mo, no, po, ldo = _matrix(out, "out", like.dtype)
+        if mo != m or no != n:
+            raise ValueError(f"out {tuple(out.shape)}: expected ({m}, {n})")
+    size = _bytes(out)
+    if base is not None and not (po == pb and ldo == ldb):
+        _disjoint(po, size, out, base, "base")
+    for t, name in others:
+        _disjoint(po, size, out, t, name)
+    return pb, ldb, out, po, ldo
 
 
 def adapter_forward(base: Optional[torch.Tensor], x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, plan: AdapterPlan,
@@ -109,15 +112,13 @@ def adapter_forward(base: Optional[torch.Tensor], x: torch.Tensor, a: torch.Tens
     """base (M, N) or None (zero), x (M, K), a (adapters, R, K), b (adapters, N, R), scales (adapters,) float32 ->
     out = base + scales[a] B_a (A_a x) row by row; rows without an adapter: base.  out: a tensor to write (base itself: in place),
     else a new one.  want_t: (out, t), t (M, R) float32 = A_a x, zero in rows without an adapter — what `adapter_grad` needs."""
-    px, ldx = _matrix(x, "x")
-    m, k = x.shape
+    m, k, px, ldx = _matrix(x, "x")
     n = b.shape[1] if isinstance(b, torch.Tensor) and b.dim() == 3 else 0
     rank, count = _weights(a, b, scales, plan, x.dtype, k, n, m)
-    pb, ldb, out = _result(base, out, m, n, x, [(x, "x"), (a, "a"), (b, "b"), (scales, "scales")] if out is not None else [])
+    pb, ldb, out, po, ldo = _result(base, out, m, n, x, ((x, "x"), (a, "a"), (b, "b"), (scales, "scales"), (plan.data, "plan")))
     t = torch.empty((m, rank), dtype=_f32, device=x.device) if want_t else None
     L.check(L.load().jm_adapter_forward(m, k, n, rank, count, TYPES[x.dtype], px, ldx, a.data_ptr(), b.data_ptr(), scales.data_ptr(), plan.data.data_ptr(),
-                                        pb, ldb, out.data_ptr(), out.stride(0) if m > 1 else n, t.data_ptr() if want_t else None, L.stream_ptr()),
-            "adapter_forward")
+                                        pb, ldb, po, ldo, t.data_ptr() if want_t else None, L.stream_ptr()), "adapter_forward")
     return (out, t) if want_t else out
 
 
@@ -126,34 +127,30 @@ def adapter_grad(dy: torch.Tensor, x: Union[torch.Tensor, Rows8], t: torch.Tenso
     """the gradients of adapter_forward: dy (M, N), x (M, K) or its kept form, t from the forward ->
     (dx (M, K) = base + scales[a] A_a^T (B_a^T dy), da like a, db like b).  base: the shared projection's data gradient, or None;
     out: a tensor for dx (base itself: in place).  An adapter without rows gets zeros."""
-    pdy, ldd = _matrix(dy, "dy")
-    m, n = dy.shape
-    kept = isinstance(x, Rows8)
-    if kept:
-        _kept(x, "x")
-        px, ldx = None, 0
-        pc, ldc, pe = x.codes.data_ptr(), x.codes.shape[1], x.exps.data_ptr()
+    m, n, pdy, ldd = _matrix(dy, "dy")
+    px, ldx, pc, ldc, pe, lde = None, 0, None, 0, None, 0
+    if isinstance(x, Rows8):
+        mx, k, pc, ldc, pe, lde = _kept(x, "x")
+        source = x.data
     else:
-        px, ldx = _matrix(x, "x", dy.dtype)
-        pc, ldc, pe = None, 0, None
-    if x.shape[0] != m:
-        raise ValueError(f"dy of {m} rows for an input of {x.shape[0]}")
-    k = x.shape[1]
+        mx, k, px, ldx = _matrix(x, "x", dy.dtype)
+        source = x
+        if m == 0:
+            px = a.data_ptr()          # (an empty tensor has no address; nothing is read)
+    if mx != m:
+        raise ValueError(f"dy of {m} rows for an input of {mx}")
     rank, count = _weights(a, b, scales, plan, dy.dtype, k, n, m)
     _on_device(t, "t")
-    if t.dtype != _f32 or tuple(t.shape) != (m, rank) or not t.is_contiguous():
+    if t.dtype != _f32 or t.shape != (m, rank) or not t.is_contiguous():
         raise TypeError(f"t must be a contiguous float32 tensor of ({m}, {rank}), got {t.dtype} {tuple(t.shape)}")
-    others = [] if out is None else [(dy, "dy"), (t, "t"), (a, "a"), (b, "b"), (scales, "scales")] + ([(x.codes, "x"), (x.exps, "x")] if kept else [(x, "x")])
-    pb, ldb, dx = _result(base, out, m, k, dy, others)
+    pb, ldb, dx, po, ldo = _result(base, out, m, k, dy, ((dy, "dy"), (source, "x"), (t, "t"), (a, "a"), (b, "b"), (scales, "scales"), (plan.data, "plan")))
     da, db = torch.empty_like(a), torch.empty_like(b)
     lib = L.load()
-    nbytes = lib.jm_adapter_grad_workspace_bytes(m, k, n, rank, count, TYPES[dy.dtype])
+    kind = TYPES[dy.dtype]
+    nbytes = lib.jm_adapter_grad_workspace_bytes(m, k, n, rank, count, kind)
     ws = torch.empty(((nbytes + 3) // 4,), dtype=_f32, device=dy.device)
-    if not kept and m == 0:
-        px = a.data_ptr()          # (an empty tensor has no address; nothing is read)
-    L.check(lib.jm_adapter_grad(m, k, n, rank, count, TYPES[dy.dtype], pdy, ldd, px, max(ldx, k), pc, ldc, pe, (m + 15) // 16 * 16, t.data_ptr(), a.data_ptr(), b.data_ptr(),
-                                scales.data_ptr(), plan.data.data_ptr(), pb, ldb, dx.data_ptr(), dx.stride(0) if m > 1 else k, da.data_ptr(), db.data_ptr(),
-                                ws.data_ptr(), nbytes, L.stream_ptr()), "adapter_grad")
+    L.check(lib.jm_adapter_grad(m, k, n, rank, count, kind, pdy, ldd, px, ldx, pc, ldc, pe, lde, t.data_ptr(), a.data_ptr(), b.data_ptr(), scales.data_ptr(),
+                                plan.data.data_ptr(), pb, ldb, po, ldo, da.data_ptr(), db.data_ptr(), ws.data_ptr(), nbytes, L.stream_ptr()), "adapter_grad")
     return dx, da, db
 
 
@@ -165,10 +162,10 @@ class _AdapterLinear(Function):
         y = R.linear_forward(x, w, bias)
         a, b = a.contiguous(), b.contiguous()
         y, t = adapter_forward(y, x, a, b, scales, plan, out=y, want_t=True)
-        ctx.plan, ctx.keep, ctx.channels, ctx.has_bias = plan, keep, x.shape[1], bias is not None
+        ctx.plan, ctx.keep, ctx.shape, ctx.has_bias = plan, keep, tuple(x.shape), bias is not None
         if keep:
             x8 = checkpoint_rows(x)
-            ctx.save_for_backward(x8.codes, x8.exps, w, a, b, scales, t)
+            ctx.save_for_backward(x8.data, w, a, b, scales, t)
         else:
             ctx.save_for_backward(x, w, a, b, scales, t)
         return y
@@ -177,7 +174,7 @@ class _AdapterLinear(Function):
     def backward(ctx, dy):
         saved = ctx.saved_tensors
         if ctx.keep:
-            x, (w, a, b, scales, t) = Rows8(saved[0], saved[1], ctx.channels), saved[2:]
+            x, (w, a, b, scales, t) = Rows8(saved[0], *ctx.shape), saved[1:]
         else:
             x, (w, a, b, scales, t) = saved[0], saved[1:]
         if dy.dim() != 2 or dy.stride(1) != 1 or dy.stride(0) % 4 or dy.stride(0) < dy.shape[1] or dy.data_ptr() % 16:

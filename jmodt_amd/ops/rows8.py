@@ -26,13 +26,13 @@ def _on_device(t, name: str) -> None:
         raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a GPU tensor (jmodt_amd has no CPU path); got device {t.device}")
-    if t.device.index != L._current_device():
+    if t.get_device() != L._current_device():
         raise RuntimeError(f"{name} lives on {t.device} but the current device is cuda:{L._current_device()}; "
                            "wrap the call in `with torch.cuda.device(tensor.device):`")
 
 
-def _matrix(t, name: str, dtype: Optional[torch.dtype] = None) -> Tuple[int, int]:
-    """(address, row stride) of a 2-D row tensor: unit column stride, any row stride >= its width, any alignment"""
+def _matrix(t, name: str, dtype: Optional[torch.dtype] = None) -> Tuple[int, int, int, int]:
+    """(rows, channels, address, row stride) of a 2-D row tensor: unit column stride, any row stride >= its width, any alignment"""
     _on_device(t, name)
     if t.dim() != 2:
         raise TypeError(f"{name} must be 2-D (rows, channels), got {tuple(t.shape)}")
@@ -42,6 +42,8 @@ def _matrix(t, name: str, dtype: Optional[torch.dtype] = None) -> Tuple[int, int
     elif t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     m, c = t.shape
+    if t.is_contiguous() and c:
+        return m, c, t.data_ptr(), c
     if c == 0:
         raise ValueError(f"{name} has no channels")
     if c > 1 and t.stride(1) != 1:
@@ -49,113 +51,124 @@ def _matrix(t, name: str, dtype: Optional[torch.dtype] = None) -> Tuple[int, int
     ld = t.stride(0) if m > 1 else c
     if ld < c:
         raise RuntimeError(f"{name}: rows {ld} apart overlap (width {c}); pass a contiguous tensor")
-    return t.data_ptr(), ld
+    return m, c, t.data_ptr(), ld
 
 
-def _exps(m: int, c: int, device) -> torch.Tensor:
-    """(m, blocks of c) scale bytes, column by column in memory"""
-    return torch.empty(((c + BLOCK - 1) // BLOCK, (m + 15) // 16 * 16), dtype=_u8, device=device).t()[:m]
+def _sizes(m: int, c: int) -> Tuple[int, int, int]:
+    """(bytes of a row of codes, blocks of a row, bytes of a block's scale column)"""
+    return (c + 15) & ~15, (c + BLOCK - 1) // BLOCK, (m + 15) & ~15
 
 
 class Rows8:
-    """A kept row tensor: `codes` (rows, ld) uint8, ld = the channels rounded up to 16, zeros behind the channels; `exps`
-    (rows, ceil(channels / 32)) uint8, column by column in memory, a column padded to 16 rows; a block's scale is 2^(exps - 127); `shape` = (rows, channels)."""
-    __slots__ = ("codes", "exps", "shape")
+    """A kept row tensor of `shape` = (rows, channels) in one buffer, `data` (uint8): `codes` (rows, channels rounded up to 16), zeros behind
+    the channels, then `exps`, (rows, ceil(channels / 32)) scale bytes stored column by column, a column padded to 16 rows; a block's scale is
+    2^(exps - 127).  `data` is what an autograd function saves."""
+    __slots__ = ("data", "shape")
 
-    def __init__(self, codes: torch.Tensor, exps: torch.Tensor, channels: int):
-        channels = int(channels)
-        if not (isinstance(codes, torch.Tensor) and isinstance(exps, torch.Tensor)):
-            raise TypeError("codes and exps must be tensors")
-        if codes.dtype != _u8 or exps.dtype != _u8 or codes.dim() != 2 or exps.dim() != 2:
-            raise TypeError("codes and exps must be 2-D uint8 tensors")
-        m, ld = codes.shape
-        if channels <= 0 or ld != (channels + 15) // 16 * 16 or tuple(exps.shape) != (m, (channels + BLOCK - 1) // BLOCK):
-            raise ValueError(f"{channels} channels need codes (m, {(channels + 15) // 16 * 16}) and exps (m, {(channels + BLOCK - 1) // BLOCK}); "
-                             f"got {tuple(codes.shape)} and {tuple(exps.shape)}")
-        if codes.device != exps.device:
-            raise RuntimeError(f"codes on {codes.device}, exps on {exps.device}")
-        if not codes.is_contiguous() or codes.data_ptr() % 16:
-            raise RuntimeError("codes must be contiguous and 16-byte aligned")
-        if exps.data_ptr() % 16 or (m > 1 and exps.stride(0) != 1) or (exps.shape[1] > 1 and exps.stride(1) != (m + 15) // 16 * 16):
-            raise RuntimeError("exps must be (blocks, rows rounded up to 16) in memory: Rows8.from_codes lays them out")
-        self.codes, self.exps, self.shape = codes, exps, (m, channels)
+    def __init__(self, data: torch.Tensor, rows: int, channels: int):
+        rows, channels = int(rows), int(channels)
+        if not isinstance(data, torch.Tensor) or data.dtype != _u8 or data.dim() != 1 or not data.is_contiguous():
+            raise TypeError("data must be a contiguous 1-D uint8 tensor")
+        if rows < 0 or channels <= 0:
+            raise ValueError(f"({rows}, {channels}) rows and channels")
+        ld, nb, mp = _sizes(rows, channels)
+        if data.shape[0] != rows * ld + nb * mp:
+            raise ValueError(f"({rows}, {channels}) takes {rows * ld + nb * mp} bytes, got {data.shape[0]}")
+        if data.data_ptr() % 16:
+            raise RuntimeError("data must be 16-byte aligned")
+        self.data, self.shape = data, (rows, channels)
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, exps: torch.Tensor) -> "Rows8":
-        """from codes (rows, channels) without padding, e.g. read from a file"""
-        if codes.dtype != _u8 or codes.dim() != 2:
-            raise TypeError("codes must be a 2-D uint8 tensor")
+        """from codes (rows, channels) and exps (rows, ceil(channels / 32)), e.g. read from a file"""
+        if codes.dtype != _u8 or codes.dim() != 2 or exps.dtype != _u8 or exps.dim() != 2:
+            raise TypeError("codes and exps must be 2-D uint8 tensors")
         m, c = codes.shape
-        padded = torch.zeros((m, (c + 15) // 16 * 16), dtype=_u8, device=codes.device)
-        padded[:, :c] = codes
-        columns = _exps(m, c, codes.device)
-        columns.copy_(exps)
-        return cls(padded, columns, c)
+        ld, nb, mp = _sizes(m, c)
+        if tuple(exps.shape) != (m, nb) or c == 0:
+            raise ValueError(f"{c} channels need exps of ({m}, {nb}), got {tuple(exps.shape)}")
+        out = cls(torch.zeros((m * ld + nb * mp,), dtype=_u8, device=codes.device), m, c)
+        out.codes[:, :c] = codes
+        out.exps.copy_(exps)
+        return out
+
+    @property
+    def codes(self) -> torch.Tensor:
+        m, c = self.shape
+        ld = (c + 15) & ~15
+        return self.data.as_strided((m, ld), (ld, 1))
+
+    @property
+    def exps(self) -> torch.Tensor:
+        m, c = self.shape
+        ld, nb, mp = _sizes(m, c)
+        return self.data.as_strided((m, nb), (1, mp), self.data.storage_offset() + m * ld)
 
     @property
     def device(self):
-        return self.codes.device
+        return self.data.device
 
     def nbytes(self) -> int:
-        return self.codes.numel() + self.exps.numel()
+        return self.data.numel()
 
 
-def _kept(x8, name: str) -> Rows8:
+def _kept(x8, name: str) -> Tuple[int, int, int, int, int, int]:
+    """(rows, channels, address of the codes, bytes of their rows, address of the scales, bytes of their columns)"""
     if not isinstance(x8, Rows8):
         raise TypeError(f"{name}: expected Rows8, got {type(x8).__name__}")
-    _on_device(x8.codes, name)
-    return x8
+    _on_device(x8.data, name)
+    m, c = x8.shape
+    ld = (c + 15) & ~15
+    p = x8.data.data_ptr()
+    return m, c, p, ld, p + m * ld, (m + 15) & ~15
 
 
 def checkpoint_rows(x: torch.Tensor) -> Rows8:
     """x (M, C) float32 / bfloat16 / float16 (any row stride) -> its kept form.  Not differentiable: it stands for x in x's backward."""
-    px, ldx = _matrix(x, "x")
-    m, c = x.shape
-    codes = torch.empty((m, (c + 15) // 16 * 16), dtype=_u8, device=x.device)
-    exps = _exps(m, c, x.device)
-    L.check(L.load().jm_rows8_pack(m, c, TYPES[x.dtype], px, ldx, codes.data_ptr(), codes.shape[1], exps.data_ptr(), (m + 15) // 16 * 16, L.stream_ptr()), "checkpoint_rows")
-    return Rows8(codes, exps, c)
+    m, c, px, ldx = _matrix(x, "x")
+    ld, nb, mp = _sizes(m, c)
+    data = torch.empty((m * ld + nb * mp,), dtype=_u8, device=x.device)
+    pc = data.data_ptr()
+    L.check(L.load().jm_rows8_pack(m, c, TYPES[x.dtype], px, ldx, pc, ld, pc + m * ld, mp, L.stream_ptr()), "checkpoint_rows")
+    out = Rows8.__new__(Rows8)
+    out.data, out.shape = data, (m, c)
+    return out
 
 
 def restore_rows(x8: Rows8, dtype: torch.dtype = _f32) -> torch.Tensor:
     """the kept values (M, C), exact in float32 and bfloat16, rounded once in float16"""
-    _kept(x8, "x8")
+    m, c, pc, ld, pe, mp = _kept(x8, "x8")
     if dtype not in TYPES:
         raise TypeError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
-    m, c = x8.shape
-    out = torch.empty((m, c), dtype=dtype, device=x8.device)
-    L.check(L.load().jm_rows8_restore(m, c, TYPES[dtype], x8.codes.data_ptr(), x8.codes.shape[1], x8.exps.data_ptr(), (m + 15) // 16 * 16, out.data_ptr(), c, L.stream_ptr()),
-            "restore_rows")
+    out = torch.empty((m, c), dtype=dtype, device=x8.data.device)
+    L.check(L.load().jm_rows8_restore(m, c, TYPES[dtype], pc, ld, pe, mp, out.data_ptr(), c, L.stream_ptr()), "restore_rows")
     return out
 
 
 def relu_mask8(dy: torch.Tensor, y8: Rows8) -> torch.Tensor:
     """kept y > 0 ? dy : 0 as a new float32 tensor: the gradient through a ReLU from its kept output"""
-    pdy, ldd = _matrix(dy, "dy", _f32)
-    _kept(y8, "y8")
-    if tuple(dy.shape) != y8.shape:
+    m, c, pdy, ldd = _matrix(dy, "dy", _f32)
+    m8, c8, pc, ld, _, _ = _kept(y8, "y8")
+    if (m, c) != (m8, c8):
         raise ValueError(f"dy {tuple(dy.shape)} for a kept output {y8.shape}")
-    m, c = dy.shape
     out = torch.empty((m, c), dtype=_f32, device=dy.device)
-    L.check(L.load().jm_rows8_relu_mask(m, c, pdy, ldd, y8.codes.data_ptr(), y8.codes.shape[1], out.data_ptr(), c, L.stream_ptr()), "relu_mask8")
+    L.check(L.load().jm_rows8_relu_mask(m, c, pdy, ldd, pc, ld, out.data_ptr(), c, L.stream_ptr()), "relu_mask8")
     return out
 
 
 def linear_wgrad8(dy: torch.Tensor, x8: Rows8, want_bias: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(dw (N, K) = dy^T x, dbias (N) or None) in float32, dy (M, N) float32 / bfloat16 / float16, x (M, K) kept: ops.rows.linear_wgrad
     with the input as `checkpoint_rows` left it"""
-    pdy, ldd = _matrix(dy, "dy")
-    _kept(x8, "x8")
-    m, n = dy.shape
-    if x8.shape[0] != m:
-        raise ValueError(f"dy of {m} rows for a kept input of {x8.shape[0]}")
-    k = x8.shape[1]
+    m, n, pdy, ldd = _matrix(dy, "dy")
+    m8, k, pc, ld, pe, mp = _kept(x8, "x8")
+    if m8 != m:
+        raise ValueError(f"dy of {m} rows for a kept input of {m8}")
     lib = L.load()
-    dw = torch.empty((n, k), dtype=_f32, device=dy.device)
-    db = torch.empty((n,), dtype=_f32, device=dy.device) if want_bias else None
+    device = dy.device
+    dw = torch.empty((n, k), dtype=_f32, device=device)
+    db = torch.empty((n,), dtype=_f32, device=device) if want_bias else None
     nbytes = lib.jm_rows8_wgrad_workspace_bytes(m, n, k)
-    ws = torch.empty((nbytes // 4,), dtype=_f32, device=dy.device) if nbytes else None
-    L.check(lib.jm_rows8_linear_wgrad(m, n, k, TYPES[dy.dtype], pdy, ldd, x8.codes.data_ptr(), x8.codes.shape[1], x8.exps.data_ptr(), (m + 15) // 16 * 16, dw.data_ptr(), k,
-                                      db.data_ptr() if want_bias else None, ws.data_ptr() if ws is not None else None, nbytes, L.stream_ptr()),
-            "linear_wgrad8")
+    ws = torch.empty((nbytes // 4,), dtype=_f32, device=device) if nbytes else None
+    L.check(lib.jm_rows8_linear_wgrad(m, n, k, TYPES[dy.dtype], pdy, ldd, pc, ld, pe, mp, dw.data_ptr(), k, db.data_ptr() if want_bias else None,
+                                      ws.data_ptr() if nbytes else None, nbytes, L.stream_ptr()), "linear_wgrad8")
     return dw, db

@@ -18,7 +18,7 @@ def test_host_tensors_are_refused():
     with pytest.raises(RuntimeError):
         R8.checkpoint_rows(x)
     k = R8.Rows8.from_codes(torch.zeros(4, 8, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8))
-    assert k.shape == (4, 8) and k.nbytes() == 68
+    assert k.shape == (4, 8) and k.nbytes() == 80
     for call in (lambda: R8.restore_rows(k), lambda: R8.linear_wgrad8(x, k), lambda: R8.relu_mask8(x, k), lambda: AD.AdapterPlan(torch.zeros(4, dtype=torch.int32), 2)):
         with pytest.raises(RuntimeError):
             call()

@@ -237,8 +237,14 @@ def test_refusals():
     with pytest.raises(TypeError):
         R8.relu_mask8(x.half(), k)
     with pytest.raises(ValueError):
-        R8.Rows8(k.codes, k.exps, 40)
+        R8.Rows8(k.data, 6, 40)
     with pytest.raises(ValueError):
-        R8.Rows8(k.codes, k.exps[:5].contiguous(), 20)
+        R8.Rows8(k.data, 5, 20)
     with pytest.raises(TypeError):
-        R8.Rows8(k.codes.int(), k.exps, 20)
+        R8.Rows8(k.codes, 6, 20)
+    with pytest.raises(ValueError):
+        R8.Rows8.from_codes(k.codes[:, :20], k.exps[:5])
+    with pytest.raises(TypeError):
+        R8.Rows8.from_codes(k.codes.int(), k.exps)
+    again = R8.Rows8.from_codes(k.codes[:, :20], k.exps)
+    assert torch.equal(again.codes, k.codes) and torch.equal(again.exps, k.exps) and again.nbytes() == k.nbytes()
