@@ -24,7 +24,7 @@ constexpr int PL_MAX_ADAPTERS = 1023;        // + the rows without an adapter: o
 constexpr int AD_WIDE_ROWS = 16384;
 // rows of a tile: 16 while that leaves CUs idle, 32 where there are enough tiles (A and B are read once a tile)
 static __host__ __device__ __forceinline__ int ad_tile(int m) { return m < AD_WIDE_ROWS ? 16 : 32; }
-constexpr int AD_CHUNK = 1024;       // rows of a chunk (weight gradients)
+constexpr int AD_CHUNK = 512;       // rows of a chunk (weight gradients)
 constexpr int AD_MAX_ROWS = 1 << 30, AD_MAX_WIDTH = 1 << 20;        // tile counts, grids and per-adapter element counts stay in range
 
 struct PlanLayout {                  // offsets in ints; header: [0] tiles, [1] chunks
@@ -472,7 +472,7 @@ adapter_transpose_kernel(int rank, int k, int n, const T* __restrict__ a, T* __r
 
 // ------------------------------------------------------------------------------------------------ gradients of A and B
 struct AdaptGrad {
-    int m, k, n, rank, adapters;
+    int m, k, n, rank, adapters, direct;
     const int* plan; size_t o_order, o_chunks, o_chunk_first;
     const void* x; long long ldx;
     const unsigned char* codes; int ldc; const unsigned char* exps; int lde;      // x kept in 8 bits (x NULL)
@@ -483,120 +483,267 @@ struct AdaptGrad {
     void *da, *db;
 };
 
-// 4 consecutive channels of a row, zeros beyond the width
-template <int TY, bool KEPT>
-__device__ __forceinline__ f32x4 grad_load4(const AdaptGrad& p, const void* src, long long ld, size_t row, int c, int width) {
-    f32x4 v;
-    if (KEPT) {
-        const float s = __uint_as_float((unsigned)p.exps[(size_t)(min(c, width - 1) / 32) * p.lde + row] << 23);       // scale bytes: 27 .. 247
-        unsigned w = 0;
-        if (c < width) w = *reinterpret_cast<const unsigned*>(p.codes + row * p.ldc + c);
-        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
-        const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-        v = f32x4{lo[0] * s, lo[1] * s, hi[0] * s, hi[1] * s};
-    } else {
-        typedef typename Elem<TY>::T T;
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        const T* q = (const T*)src + row * ld + c;
-        T4 r;
-        if (c + 4 <= width) {
-            __builtin_memcpy(&r, q, sizeof(T4));
-        } else {
+// CW consecutive channels of a row as they are stored (kept: e4m3 codes and the scale of their block), zeros beyond the width
+template <int TY, bool KEPT, int CW>
+struct GradRun {
+    typedef typename Elem<TY>::T T;
+    typedef T V __attribute__((ext_vector_type(CW)));
+    V v;
+    unsigned w[CW / 4], e;
+    __device__ __forceinline__ void load(const AdaptGrad& p, const void* src, long long ld, size_t row, int c, int width) {
+        if constexpr (KEPT) {
+            e = p.exps[(size_t)(min(c, width - 1) / 32) * p.lde + row];
+            const unsigned* q = reinterpret_cast<const unsigned*>(p.codes + row * p.ldc + c);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                T t = (T)0.f;
-                if (c + e < width) t = q[e];
-                r[e] = t;
+            for (int h = 0; h < CW / 4; ++h) w[h] = 0u;
+            if (c + CW <= p.ldc)
+#pragma unroll
+                for (int h = 0; h < CW / 4; ++h) w[h] = q[h];
+        } else {
+            const T* q = (const T*)src + row * ld + c;
+            if (c + CW <= width) {
+                __builtin_memcpy(&v, q, sizeof(V));
+            } else {
+#pragma unroll
+                for (int j = 0; j < CW; ++j) {
+                    T t = (T)0.f;
+                    if (c + j < width) t = q[j];
+                    v[j] = t;
+                }
             }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (float)r[e];
     }
-    return v;
-}
+    // channels 2 h, 2 h + 1 as two bfloat16 (rows of bfloat16, kept rows)
+    __device__ __forceinline__ unsigned pair(int h) const {
+        unsigned o;
+        if constexpr (KEPT) {
+            const float s = __uint_as_float(e << 23);
+            const auto d = (h & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w[h / 2], s, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w[h / 2], s, false);
+            __builtin_memcpy(&o, &d, 4);
+        } else {
+            typedef T V2 __attribute__((ext_vector_type(2)));
+            const V2 d = {v[2 * h], v[2 * h + 1]};
+            __builtin_memcpy(&o, &d, 4);
+        }
+        return o;
+    }
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (KEPT) {
+            const auto d = (j & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j / 4], true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w[j / 4], false);
+            return d[j & 1] * __uint_as_float(e << 23);      // scale bytes: 27 .. 247
+        } else {
+            return (float)v[j];
+        }
+    }
+};
 
-// Workgroup = (chunk of one adapter's rows) x (64 channels of x, then of dy) x (64 rank indices); its four waves take every fourth group
-// of four rows, 16 x 16 x 4 float32 products of T (t or u: rank) with X (channels), UR groups in flight, and add their tiles in wave
-// order through LDS.
-template <int TY, bool KEPT, int RB>
-__global__ void __launch_bounds__(256)
-adapter_wgrad_kernel(AdaptGrad p) {
-    constexpr int UR = 8;
-    __shared__ union {
-        f32x4 red[3][RB * 4][64];
-        int order[AD_CHUNK];
-    } sh;
-    if ((int)blockIdx.x >= p.plan[1]) return;
-    const int4 chunk = *reinterpret_cast<const int4*>(p.plan + p.o_chunks + 4 * (size_t)blockIdx.x);
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
-    const int tk = (p.k + 63) / 64;
-    const bool isA = (int)blockIdx.y < tk;
-    const int c0 = (isA ? (int)blockIdx.y : (int)blockIdx.y - tk) * 64, width = isA ? p.k : p.n, r0 = blockIdx.z * 64;
-    const float* T = isA ? p.u : p.t;
-    for (int q = threadIdx.x; q < chunk.z; q += 256) sh.order[q] = p.plan[p.o_order + chunk.y + q];
+// the four waves' tiles through LDS, added in wave order, to their place
+template <int TY, int RB, int CW>
+__device__ __forceinline__ void adapter_wgrad_finish(const AdaptGrad& p, float* lds, int4 chunk, int ad, bool isA, int c0, int r0, const f32x4 (&acc)[RB][CW]) {
+    constexpr int TR = 16 * RB, TC = 16 * CW;
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6, width = isA ? p.k : p.n;
     __syncthreads();
-    f32x4 acc[RB][4];
+    // D: rows = rank index 4 g + q, column i = channel CW i + j of the tile
+    float* const mine = lds + wave * TR * TC;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[rb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto body = [&](auto kept_, const void* src, long long ld) __attribute__((always_inline)) {
-        constexpr bool K8 = decltype(kept_)::value;
-        for (int q0 = wave * 4; q0 < chunk.z; q0 += 16 * UR) {
-            f32x4 xv[UR];
-            float tv[UR][RB];
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int u = 0; u < UR; ++u) {               // (rows beyond the chunk: the last one, counted as zeros)
-                const size_t row = (size_t)sh.order[min(q0 + 16 * u + g, chunk.z - 1)];
-                xv[u] = grad_load4<TY, K8>(p, src, ld, row, c0 + 4 * i, width);
+            for (int j = 0; j < CW; j += 4)
+                *reinterpret_cast<f32x4*>(mine + (rb * 16 + 4 * g + q) * TC + CW * i + j) = f32x4{acc[rb][j][q], acc[rb][j + 1][q], acc[rb][j + 2][q], acc[rb][j + 3][q]};
+    __syncthreads();
+    typedef typename Elem<TY>::T E;
+    float* part = p.part + (size_t)blockIdx.x * p.rank * ((size_t)p.k + p.n);
+    const float scale = p.direct ? p.scales[ad] : 1.f;
+    for (int e = threadIdx.x; e < TR * TC; e += 256) {       // (dA runs along the channels, dB along the rank)
+        const int rt = isA ? e / TC : e % TR, ct = isA ? e % TC : e / TR, r = r0 + rt, c = c0 + ct;
+        if (r >= p.rank || c >= width) continue;
+        const float* v = lds + rt * TC + ct;
+        const float sum = (v[0] + v[TR * TC]) + (v[2 * TR * TC] + v[3 * TR * TC]);
+        const size_t at = isA ? (size_t)r * p.k + c : (size_t)c * p.rank + r;
+        if (p.direct) ((E*)(isA ? p.da : p.db))[(size_t)ad * p.rank * width + at] = (E)(chunk.z > 0 ? scale * sum : 0.f);
+        else part[(isA ? 0 : (size_t)p.rank * p.k) + at] = sum;
+    }
+}
+
+// Workgroup = (chunk of one adapter's rows) x (16 CW channels of x, then of dy) x (16 RB rank indices); its four waves take every fourth
+// group of four rows, 16 x 16 x 4 float32 products of T (t or u: rank) with X (CW channels a lane), UR groups in flight while UR are
+// multiplied, and add their tiles in wave order through LDS.  Bound by the loads' latency: a chunk's rows are 512 / 16 = 32 groups a wave.
+// With at most one chunk an adapter (direct) the workgroups are the adapters' and write dA and dB themselves.
+template <int TY, bool KEPT, int RB, int CW>
+__device__ __forceinline__ void adapter_wgrad_tile(const AdaptGrad& p, float* lds, int4 chunk, int ad, bool isA, int c0, int r0) {
+    constexpr int UR = 4;
+    int* const rows = reinterpret_cast<int*>(lds);
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int width = isA ? p.k : p.n;
+    const void* src = isA ? p.x : p.dy;
+    const long long ld = isA ? p.ldx : p.lddy;
+    const float* T = isA ? p.u : p.t;
+    for (int q = threadIdx.x; q < chunk.z; q += 256) rows[q] = p.plan[p.o_order + chunk.y + q];
+    __syncthreads();
+    f32x4 acc[RB][CW];
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) tv[u][rb] = T[row * p.rank + min(r0 + rb * 16 + i, p.rank - 1)];
-            }
+    for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-            for (int u = 0; u < UR; ++u) {
-                const bool ok = q0 + 16 * u + g < chunk.z;
+        for (int j = 0; j < CW; ++j) acc[rb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    struct Batch {
+        GradRun<TY, KEPT, CW> x[UR];
+        float t[UR][RB];
+    };
+    auto fetch = [&](Batch& b, int q0) __attribute__((always_inline)) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) xv[u][e] = ok ? xv[u][e] : 0.f;
+        for (int u = 0; u < UR; ++u) {                       // (rows beyond the chunk: the last one, counted as zeros)
+            const size_t row = (size_t)rows[min(q0 + 16 * u + g, chunk.z - 1)];
+            b.x[u].load(p, src, ld, row, c0 + CW * i, width);
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) {
-                    const float t = ok ? tv[u][rb] : 0.f;
+            for (int rb = 0; rb < RB; ++rb) b.t[u][rb] = T[row * p.rank + min(r0 + rb * 16 + i, p.rank - 1)];
+        }
+    };
+    auto multiply = [&](const Batch& b, int q0) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[rb][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(t, xv[u][j], acc[rb][j], 0, 0, 0);
-                }
+        for (int u = 0; u < UR; ++u) {
+            const bool ok = q0 + 16 * u + g < chunk.z;
+            float xv[CW];
+#pragma unroll
+            for (int j = 0; j < CW; ++j) xv[j] = ok ? b.x[u].get(j) : 0.f;
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                const float t = ok ? b.t[u][rb] : 0.f;
+#pragma unroll
+                for (int j = 0; j < CW; ++j) acc[rb][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(t, xv[j], acc[rb][j], 0, 0, 0);
             }
         }
     };
-    if (KEPT && isA) body(std::integral_constant<bool, KEPT>{}, nullptr, 0);
-    else body(std::false_type{}, isA ? p.x : p.dy, isA ? p.ldx : p.lddy);
+    if (chunk.z > 0) {
+        constexpr int ST = 16 * UR;                          // rows of a batch of the four waves
+        Batch b[2];
+        int q = wave * 4;
+        fetch(b[0], q);
+        for (; q < chunk.z; q += 2 * ST) {
+            if (q + ST < chunk.z) fetch(b[1], q + ST);
+            multiply(b[0], q);
+            if (q + 2 * ST < chunk.z) fetch(b[0], q + 2 * ST);
+            if (q + ST < chunk.z) multiply(b[1], q + ST);
+        }
+    }
+    adapter_wgrad_finish<TY, RB, CW>(p, lds, chunk, ad, isA, c0, r0, acc);
+}
+
+// The same tile on the bf16 matrix pipe, for channels that are exact in bfloat16 (bfloat16 rows, kept rows): T enters as three bfloat16
+// pieces that add up to it (rows8.hip's cut), so products are exact and only the float32 additions round — at a third of sixteen times the
+// float32 rate, and bound by memory up to a rank of 32.  A lane's 8 contraction elements are 8 rows; it holds 8 channels of each and turns
+// the 8 x 8 block over in its registers.
+template <bool KEPT, int RB>
+__device__ __forceinline__ void adapter_wgrad_tile_bf16(const AdaptGrad& p, float* lds, int4 chunk, int ad, bool isA, int c0, int r0) {
+    constexpr int CW = 8, STEP = 4 * 32;
+    int* const rows = reinterpret_cast<int*>(lds);
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+    const int width = isA ? p.k : p.n;
+    const void* src = isA ? p.x : p.dy;
+    const long long ld = isA ? p.ldx : p.lddy;
+    const float* T = isA ? p.u : p.t;
+    for (int q = threadIdx.x; q < chunk.z; q += 256) rows[q] = p.plan[p.o_order + chunk.y + q];
     __syncthreads();
-    auto& red = sh.red;
-    if (wave > 0)
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) red[wave - 1][rb * 4 + j][lane] = acc[rb][j];
-    __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int w = 0; w < 3; ++w)
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[rb][j] += red[w][rb * 4 + j][lane];
-    // D: rows = rank index 4 g + q, column i = channel c0 + 4 i + j
-    float* part = p.part + (size_t)blockIdx.x * p.rank * (p.k + p.n);
+    f32x4 acc[RB][CW];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < CW; ++j) acc[rb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    struct Batch {
+        GradRun<JM_BF16, KEPT, CW> x[8];
+        float t[RB][8];
+    };
+    auto fetch = [&](Batch& b, int q0) __attribute__((always_inline)) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int r = r0 + rb * 16 + 4 * g + q, c = c0 + 4 * i + j;
-                if (r < p.rank && c < width) {
-                    if (isA) part[(size_t)r * p.k + c] = acc[rb][j][q];
-                    else part[(size_t)p.rank * p.k + (size_t)c * p.rank + r] = acc[rb][j][q];
+        for (int e = 0; e < 8; ++e) {                        // (rows beyond the chunk: the last one, counted as zeros)
+            const size_t row = (size_t)rows[min(q0 + 8 * g + e, chunk.z - 1)];
+            b.x[e].load(p, src, ld, row, c0 + CW * i, width);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) b.t[rb][e] = T[row * p.rank + min(r0 + rb * 16 + i, p.rank - 1)];
+        }
+    };
+    auto multiply = [&](const Batch& b, int q0) __attribute__((always_inline)) {
+        unsigned xw[8][4];                                   // two channels a word
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool ok = q0 + 8 * g + e < chunk.z;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) xw[e][h] = ok ? b.x[e].pair(h) : 0u;
+        }
+        bf16x8 xf[CW];
+#pragma unroll
+        for (int j = 0; j < CW; ++j) {
+            u32x4 w;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) w[h] = (j & 1) ? pack_hi(xw[2 * h][j / 2], xw[2 * h + 1][j / 2]) : pack_lo(xw[2 * h][j / 2], xw[2 * h + 1][j / 2]);
+            xf[j] = __builtin_bit_cast(bf16x8, w);
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            u32x4 piece[3];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                unsigned a = q0 + 8 * g + 2 * h < chunk.z ? __float_as_uint(b.t[rb][2 * h]) : 0u;
+                unsigned c = q0 + 8 * g + 2 * h + 1 < chunk.z ? __float_as_uint(b.t[rb][2 * h + 1]) : 0u;
+#pragma unroll
+                for (int s = 0; s < 3; ++s) {
+                    piece[s][h] = pack_hi(a, c);
+                    if (s < 2) {                             // what the cut left; of an infinity nothing, of a NaN a NaN
+                        const float fa = __uint_as_float(a), fc = __uint_as_float(c);
+                        a = __builtin_isinf(fa) ? 0u : __float_as_uint(fa - __uint_as_float(a & 0xffff0000u));
+                        c = __builtin_isinf(fc) ? 0u : __float_as_uint(fc - __uint_as_float(c & 0xffff0000u));
+                    }
                 }
             }
+#pragma unroll
+            for (int s = 2; s >= 0; --s) {
+                const bf16x8 tf = __builtin_bit_cast(bf16x8, piece[s]);
+#pragma unroll
+                for (int j = 0; j < CW; ++j) acc[rb][j] = mma16(acc[rb][j], tf, xf[j]);
+            }
+        }
+    };
+    if (chunk.z > 0) {
+        Batch b[2];
+        int q = wave * 32;
+        if (q < chunk.z) fetch(b[0], q);
+        for (; q < chunk.z; q += 2 * STEP) {
+            if (q + STEP < chunk.z) fetch(b[1], q + STEP);
+            multiply(b[0], q);
+            if (q + 2 * STEP < chunk.z) fetch(b[0], q + 2 * STEP);
+            if (q + STEP < chunk.z) multiply(b[1], q + STEP);
+        }
+    }
+    adapter_wgrad_finish<JM_BF16, RB, CW>(p, lds, chunk, ad, isA, c0, r0, acc);
+}
+
+template <int TY, bool KEPT, int RB, int CW>
+__global__ void __launch_bounds__(256)
+adapter_wgrad_kernel(AdaptGrad p) {
+    __shared__ __attribute__((aligned(16))) float lds[4 * 16 * RB * 16 * CW];       // the rows of the chunk, then the waves' tiles
+    static_assert(sizeof(lds) >= AD_CHUNK * sizeof(int), "the row list is kept there");
+    int ad = 0;
+    int4 chunk;
+    if (p.direct) {
+        ad = blockIdx.x;
+        const int c = p.plan[p.o_chunk_first + ad];
+        chunk = make_int4(ad, 0, 0, 0);
+        if (p.plan[p.o_chunk_first + ad + 1] > c) chunk = *reinterpret_cast<const int4*>(p.plan + p.o_chunks + 4 * (size_t)c);
+    } else {
+        if ((int)blockIdx.x >= p.plan[1]) return;
+        chunk = *reinterpret_cast<const int4*>(p.plan + p.o_chunks + 4 * (size_t)blockIdx.x);
+    }
+    const int tk = (p.k + 16 * CW - 1) / (16 * CW), r0 = blockIdx.z * 16 * RB;
+    const bool isA = (int)blockIdx.y < tk;
+    const int c0 = (isA ? (int)blockIdx.y : (int)blockIdx.y - tk) * 16 * CW;
+    if constexpr (TY == JM_BF16 && CW == 8) {
+        if (isA) adapter_wgrad_tile_bf16<KEPT, RB>(p, lds, chunk, ad, true, c0, r0);
+        else adapter_wgrad_tile_bf16<false, RB>(p, lds, chunk, ad, false, c0, r0);
+    } else {
+        if (isA) adapter_wgrad_tile<TY, KEPT, RB, CW>(p, lds, chunk, ad, true, c0, r0);
+        else adapter_wgrad_tile<TY, false, RB, CW>(p, lds, chunk, ad, false, c0, r0);
+    }
 }
 
 // dA, dB of an adapter = s times the sum of its chunks' partials, in chunk order (zero without rows)
@@ -607,19 +754,17 @@ adapter_wgrad_reduce_kernel(AdaptGrad p) {
     const int e = blockIdx.x * 256 + threadIdx.x, ad = blockIdx.y;
     if (e >= per) return;
     const int c_begin = p.plan[p.o_chunk_first + ad], c_end = p.plan[p.o_chunk_first + ad + 1];
-    float s = 0.f;
-    float s1 = 0.f, s2 = 0.f, s3 = 0.f;                  // four chains: the loads of consecutive chunks are in flight together
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};   // eight chains: the loads of consecutive chunks are in flight together
     int c = c_begin;
-    for (; c + 4 <= c_end; c += 4) {
-        s += p.part[(size_t)c * per + e];        s1 += p.part[(size_t)(c + 1) * per + e];
-        s2 += p.part[(size_t)(c + 2) * per + e]; s3 += p.part[(size_t)(c + 3) * per + e];
-    }
-    for (; c < c_end; ++c) s += p.part[(size_t)c * per + e];
-    s = ((s + s1) + (s2 + s3)) * p.scales[ad];
+    for (; c + 8 <= c_end; c += 8)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s[u] += p.part[(size_t)(c + u) * per + e];
+    for (; c < c_end; ++c) s[0] += p.part[(size_t)c * per + e];
+    float v = (((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]))) * p.scales[ad];
     const int na = p.rank * p.k;
-    if (c_begin == c_end) s = 0.f;
-    if (e < na) ((T*)p.da)[(size_t)ad * na + e] = (T)s;
-    else ((T*)p.db)[(size_t)ad * p.rank * p.n + (e - na)] = (T)s;
+    if (c_begin == c_end) v = 0.f;
+    if (e < na) ((T*)p.da)[(size_t)ad * na + e] = (T)v;
+    else ((T*)p.db)[(size_t)ad * p.rank * p.n + (e - na)] = (T)v;
 }
 
 static size_t elem_size(int type) { return type == JM_F32 ? 4 : 2; }
@@ -645,12 +790,16 @@ static void launch_rows(int type, const Adapt& p, int tiles, hipStream_t s) {
     else launch_rows<JM_F16>(p, grid, s);
 }
 
+// rank indices and channels of a workgroup: 16 x 128, 32 x 128, 64 x 64 (accumulators of a wave: 32, 64, 64 registers); on the bf16 pipe, whose
+// operands take more registers, 32 x 128 beyond a rank of 32 too
 template <int TY, bool KEPT>
-static void launch_wgrad(const AdaptGrad& p, int chunks, hipStream_t s) {
-    const dim3 grid((unsigned)chunks, (unsigned)(divup(p.k, 64) + divup(p.n, 64)), (unsigned)divup(p.rank, 64)), block(256);
-    if (p.rank <= 16) hipLaunchKernelGGL((adapter_wgrad_kernel<TY, KEPT, 1>), grid, block, 0, s, p);
-    else if (p.rank <= 32) hipLaunchKernelGGL((adapter_wgrad_kernel<TY, KEPT, 2>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((adapter_wgrad_kernel<TY, KEPT, 4>), grid, block, 0, s, p);
+static void launch_wgrad(const AdaptGrad& p, int groups, hipStream_t s) {
+    const bool wide = p.rank <= 32 || TY == JM_BF16;
+    const int cw = wide ? 128 : 64, rw = p.rank <= 16 ? 16 : (wide ? 32 : 64);
+    const dim3 grid((unsigned)groups, (unsigned)(divup(p.k, cw) + divup(p.n, cw)), (unsigned)divup(p.rank, rw)), block(256);
+    if (p.rank <= 16) hipLaunchKernelGGL((adapter_wgrad_kernel<TY, KEPT, 1, 8>), grid, block, 0, s, p);
+    else if (wide) hipLaunchKernelGGL((adapter_wgrad_kernel<TY, KEPT, 2, 8>), grid, block, 0, s, p);
+    else if constexpr (TY != JM_BF16) hipLaunchKernelGGL((adapter_wgrad_kernel<TY, KEPT, 4, 4>), grid, block, 0, s, p);
 }
 
 struct GradLayout { size_t at, bt, u, part, total; };        // bytes
@@ -738,7 +887,8 @@ int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const
     AdaptGrad q{};
     q.m = m; q.k = k; q.n = n; q.rank = rank; q.adapters = adapters; q.plan = plan; q.o_order = l.order; q.o_chunks = l.chunks;
     q.o_chunk_first = l.chunk_first; q.x = x; q.ldx = ldx; q.codes = codes; q.ldc = ldc; q.exps = exps; q.lde = lde;
-    q.dy = dy; q.lddy = lddy; q.t = t; q.u = (const float*)(w + gl.u); q.scales = scales; q.part = (float*)(w + gl.part); q.da = da; q.db = db;
+    q.dy = dy; q.lddy = lddy; q.t = t; q.u = (const float*)(w + gl.u); q.scales = scales; q.part = (float*)(w + gl.part); q.direct = m > 0 && m <= AD_CHUNK; q.da = da; q.db = db;
+    const int groups = q.direct ? adapters : l.max_chunks;
     if (m > 0) {
         const dim3 gt((unsigned)((divup(k, 32) + divup(n, 32)) * divup(rank, 32)), (unsigned)adapters);
         if (type == JM_F32) {
@@ -753,15 +903,16 @@ int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const
         p.copy = base != dx;
         launch_rows(type, p, l.max_tiles, s);
         if (x) {
-            if (type == JM_F32) launch_wgrad<JM_F32, false>(q, l.max_chunks, s);
-            else if (type == JM_BF16) launch_wgrad<JM_BF16, false>(q, l.max_chunks, s);
-            else launch_wgrad<JM_F16, false>(q, l.max_chunks, s);
+            if (type == JM_F32) launch_wgrad<JM_F32, false>(q, groups, s);
+            else if (type == JM_BF16) launch_wgrad<JM_BF16, false>(q, groups, s);
+            else launch_wgrad<JM_F16, false>(q, groups, s);
         } else {
-            if (type == JM_F32) launch_wgrad<JM_F32, true>(q, l.max_chunks, s);
-            else if (type == JM_BF16) launch_wgrad<JM_BF16, true>(q, l.max_chunks, s);
-            else launch_wgrad<JM_F16, true>(q, l.max_chunks, s);
+            if (type == JM_F32) launch_wgrad<JM_F32, true>(q, groups, s);
+            else if (type == JM_BF16) launch_wgrad<JM_BF16, true>(q, groups, s);
+            else launch_wgrad<JM_F16, true>(q, groups, s);
         }
     }
+    if (q.direct) return check_launch("adapter_grad");
     const dim3 gr((unsigned)divup(rank * (k + n), 256), (unsigned)adapters);
     if (type == JM_F32) hipLaunchKernelGGL((adapter_wgrad_reduce_kernel<float>), gr, dim3(256), 0, s, q);
     else if (type == JM_BF16) hipLaunchKernelGGL((adapter_wgrad_reduce_kernel<__bf16>), gr, dim3(256), 0, s, q);

@@ -52,4 +52,9 @@ __device__ __forceinline__ f32x4 mma16(f32x4 c, const f32x8& a, const f32x8& b) 
 __device__ __forceinline__ f32x4 mma16(f32x4 c, const bf16x8& a, const bf16x8& b) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mma16(f32x4 c, const f16x8& a, const f16x8& b) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+// the upper (lower) halves of two words as one: half of a | half of b << 16
+__device__ __forceinline__ unsigned pack_hi(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+__device__ __forceinline__ unsigned pack_lo(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+
 }  // namespace jm

@@ -174,8 +174,6 @@ struct Wgrad8 {
     long long lddw;
 };
 
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-
 // four consecutive columns of a row.  The columns of a group that lies outside the matrix are whatever lies inside (they only reach
 // outputs that are never stored); a group that straddles the edge (`ragged`, widths that are no multiple of 4) is read from width - 4 and shifted
 template <int TY> struct Quad;
@@ -208,10 +206,6 @@ template <int TY> struct Quad16 {
 };
 template <> struct Quad<JM_BF16> : Quad16<JM_BF16> {};
 template <> struct Quad<JM_F16> : Quad16<JM_F16> {};
-
-// the upper halves of two words as one: (hi half of a) | (hi half of b) << 16
-__device__ __forceinline__ unsigned pack_hi(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
-__device__ __forceinline__ unsigned pack_lo(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 
 template <int TY, bool SMALL, int W8_T>
 __global__ void __launch_bounds__(512, 1)
