@@ -490,9 +490,10 @@ struct GradRun {
     typedef T V __attribute__((ext_vector_type(CW)));
     V v;
     unsigned w[CW / 4], e;
-    __device__ __forceinline__ void load(const AdaptGrad& p, const void* src, long long ld, size_t row, int c, int width) {
+    // scale: kept rows, the scale byte of the row and the channels' block
+    __device__ __forceinline__ void load(const AdaptGrad& p, const void* src, long long ld, size_t row, int c, int width, const unsigned char* scale) {
         if constexpr (KEPT) {
-            e = p.exps[(size_t)(min(c, width - 1) / 32) * p.lde + row];
+            e = *scale;
             const unsigned* q = reinterpret_cast<const unsigned*>(p.codes + row * p.ldc + c);
 #pragma unroll
             for (int h = 0; h < CW / 4; ++h) w[h] = 0u;
@@ -580,8 +581,18 @@ __device__ __forceinline__ void adapter_wgrad_tile(const AdaptGrad& p, float* ld
     const void* src = isA ? p.x : p.dy;
     const long long ld = isA ? p.ldx : p.lddy;
     const float* T = isA ? p.u : p.t;
-    for (int q = threadIdx.x; q < chunk.z; q += 256) rows[q] = p.plan[p.o_order + chunk.y + q];
+    // the chunk's rows, and of kept rows the scales of the tile's blocks of 32 channels, once for all batches
+    unsigned char* const scales = reinterpret_cast<unsigned char*>(rows + AD_CHUNK);
+    for (int q = threadIdx.x; q < chunk.z; q += 256) {
+        const int row = p.plan[p.o_order + chunk.y + q];
+        rows[q] = row;
+        if constexpr (KEPT) {
+#pragma unroll
+            for (int b = 0; b < CW / 2; ++b) scales[b * AD_CHUNK + q] = p.exps[(size_t)min(c0 / 32 + b, (width - 1) / 32) * p.lde + row];
+        }
+    }
     __syncthreads();
+    const unsigned char* const scale = scales + (CW * i / 32) * AD_CHUNK;
     f32x4 acc[RB][CW];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
@@ -594,8 +605,9 @@ __device__ __forceinline__ void adapter_wgrad_tile(const AdaptGrad& p, float* ld
     auto fetch = [&](Batch& b, int q0) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < UR; ++u) {                       // (rows beyond the chunk: the last one, counted as zeros)
-            const size_t row = (size_t)rows[min(q0 + 16 * u + g, chunk.z - 1)];
-            b.x[u].load(p, src, ld, row, c0 + CW * i, width);
+            const int at = min(q0 + 16 * u + g, chunk.z - 1);
+            const size_t row = (size_t)rows[at];
+            b.x[u].load(p, src, ld, row, c0 + CW * i, width, scale + at);
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) b.t[u][rb] = T[row * p.rank + min(r0 + rb * 16 + i, p.rank - 1)];
         }
@@ -643,8 +655,18 @@ __device__ __forceinline__ void adapter_wgrad_tile_bf16(const AdaptGrad& p, floa
     const void* src = isA ? p.x : p.dy;
     const long long ld = isA ? p.ldx : p.lddy;
     const float* T = isA ? p.u : p.t;
-    for (int q = threadIdx.x; q < chunk.z; q += 256) rows[q] = p.plan[p.o_order + chunk.y + q];
+    // the chunk's rows, and of kept rows the scales of the tile's blocks of 32 channels, once for all batches
+    unsigned char* const scales = reinterpret_cast<unsigned char*>(rows + AD_CHUNK);
+    for (int q = threadIdx.x; q < chunk.z; q += 256) {
+        const int row = p.plan[p.o_order + chunk.y + q];
+        rows[q] = row;
+        if constexpr (KEPT) {
+#pragma unroll
+            for (int b = 0; b < CW / 2; ++b) scales[b * AD_CHUNK + q] = p.exps[(size_t)min(c0 / 32 + b, (width - 1) / 32) * p.lde + row];
+        }
+    }
     __syncthreads();
+    const unsigned char* const scale = scales + (CW * i / 32) * AD_CHUNK;
     f32x4 acc[RB][CW];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
@@ -657,8 +679,9 @@ __device__ __forceinline__ void adapter_wgrad_tile_bf16(const AdaptGrad& p, floa
     auto fetch = [&](Batch& b, int q0) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {                        // (rows beyond the chunk: the last one, counted as zeros)
-            const size_t row = (size_t)rows[min(q0 + 8 * g + e, chunk.z - 1)];
-            b.x[e].load(p, src, ld, row, c0 + CW * i, width);
+            const int at = min(q0 + 8 * g + e, chunk.z - 1);
+            const size_t row = (size_t)rows[at];
+            b.x[e].load(p, src, ld, row, c0 + CW * i, width, scale + at);
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) b.t[rb][e] = T[row * p.rank + min(r0 + rb * 16 + i, p.rank - 1)];
         }
@@ -705,14 +728,10 @@ __device__ __forceinline__ void adapter_wgrad_tile_bf16(const AdaptGrad& p, floa
         }
     };
     if (chunk.z > 0) {
-        Batch b[2];
-        int q = wave * 32;
-        if (q < chunk.z) fetch(b[0], q);
-        for (; q < chunk.z; q += 2 * STEP) {
-            if (q + STEP < chunk.z) fetch(b[1], q + STEP);
-            multiply(b[0], q);
-            if (q + 2 * STEP < chunk.z) fetch(b[0], q + 2 * STEP);
-            if (q + STEP < chunk.z) multiply(b[1], q + STEP);
+        for (int q = wave * 32; q < chunk.z; q += STEP) {
+            Batch b;
+            fetch(b, q);
+            multiply(b, q);
         }
     }
     adapter_wgrad_finish<JM_BF16, RB, CW>(p, lds, chunk, ad, isA, c0, r0, acc);
@@ -722,7 +741,7 @@ template <int TY, bool KEPT, int RB, int CW>
 __global__ void __launch_bounds__(256)
 adapter_wgrad_kernel(AdaptGrad p) {
     __shared__ __attribute__((aligned(16))) float lds[4 * 16 * RB * 16 * CW];       // the rows of the chunk, then the waves' tiles
-    static_assert(sizeof(lds) >= AD_CHUNK * sizeof(int), "the row list is kept there");
+    static_assert(sizeof(lds) >= AD_CHUNK * (sizeof(int) + CW / 2), "the row list and the scales are kept there");
     int ad = 0;
     int4 chunk;
     if (p.direct) {
