@@ -42,10 +42,14 @@ def _weights(a, b, scales, plan, dtype, k: int, n: int, m: int):
     """checks of the adapters' tensors -> (rank, adapters)"""
     if not isinstance(plan, AdapterPlan):
         raise TypeError(f"plan: expected AdapterPlan, got {type(plan).__name__}")
-    _on_device(plan.data, "plan")
-    _on_device(a, "a")
-    _on_device(b, "b")
-    _on_device(scales, "scales")
+    dev = L._current_device()
+    try:
+        here = plan.data.get_device() == dev and a.get_device() == dev and b.get_device() == dev and scales.get_device() == dev
+    except AttributeError:
+        here = False
+    if not here:
+        for v, name in ((plan.data, "plan"), (a, "a"), (b, "b"), (scales, "scales")):
+            _on_device(v, name)
     if a.dtype != dtype or b.dtype != dtype:
         raise TypeError(f"a and b must be {dtype} like the rows, got {a.dtype} and {b.dtype}")
     if a.dim() != 3 or not a.is_contiguous() or b.dim() != 3 or not b.is_contiguous():
@@ -91,7 +95,7 @@ def _result(base, out, m: int, n: int, like: torch.Tensor, others):
         if mb != m or nb != n:
             raise ValueError(f"base {tuple(base.shape)}: expected ({m}, {n})")
     if out is None:
-        out = torch.empty((m, n), dtype=like.dtype, device=like.device)
+        out = torch.empty_like(base) if ldb == n else torch.empty((m, n), dtype=like.dtype, device=like.device)
         return pb, ldb, out, out.data_ptr(), n
     if out is base:
         po, ldo = pb, ldb

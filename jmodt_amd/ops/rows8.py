@@ -33,6 +33,13 @@ def _on_device(t, name: str) -> None:
 
 def _matrix(t, name: str, dtype: Optional[torch.dtype] = None) -> Tuple[int, int, int, int]:
     """(rows, channels, address, row stride) of a 2-D row tensor: unit column stride, any row stride >= its width, any alignment"""
+    try:
+        if t.get_device() == L._current_device() and t.dim() == 2 and t.is_contiguous() and (t.dtype is dtype or (dtype is None and t.dtype in TYPES)):
+            m, c = t.shape
+            if c:
+                return m, c, t.data_ptr(), c
+    except AttributeError:
+        pass                                                 # (not a tensor: refused below, like everything else that is not the usual case)
     _on_device(t, name)
     if t.dim() != 2:
         raise TypeError(f"{name} must be 2-D (rows, channels), got {tuple(t.shape)}")
@@ -42,8 +49,6 @@ def _matrix(t, name: str, dtype: Optional[torch.dtype] = None) -> Tuple[int, int
     elif t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     m, c = t.shape
-    if t.is_contiguous() and c:
-        return m, c, t.data_ptr(), c
     if c == 0:
         raise ValueError(f"{name} has no channels")
     if c > 1 and t.stride(1) != 1:
@@ -116,7 +121,8 @@ def _kept(x8, name: str) -> Tuple[int, int, int, int, int, int]:
     """(rows, channels, address of the codes, bytes of their rows, address of the scales, bytes of their columns)"""
     if not isinstance(x8, Rows8):
         raise TypeError(f"{name}: expected Rows8, got {type(x8).__name__}")
-    _on_device(x8.data, name)
+    if x8.data.get_device() != L._current_device():
+        _on_device(x8.data, name)
     m, c = x8.shape
     ld = (c + 15) & ~15
     p = x8.data.data_ptr()
