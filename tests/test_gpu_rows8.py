@@ -248,3 +248,16 @@ def test_refusals():
         R8.Rows8.from_codes(k.codes.int(), k.exps)
     again = R8.Rows8.from_codes(k.codes[:, :20], k.exps)
     assert torch.equal(again.codes, k.codes) and torch.equal(again.exps, k.exps) and again.nbytes() == k.nbytes()
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,c", [(1, 1), (3, 1), (9, 2), (40, 3), (5, 9), (2, 33)])
+def test_keep_at_the_end_of_a_buffer(m, c, dtype):
+    """rows that end where their storage ends, between guard values that must neither be used nor changed"""
+    buf = torch.full((m * c + 64,), float("nan"), device="cuda", dtype=dtype)
+    x = buf[32:32 + m * c].view(m, c)
+    x.copy_(make(m, c, dtype, seed=m * c))
+    k = R8.checkpoint_rows(x)
+    codes, exps = encode_ref(x)
+    assert np.array_equal(codes & 127, k.codes.cpu().numpy()[:, :c] & 127) and np.array_equal(exps, k.exps.cpu().numpy())
+    assert torch.isnan(buf[:32]).all() and torch.isnan(buf[32 + m * c:]).all()
