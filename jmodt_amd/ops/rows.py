@@ -210,11 +210,20 @@ class _RowsMLP(Function):
 
 
 def rows_mlp(x1: torch.Tensor, layers: Sequence[Tuple[torch.Tensor, Optional[torch.Tensor]]], acts: Sequence[int],
-             x2: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """[x1 | x2] (M, k1 + k2) through the dense layers [(W (n, k), b (n) or None), ...] with activations acts"""
+             x2: Optional[torch.Tensor] = None, keep: str = "float32") -> torch.Tensor:
+    """[x1 | x2] (M, k1 + k2) through the dense layers [(W (n, k), b (n) or None), ...] with activations acts.
+    keep: what the backward finds of the inputs and the hidden activations — "float32": themselves; "e4m3": their 8-bit form
+    (ops/rows8.py: a quarter of the memory, weight gradients from the rounded activations, everything else as before; no tanh)"""
     flat = []
     for W, b in layers:
         flat += [W, b]
+    if keep == "e4m3":
+        from .rows8 import _RowsMLP8
+        if any(int(a) not in (0, 1) for a in acts):
+            raise ValueError("keep='e4m3' takes layers without activation or with ReLU (the gradient of tanh needs its output)")
+        return _RowsMLP8.apply(x1, x2, tuple(int(a) for a in acts), *flat)
+    if keep != "float32":
+        raise ValueError(f"keep must be 'float32' or 'e4m3', got {keep!r}")
     return _RowsMLP.apply(x1, x2, tuple(int(a) for a in acts), *flat)
 
 

@@ -13,6 +13,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import Function
 
 from .. import _lib as L
 
@@ -151,30 +152,92 @@ def restore_rows(x8: Rows8, dtype: torch.dtype = _f32) -> torch.Tensor:
     return out
 
 
-def relu_mask8(dy: torch.Tensor, y8: Rows8) -> torch.Tensor:
-    """kept y > 0 ? dy : 0 as a new float32 tensor: the gradient through a ReLU from its kept output"""
+def relu_mask8(dy: torch.Tensor, y8: Rows8, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """kept y > 0 ? dy : 0 in float32 (a new tensor, or `out`, which may be dy): the gradient through a ReLU from its kept output"""
     m, c, pdy, ldd = _matrix(dy, "dy", _f32)
     m8, c8, pc, ld, _, _ = _kept(y8, "y8")
     if (m, c) != (m8, c8):
         raise ValueError(f"dy {tuple(dy.shape)} for a kept output {y8.shape}")
-    out = torch.empty((m, c), dtype=_f32, device=dy.device)
-    L.check(L.load().jm_rows8_relu_mask(m, c, pdy, ldd, pc, ld, out.data_ptr(), c, L.stream_ptr()), "relu_mask8")
+    if out is None:
+        out = torch.empty((m, c), dtype=_f32, device=dy.device)
+    mo, co, po, ldo = _matrix(out, "out", _f32)
+    if (mo, co) != (m, c):
+        raise ValueError(f"out {tuple(out.shape)}: expected ({m}, {c})")
+    L.check(L.load().jm_rows8_relu_mask(m, c, pdy, ldd, pc, ld, po, ldo, L.stream_ptr()), "relu_mask8")
     return out
 
 
-def linear_wgrad8(dy: torch.Tensor, x8: Rows8, want_bias: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+def linear_wgrad8(dy: torch.Tensor, x8: Rows8, want_bias: bool = True, out: Optional[torch.Tensor] = None,
+                  col0: int = 0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(dw (N, K) = dy^T x, dbias (N) or None) in float32, dy (M, N) float32 / bfloat16 / float16, x (M, K) kept: ops.rows.linear_wgrad
-    with the input as `checkpoint_rows` left it"""
+    with the input as `checkpoint_rows` left it.  out / col0: write the block into columns col0 .. of an (N, >= col0 + K) tensor."""
     m, n, pdy, ldd = _matrix(dy, "dy")
     m8, k, pc, ld, pe, mp = _kept(x8, "x8")
     if m8 != m:
         raise ValueError(f"dy of {m} rows for a kept input of {m8}")
     lib = L.load()
     device = dy.device
-    dw = torch.empty((n, k), dtype=_f32, device=device)
+    if out is None:
+        dw = torch.empty((n, k), dtype=_f32, device=device)
+        pw, ldw = dw.data_ptr(), k
+    else:
+        dw = out
+        nw, kw, pw, ldw = _matrix(out, "out", _f32)
+        if nw != n or col0 < 0 or col0 + k > kw:
+            raise ValueError(f"out {tuple(out.shape)} for columns {col0} .. {col0 + k - 1} of ({n}, ...)")
+        pw += 4 * col0
     db = torch.empty((n,), dtype=_f32, device=device) if want_bias else None
     nbytes = lib.jm_rows8_wgrad_workspace_bytes(m, n, k)
     ws = torch.empty((nbytes // 4,), dtype=_f32, device=device) if nbytes else None
-    L.check(lib.jm_rows8_linear_wgrad(m, n, k, TYPES[dy.dtype], pdy, ldd, pc, ld, pe, mp, dw.data_ptr(), k, db.data_ptr() if want_bias else None,
+    L.check(lib.jm_rows8_linear_wgrad(m, n, k, TYPES[dy.dtype], pdy, ldd, pc, ld, pe, mp, pw, ldw, db.data_ptr() if want_bias else None,
                                       ws.data_ptr() if nbytes else None, nbytes, L.stream_ptr()), "linear_wgrad8")
     return dw, db
+
+
+class _RowsMLP8(Function):
+    """ops.rows._RowsMLP with its inputs and its hidden activations kept in 8 bits: apply(x1, x2 or None, acts, W_0, b_0, W_1, b_1, ...), acts
+    in {0 none, 1 ReLU}.  The forward's values are the float32 route's own; of the gradients only dW_l see the rounding of the kept
+    activations (the masks are exact, dx and db need none of them)."""
+
+    @staticmethod
+    def forward(ctx, x1, x2, acts, *wb):
+        from . import rows as R
+        Ws, bs = wb[0::2], wb[1::2]
+        kept = [checkpoint_rows(x1)] + ([checkpoint_rows(x2)] if x2 is not None else [])
+        cur, cur2 = x1, x2
+        for l, act in enumerate(acts):
+            cur, cur2 = R.linear_forward(cur, Ws[l], bs[l], act, x2=cur2), None
+            if act == 1 or l + 1 < len(acts):
+                kept.append(checkpoint_rows(cur))
+        ctx.acts, ctx.has_x2, ctx.has_b = acts, x2 is not None, tuple(b is not None for b in bs)
+        ctx.shapes = [k.shape for k in kept]
+        ctx.save_for_backward(*[k.data for k in kept], *Ws)
+        return cur
+
+    @staticmethod
+    def backward(ctx, dy):
+        from . import rows as R
+        nk, acts, need = len(ctx.shapes), ctx.acts, ctx.needs_input_grad
+        kept = [Rows8(d, *s) for d, s in zip(ctx.saved_tensors[:nk], ctx.shapes)]
+        Ws = ctx.saved_tensors[nk:]
+        inputs, ys = kept[:2 if ctx.has_x2 else 1], kept[2 if ctx.has_x2 else 1:]
+        if dy.stride(1) != 1 or dy.stride(0) % 4 or dy.stride(0) < dy.shape[1] or dy.data_ptr() % 16:
+            dy = dy.contiguous()
+        if acts[-1] == 1:
+            dy = relu_mask8(dy, ys[-1])
+        grads = [None] * (2 * len(acts))
+        for l in range(len(acts) - 1, 0, -1):
+            if need[3 + 2 * l] or need[4 + 2 * l]:
+                grads[2 * l], grads[2 * l + 1] = linear_wgrad8(dy, ys[l - 1], want_bias=ctx.has_b[l])
+            dy = R.linear_dgrad(dy, Ws[l], 0, Ws[l].shape[1])
+            if acts[l - 1] == 1:
+                relu_mask8(dy, ys[l - 1], out=dy)
+        if need[3] or need[4]:
+            dw = torch.empty(Ws[0].shape, dtype=_f32, device=dy.device)
+            k1 = inputs[0].shape[1]
+            grads[0], grads[1] = linear_wgrad8(dy, inputs[0], want_bias=ctx.has_b[0], out=dw)
+            if ctx.has_x2:
+                linear_wgrad8(dy, inputs[1], want_bias=False, out=dw, col0=k1)
+        dx1 = R.linear_dgrad(dy, Ws[0], 0, inputs[0].shape[1]) if need[0] else None
+        dx2 = R.linear_dgrad(dy, Ws[0], inputs[0].shape[1], inputs[1].shape[1]) if ctx.has_x2 and need[1] else None
+        return (dx1, dx2, None, *grads)

@@ -128,7 +128,7 @@ def prepare_rows(engine) -> None:
 
 
 def joint_step(engine, xyz, image, pts_xy, gt_tids, optimizer, world: Optional[int] = None, rois_per_frame: int = 64,
-               bucket_bytes: int = 64 << 20, route: str = "auto", next_xyz=None, local: bool = False) -> torch.Tensor:
+               bucket_bytes: int = 64 << 20, route: str = "auto", next_xyz=None, local: bool = False, keep: str = "float32") -> torch.Tensor:
     """one data-parallel joint-mode step on this rank's frames: differentiable forward, thin loss, backward through the whole
     detector, the gradient of every parameter all-reduced in 64 MiB buckets (66.9 MB at the reference widths: ONE
     collective), optimizer step.  Returns the local loss (device scalar, detached).
@@ -137,7 +137,8 @@ def joint_step(engine, xyz, image, pts_xy, gt_tids, optimizer, world: Optional[i
     "operators" = the un-fused operator route above (torch autograd over (B, C, npoint, nsample) tensors; any BatchNorm mode),
     "auto" = rows whenever the BatchNorms are frozen (the faster of the two: DESIGN.md section 6; the HIP-graph form of the rows route
     measured slower than eager and lives under tools/quarantine/).  next_xyz: the next batch's cloud — its FPS pyramid / neighbour search
-    starts on the side stream under this step (rows route).  world / local: see dist.group_world."""
+    starts on the side stream under this step (rows route).  world / local: see dist.group_world.  keep (rows route): "e4m3" = the
+    dense layers keep their activations in 8 bits for the backward (train_rows.joint_forward_rows)."""
     import torch.distributed as tdist
     from .ops.affinity_train import AffinityTrainState
     params = [p for p in _engine_lists(engine)[1] if p.requires_grad]
@@ -150,11 +151,13 @@ def joint_step(engine, xyz, image, pts_xy, gt_tids, optimizer, world: Optional[i
         route = "rows" if frozen_bn(engine) and xyz.is_cuda else "operators"
     if route not in ("rows", "operators"):
         raise ValueError(f"joint_step: route {route!r} (rows | operators | auto)")
+    if keep != "float32" and route != "rows":
+        raise ValueError(f"joint_step: keep={keep!r} belongs to the rows route, this one is {route!r}")
     if route == "rows":
         if not frozen_bn(engine):
             raise RuntimeError("joint_step(route='rows') folds the BatchNorms: call train_joint.freeze_bn(engine) (or engine.eval()) first")
         loss = prof.region("joint_forward+backward(span)", lambda: _rows_forward_backward(engine, xyz, image, pts_xy, gt_tids, world, local,
-                                                                                        rois_per_frame, next_xyz))
+                                                                                        rois_per_frame, next_xyz, keep))
     else:
         out = prof.region("joint_forward(span)", lambda: joint_forward(engine, xyz, image, pts_xy, rois_per_frame))
         counts = None
@@ -173,7 +176,7 @@ def joint_step(engine, xyz, image, pts_xy, gt_tids, optimizer, world: Optional[i
     return loss.detach()
 
 
-def _rows_forward_backward(engine, xyz, image, pts_xy, gt_tids, world, local, rois_per_frame, next_xyz):
+def _rows_forward_backward(engine, xyz, image, pts_xy, gt_tids, world, local, rois_per_frame, next_xyz, keep="float32"):
     """forward and backward of the rows route, issued in the order that keeps three streams busy: backbone + RPN heads forward
     (main / image streams) -> proposals + RoI pooling (no gradient) -> the BACKWARD of the RPN part of the loss (main / image
     streams: the loss is a sum, its parts back-propagate independently) -> RCNN forward, its loss and backward on the RCNN stream,
@@ -185,7 +188,7 @@ def _rows_forward_backward(engine, xyz, image, pts_xy, gt_tids, world, local, ro
     pyr = engine._take_prefetched(xyz)
     if next_xyz is not None:
         engine.prefetch(next_xyz, None)
-    fold = BnFold(engine.rpn)                   # (the RCNN branch folds its own BatchNorms, on its stream, into its own graph)
+    fold = BnFold(engine.rpn, keep=keep)        # (the RCNN branch folds its own BatchNorms, on its stream, into its own graph)
     out = rpn_forward_rows(engine, xyz, image, pts_xy, fold, pyr)
     rois, pts_input, count = pooled_rois(engine, xyz, out, rois_per_frame)
     pooled_ev = torch.cuda.Event()
@@ -196,7 +199,7 @@ def _rows_forward_backward(engine, xyz, image, pts_xy, gt_tids, world, local, ro
     B = gt_tids.shape[0]
 
     def rcnn_half():
-        rc = rcnn_branch_rows(engine, pts_input, count, ready=pooled_ev)
+        rc = rcnn_branch_rows(engine, pts_input, count, ready=pooled_ev, keep=keep)
         side = rc.pop("_stream")
         with torch.cuda.stream(side):
             feats = rc["rcnn_feat"].view(B, -1, rc["rcnn_feat"].shape[-1])

@@ -69,9 +69,11 @@ class BnFold:
     W * s[:, None] from ONE multi-tensor kernel (ops/rows.fold_all) whose backward — d(W) = d(Wf) * s, d(s) = rowsum(d(Wf) * W) —
     is one more.  Differentiable w.r.t. W, gamma, beta (the running statistics are buffers)."""
 
-    def __init__(self, root, pairs=None):
+    def __init__(self, root, pairs=None, keep="float32"):
         """root: the module whose BatchNorms are folded — or `pairs`, an explicit [(convolution, BatchNorm)] list (a section of
-        the network: tools/quarantine/train_graphs.py)"""
+        the network: tools/quarantine/train_graphs.py).  keep: how the dense layers that run on this fold's weights keep their
+        activations for the backward (ops.rows.rows_mlp)"""
+        self.keep = keep
         pairs = bn_pairs(root) if pairs is None else list(pairs)
         self._slots = {}
         if not pairs:
@@ -156,7 +158,7 @@ def _head_rows(fold: BnFold, head: nn.Sequential, x: torch.Tensor) -> torch.Tens
         if isinstance(m, nn.Dropout):
             if m.training and m.p > 0:
                 if cur_layers:
-                    out = R.rows_mlp(out, cur_layers, cur_acts)
+                    out = R.rows_mlp(out, cur_layers, cur_acts, keep=fold.keep)
                     cur_layers, cur_acts = [], []
                 out = F.dropout(out, m.p, True)
             continue
@@ -164,7 +166,7 @@ def _head_rows(fold: BnFold, head: nn.Sequential, x: torch.Tensor) -> torch.Tens
         cur_layers.append(_pad_rows(W, b))
         cur_acts.append(1 if getattr(m, "activation", None) is not None else 0)
     if cur_layers:
-        out = R.rows_mlp(out, cur_layers, cur_acts)
+        out = R.rows_mlp(out, cur_layers, cur_acts, keep=fold.keep)
     return out
 
 
@@ -181,9 +183,9 @@ def _attention_rows(fold: BnFold, mod, point: torch.Tensor, img: torch.Tensor) -
     z = R.rows_mlp(t, [_pad_rows(w3, ia.fc3.bias)], [0])                                        # (M, 4): column 0 is the logit
     gate = torch.sigmoid(z[:, :1])
     Wi, bi = fold.conv(ia.conv1[0], ia.conv1[1])
-    j = R.rows_mlp(img, [(Wi, bi)], [1]) * gate
+    j = R.rows_mlp(img, [(Wi, bi)], [1], keep=fold.keep) * gate
     Wf, bf = fold.conv(mod.conv1, mod.bn1)
-    return R.rows_mlp(point, [(Wf, bf)], [1], x2=j)
+    return R.rows_mlp(point, [(Wf, bf)], [1], x2=j, keep=fold.keep)
 
 
 def _sa_level_rows(fold: BnFold, sa, xyz: torch.Tensor, feats: Optional[torch.Tensor], new_xyz: torch.Tensor, grid=None,
@@ -301,7 +303,7 @@ def _image_fusion_map(fold: BnFold, net, maps: List[torch.Tensor]) -> torch.Tens
         # the 1 x 1 fusion convolution + bias + ReLU IS a dense layer on the (B H W, C) rows of the channels-last map: one bounds-checked
         # GEMM launch per direction (csrc/rows_gemm.hip) instead of a library convolution, a bias / ReLU pass and a channel sum
         B, ctot, H, W = de.shape
-        y = R.rows_mlp(de.permute(0, 2, 3, 1).reshape(B * H * W, ctot), [(Wf2, b_eff)], [1])  # (B H W, q)
+        y = R.rows_mlp(de.permute(0, 2, 3, 1).reshape(B * H * W, ctot), [(Wf2, b_eff)], [1], keep=fold.keep)  # (B H W, q)
         return y.view(B, H, W, Wf2.shape[0]).permute(0, 3, 1, 2)                              # = channels-last (B, q, H, W)
     return _BiasReluInplace.apply(F.conv2d(de, Wf, None), b_eff)
 
@@ -374,7 +376,7 @@ def backbone_forward_rows(engine, xyz: torch.Tensor, image: torch.Tensor, pts_xy
             carried = R.three_interpolate_rows(l_feats[i], nn3, w)
             mlp = net.FP_modules[i].mlp
             layers = [fold.unit(u) for u in mlp]
-            l_feats[i - 1] = R.rows_mlp(carried, layers, [1] * len(layers), x2=l_feats[i - 1])
+            l_feats[i - 1] = R.rows_mlp(carried, layers, [1] * len(layers), x2=l_feats[i - 1], keep=fold.keep)
     main.wait_event(fused_ev)
     with prof.scope("li_fusion_final"):
         out = _attention_rows(fold, net.final_fusion_img_point, l_feats[0], R.feature_gather_rows(fused_img, pts_xy))
@@ -416,9 +418,9 @@ def rcnn_forward_rows(engine, pts_input: torch.Tensor, fold: BnFold, count: Opti
     up = [fold.unit(u) for u in net.xyz_up_layer]
     W0, b0 = up[0]
     up[0] = (_pad_dim(W0, 1, x5.shape[1] - W0.shape[1]), b0)
-    xyz_feat = R.rows_mlp(x5, up, [1] * len(up))
+    xyz_feat = R.rows_mlp(x5, up, [1] * len(up), keep=fold.keep)
     Wm, bm = fold.unit(net.merge_down_layer[0])
-    feats = R.rows_mlp(xyz_feat, [(Wm, bm)], [1], x2=rpn_feat)              # (R S, C): merge_down on [xyz_feature | rpn_feature]
+    feats = R.rows_mlp(xyz_feat, [(Wm, bm)], [1], x2=rpn_feat, keep=fold.keep)              # (R S, C): merge_down on [xyz_feature | rpn_feature]
     l_xyz = xyz
     canon = None
     if count is not None:
@@ -480,7 +482,7 @@ def pooled_rois(engine, xyz, rpn_out: Dict[str, torch.Tensor], rois_per_frame: i
     return rois, pooled.view(-1, cfg.rcnn_num_points, pooled.shape[-1]), count.view(-1)
 
 
-def rcnn_branch_rows(engine, pts_input, count, fold: Optional[BnFold] = None, ready: Optional[torch.cuda.Event] = None) -> Dict[str, torch.Tensor]:
+def rcnn_branch_rows(engine, pts_input, count, fold: Optional[BnFold] = None, ready: Optional[torch.cuda.Event] = None, keep: str = "float32") -> Dict[str, torch.Tensor]:
     """stream R: the RCNN (rcnn.py:158-202).  Its BACKWARD then runs there too (autograd: a node's backward on its forward's
     stream), next to the backbone's backward on the main stream — neither feeds the other: roipool3d has no gradient.  The
     caller's stream waits for the outputs (main.wait_stream) before it reads them.
@@ -497,7 +499,7 @@ def rcnn_branch_rows(engine, pts_input, count, fold: Optional[BnFold] = None, re
     else:
         side.wait_stream(main)
     with torch.cuda.stream(side):
-        out = rcnn_forward_rows(engine, pts_input, BnFold(engine.rcnn_net) if fold is None else fold, count)
+        out = rcnn_forward_rows(engine, pts_input, BnFold(engine.rcnn_net, keep=keep) if fold is None else fold, count)
     if side is not main:
         pts_input.record_stream(side)
         count.record_stream(side)
@@ -505,15 +507,18 @@ def rcnn_branch_rows(engine, pts_input, count, fold: Optional[BnFold] = None, re
     return out
 
 
-def joint_forward_rows(engine, xyz, image, pts_xy, rois_per_frame: int = 64, pyr: Optional[FpsPyramid] = None) -> Dict[str, torch.Tensor]:
+def joint_forward_rows(engine, xyz, image, pts_xy, rois_per_frame: int = 64, pyr: Optional[FpsPyramid] = None,
+                       keep: str = "float32") -> Dict[str, torch.Tensor]:
     """the detector in TRAIN composition (point_rcnn.py:24-70) on rows; same outputs as train_joint.joint_forward.
     Its backward runs on three streams (main, image, RCNN), each node on the stream of its forward; gradients cross streams only
     through the autograd engine's own hand-over.  Safe next to other live autograd graphs over the same parameters (an earlier
-    step's outputs, DDP's stashed AccumulateGrad nodes: tests/test_gpu_rows.py holds two of them across ten asynchronous steps)."""
-    fold = BnFold(engine.rpn)
+    step's outputs, DDP's stashed AccumulateGrad nodes: tests/test_gpu_rows.py holds two of them across ten asynchronous steps).
+    keep: "e4m3" = the dense layers keep their activations in 8 bits for the backward (ops.rows.rows_mlp; the set-abstraction scales and
+    the attention's tanh layer stay in float32)."""
+    fold = BnFold(engine.rpn, keep=keep)
     out = rpn_forward_rows(engine, xyz, image, pts_xy, fold, pyr)
     rois, pts_input, count = pooled_rois(engine, xyz, out, rois_per_frame)
-    rc = rcnn_branch_rows(engine, pts_input, count)
+    rc = rcnn_branch_rows(engine, pts_input, count, keep=keep)
     side = rc.pop("_stream")
     main = torch.cuda.current_stream(xyz.device)
     if side is not main:
