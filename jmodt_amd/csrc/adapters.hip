@@ -25,6 +25,8 @@ constexpr int AD_WIDE_ROWS = 16384;
 // rows of a tile: 16 while that leaves CUs idle, 32 where there are enough tiles (A and B are read once a tile)
 static __host__ __device__ __forceinline__ int ad_tile(int m) { return m < AD_WIDE_ROWS ? 16 : 32; }
 constexpr int AD_CHUNK = 512;       // rows of a chunk (weight gradients)
+constexpr int AD_GATHER_ROWS = 2048;        // up to here the backward gathers A and B transposed instead of transposing them first
+static_assert(AD_GATHER_ROWS < AD_WIDE_ROWS, "there tiles have 16 rows");
 constexpr int AD_MAX_ROWS = 1 << 30, AD_MAX_WIDTH = 1 << 20;        // tile counts, grids and per-adapter element counts stay in range
 
 struct PlanLayout {                  // offsets in ints; header: [0] tiles, [1] chunks
@@ -237,7 +239,9 @@ struct Run16 {
 // t enters the second product as the sum of two values of the 16-bit type (16 significant bits in bfloat16, 22 in float16, where the
 // row is scaled by a power of two first: t may leave float16's range although out does not); as it is in float32.  With a rank of up
 // to 16 both values share one product: the contraction is 32 long, [hi | lo] times [B | B].
-template <int TY, int RB, int MB>
+// WT: A and B are given transposed, (k, rank) and (rank, n) — the backward on B and A as they are: their elements are gathered one by one,
+// which few tiles can afford and many cannot (there a kernel of its own transposes them first).
+template <int TY, int RB, int MB, bool WT>
 __global__ void __launch_bounds__(256)
 adapter_rows_kernel(Adapt p) {
     typedef typename Elem<TY>::T T;
@@ -290,7 +294,25 @@ adapter_rows_kernel(Adapt p) {
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) xr[mb] = (const T*)p.x + row[mb] * p.ldx + 8 * g;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) ar[rb] = A + (size_t)min(rb * 16 + i, p.rank - 1) * p.k + 8 * g;
+        for (int rb = 0; rb < RB; ++rb) {
+            const int r = min(rb * 16 + i, p.rank - 1);
+            ar[rb] = WT ? A + (size_t)(8 * g) * p.rank + r : A + (size_t)r * p.k + 8 * g;
+        }
+        // elements 0 .. left - 1 (of 8) of step s; WT: A lies as (k, rank)
+        auto load_a = [&](const T* q, int s, int left) __attribute__((always_inline)) {
+            if constexpr (WT) {
+                V8 v;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    T t = (T)0.f;
+                    if (e < left) t = q[(size_t)(32 * s + e) * p.rank];
+                    v[e] = t;
+                }
+                return v;
+            } else {
+                return load8_upto<V8>(q + 32 * s, left);
+            }
+        };
         f32x4 acc[MB][RB];
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb)
@@ -307,7 +329,7 @@ adapter_rows_kernel(Adapt p) {
 #pragma unroll
                 for (int mb = 0; mb < MB; ++mb) xv[u][mb] = load8<V8>(xr[mb] + 32 * (s + u));
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) av[u][rb] = load8<V8>(ar[rb] + 32 * (s + u));
+                for (int rb = 0; rb < RB; ++rb) av[u][rb] = load_a(ar[rb], s + u, 8);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -328,7 +350,7 @@ adapter_rows_kernel(Adapt p) {
             for (int mb = 0; mb < MB; ++mb) xv[mb] = load8_upto<V8>(xr[mb] + 32 * s, left);
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
-                const V8 av = load8_upto<V8>(ar[rb] + 32 * s, left);
+                const V8 av = load_a(ar[rb], s, left);
 #pragma unroll
                 for (int mb = 0; mb < MB; ++mb) acc[mb][rb] = mma16(acc[mb][rb], av, xv[mb]);
             }
@@ -412,7 +434,8 @@ adapter_rows_kernel(Adapt p) {
         f32x4 d[MB][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const T* Br = B + (size_t)min(n0 + (i >> 2) * 16 + j * 4 + (i & 3), p.n - 1) * p.rank;
+            const int bc = min(n0 + (i >> 2) * 16 + j * 4 + (i & 3), p.n - 1);
+            const T* Br = WT ? B + bc : B + (size_t)bc * p.rank;           // WT: B lies as (rank, n)
 #pragma unroll
             for (int mb = 0; mb < MB; ++mb) d[mb][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -420,17 +443,27 @@ adapter_rows_kernel(Adapt p) {
                 if constexpr (TY == JM_F32) {
                     const int r0 = s * 16 + 4 * g;
                     f32x4 b4;
-                    if (r0 + 4 <= p.rank) __builtin_memcpy(&b4, Br + r0, 16);
+                    if (!WT && r0 + 4 <= p.rank) __builtin_memcpy(&b4, Br + r0, 16);
                     else
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) b4[e] = r0 + e < p.rank ? Br[r0 + e] : 0.f;
+                        for (int e = 0; e < 4; ++e) b4[e] = r0 + e < p.rank ? (WT ? Br[(size_t)(r0 + e) * p.n] : Br[r0 + e]) : 0.f;
 #pragma unroll
                     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) d[mb][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(b4[e], t32[mb][s][e], d[mb][j], 0, 0, 0);
                 } else {
                     const int r0 = PAIR ? 8 * (g & 1) : s * 32 + 8 * g;
-                    const V8 b8 = load8_upto<V8>(Br + r0, p.rank - r0);
+                    V8 b8;
+                    if constexpr (WT) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            T t = (T)0.f;
+                            if (r0 + e < p.rank) t = Br[(size_t)(r0 + e) * p.n];
+                            b8[e] = t;
+                        }
+                    } else {
+                        b8 = load8_upto<V8>(Br + r0, p.rank - r0);
+                    }
 #pragma unroll
                     for (int mb = 0; mb < MB; ++mb) {
                         d[mb][j] = mma16(d[mb][j], b8, hi[mb][s]);
@@ -544,15 +577,17 @@ __device__ __forceinline__ void adapter_wgrad_finish(const AdaptGrad& p, float* 
     constexpr int TR = 16 * RB, TC = 16 * CW;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6, width = isA ? p.k : p.n;
     __syncthreads();
-    // D: rows = rank index 4 g + q, column i = channel CW i + j of the tile
+    // D: rows = rank index 4 g + q, column i = channel CW i + j of the tile.  Row r of a tile is turned by 4 r columns, so that it can be read
+    // down the ranks, too (dB) without its lanes meeting in one bank
     float* const mine = lds + wave * TR * TC;
+    auto place = [&](int r, int c) { return r * TC + ((c + 4 * r) & (TC - 1)); };
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int j = 0; j < CW; j += 4)
-                *reinterpret_cast<f32x4*>(mine + (rb * 16 + 4 * g + q) * TC + CW * i + j) = f32x4{acc[rb][j][q], acc[rb][j + 1][q], acc[rb][j + 2][q], acc[rb][j + 3][q]};
+                *reinterpret_cast<f32x4*>(mine + place(rb * 16 + 4 * g + q, CW * i + j)) = f32x4{acc[rb][j][q], acc[rb][j + 1][q], acc[rb][j + 2][q], acc[rb][j + 3][q]};
     __syncthreads();
     typedef typename Elem<TY>::T E;
     float* part = p.part + (size_t)blockIdx.x * p.rank * ((size_t)p.k + p.n);
@@ -560,7 +595,7 @@ __device__ __forceinline__ void adapter_wgrad_finish(const AdaptGrad& p, float* 
     for (int e = threadIdx.x; e < TR * TC; e += 256) {       // (dA runs along the channels, dB along the rank)
         const int rt = isA ? e / TC : e % TR, ct = isA ? e % TC : e / TR, r = r0 + rt, c = c0 + ct;
         if (r >= p.rank || c >= width) continue;
-        const float* v = lds + rt * TC + ct;
+        const float* v = lds + place(rt, ct);
         const float sum = (v[0] + v[TR * TC]) + (v[2 * TR * TC] + v[3 * TR * TC]);
         const size_t at = isA ? (size_t)r * p.k + c : (size_t)c * p.rank + r;
         if (p.direct) ((E*)(isA ? p.da : p.db))[(size_t)ad * p.rank * width + at] = (E)(chunk.z > 0 ? scale * sum : 0.f);
@@ -757,11 +792,11 @@ adapter_wgrad_kernel(AdaptGrad p) {
     const bool isA = (int)blockIdx.y < tk;
     const int c0 = (isA ? (int)blockIdx.y : (int)blockIdx.y - tk) * 16 * CW;
     if constexpr (TY == JM_BF16 && CW == 8) {
-        if (isA) adapter_wgrad_tile_bf16<KEPT, RB>(p, lds, chunk, ad, true, c0, r0);
-        else adapter_wgrad_tile_bf16<false, RB>(p, lds, chunk, ad, false, c0, r0);
+        if (KEPT && isA) adapter_wgrad_tile_bf16<KEPT, RB>(p, lds, chunk, ad, true, c0, r0);
+        else adapter_wgrad_tile_bf16<false, RB>(p, lds, chunk, ad, isA, c0, r0);
     } else {
-        if (isA) adapter_wgrad_tile<TY, KEPT, RB, CW>(p, lds, chunk, ad, true, c0, r0);
-        else adapter_wgrad_tile<TY, false, RB, CW>(p, lds, chunk, ad, false, c0, r0);
+        if (KEPT && isA) adapter_wgrad_tile<TY, KEPT, RB, CW>(p, lds, chunk, ad, true, c0, r0);
+        else adapter_wgrad_tile<TY, false, RB, CW>(p, lds, chunk, ad, isA, c0, r0);
     }
 }
 
@@ -789,24 +824,25 @@ adapter_wgrad_reduce_kernel(AdaptGrad p) {
 static size_t elem_size(int type) { return type == JM_F32 ? 4 : 2; }
 
 template <int TY, int RB>
-static void launch_rows(const Adapt& p, dim3 grid, hipStream_t s) {
-    if (ad_tile(p.m) == 16) hipLaunchKernelGGL((adapter_rows_kernel<TY, RB, 1>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((adapter_rows_kernel<TY, RB, 2>), grid, dim3(256), 0, s, p);
+static void launch_rows(const Adapt& p, bool wt, dim3 grid, hipStream_t s) {
+    if (wt) hipLaunchKernelGGL((adapter_rows_kernel<TY, RB, 1, true>), grid, dim3(256), 0, s, p);
+    else if (ad_tile(p.m) == 16) hipLaunchKernelGGL((adapter_rows_kernel<TY, RB, 1, false>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((adapter_rows_kernel<TY, RB, 2, false>), grid, dim3(256), 0, s, p);
 }
 template <int TY>
-static void launch_rows(const Adapt& p, dim3 grid, hipStream_t s) {
-    if (p.rank <= 16) launch_rows<TY, 1>(p, grid, s);
-    else if (p.rank <= 32) launch_rows<TY, 2>(p, grid, s);
-    else if (p.rank <= 64) launch_rows<TY, 4>(p, grid, s);
-    else launch_rows<TY, 8>(p, grid, s);
+static void launch_rows(const Adapt& p, bool wt, dim3 grid, hipStream_t s) {
+    if (p.rank <= 16) launch_rows<TY, 1>(p, wt, grid, s);
+    else if (p.rank <= 32) launch_rows<TY, 2>(p, wt, grid, s);
+    else if (p.rank <= 64) launch_rows<TY, 4>(p, wt, grid, s);
+    else launch_rows<TY, 8>(p, wt, grid, s);
 }
-static void launch_rows(int type, const Adapt& p, int tiles, hipStream_t s) {
+static void launch_rows(int type, const Adapt& p, bool wt, int tiles, hipStream_t s) {
     // few tiles: several workgroups a tile, as far as there are channel blocks and idle CUs
     const int y = imax(1, (int)((long long)divup(p.n, 256) < 256 / tiles ? divup(p.n, 256) : 256 / tiles));
     const dim3 grid((unsigned)tiles, (unsigned)y);
-    if (type == JM_F32) launch_rows<JM_F32>(p, grid, s);
-    else if (type == JM_BF16) launch_rows<JM_BF16>(p, grid, s);
-    else launch_rows<JM_F16>(p, grid, s);
+    if (type == JM_F32) launch_rows<JM_F32>(p, wt, grid, s);
+    else if (type == JM_BF16) launch_rows<JM_BF16>(p, wt, grid, s);
+    else launch_rows<JM_F16>(p, wt, grid, s);
 }
 
 // rank indices and channels of a workgroup: 16 x 128, 32 x 128, 64 x 64 (accumulators of a wave: 32, 64, 64 registers); on the bf16 pipe, whose
@@ -877,7 +913,7 @@ int jm_adapter_forward(int m, int k, int n, int rank, int adapters, int type, co
     Adapt p{};
     p.m = m; p.k = k; p.n = n; p.rank = rank; p.plan = plan; p.o_order = l.order; p.o_tiles = l.tiles; p.x = x; p.ldx = ldx; p.a = a; p.b = b;
     p.scales = scales; p.base = base; p.ldb = ldb; p.out = out; p.ldo = ldo; p.t = t; p.copy = base != out;
-    launch_rows(type, p, l.max_tiles, (hipStream_t)stream);
+    launch_rows(type, p, false, l.max_tiles, (hipStream_t)stream);
     return check_launch("adapter_forward");
 }
 
@@ -909,18 +945,21 @@ int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const
     q.dy = dy; q.lddy = lddy; q.t = t; q.u = (const float*)(w + gl.u); q.scales = scales; q.part = (float*)(w + gl.part); q.direct = m > 0 && m <= AD_CHUNK; q.da = da; q.db = db;
     const int groups = q.direct ? adapters : l.max_chunks;
     if (m > 0) {
-        const dim3 gt((unsigned)((divup(k, 32) + divup(n, 32)) * divup(rank, 32)), (unsigned)adapters);
-        if (type == JM_F32) {
-            hipLaunchKernelGGL((adapter_transpose_kernel<float>), gt, dim3(256), 0, s, rank, k, n, (const float*)a, (float*)(w + gl.at), (const float*)b, (float*)(w + gl.bt));
-        } else {
-            typedef unsigned short u16;
-            hipLaunchKernelGGL((adapter_transpose_kernel<u16>), gt, dim3(256), 0, s, rank, k, n, (const u16*)a, (u16*)(w + gl.at), (const u16*)b, (u16*)(w + gl.bt));
+        const bool wt = m <= AD_GATHER_ROWS;
+        if (!wt) {
+            const dim3 gt((unsigned)((divup(k, 32) + divup(n, 32)) * divup(rank, 32)), (unsigned)adapters);
+            if (type == JM_F32) {
+                hipLaunchKernelGGL((adapter_transpose_kernel<float>), gt, dim3(256), 0, s, rank, k, n, (const float*)a, (float*)(w + gl.at), (const float*)b, (float*)(w + gl.bt));
+            } else {
+                typedef unsigned short u16;
+                hipLaunchKernelGGL((adapter_transpose_kernel<u16>), gt, dim3(256), 0, s, rank, k, n, (const u16*)a, (u16*)(w + gl.at), (const u16*)b, (u16*)(w + gl.bt));
+            }
         }
         Adapt p{};
         p.m = m; p.k = n; p.n = k; p.rank = rank; p.plan = plan; p.o_order = l.order; p.o_tiles = l.tiles; p.x = dy; p.ldx = lddy;
-        p.a = w + gl.bt; p.b = w + gl.at; p.scales = scales; p.base = base; p.ldb = ldb; p.out = dx; p.ldo = lddx; p.t = (float*)(w + gl.u);
+        p.a = wt ? b : w + gl.bt; p.b = wt ? a : w + gl.at; p.scales = scales; p.base = base; p.ldb = ldb; p.out = dx; p.ldo = lddx; p.t = (float*)(w + gl.u);
         p.copy = base != dx;
-        launch_rows(type, p, l.max_tiles, s);
+        launch_rows(type, p, wt, l.max_tiles, s);
         if (x) {
             if (type == JM_F32) launch_wgrad<JM_F32, false>(q, groups, s);
             else if (type == JM_BF16) launch_wgrad<JM_BF16, false>(q, groups, s);
