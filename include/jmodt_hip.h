@@ -793,6 +793,7 @@ int jm_fold_bn_multi_grad(int n, const float* const* dwf, const float* const* w,
 #define JM_F32 0    /* element types of the entries below */
 #define JM_BF16 1
 #define JM_F16 2
+/* At most 2^30 rows and 2^22 channels. */
 /* x (m, c), rows ldx apart -> e4m3 codes (m, c) in rows of ldc bytes (a multiple of 16, >= c; the bytes behind c are written as zero up to
  * the next multiple of 16) and one scale byte per row and 32 channels, exps (ceil(c / 32), m) with
  * block rows of lde bytes (a multiple of 16, >= m).  Per block: amax = the largest finite |x|, 2^e the
@@ -805,7 +806,7 @@ int jm_rows8_pack(int m, int c, int type, const void* x, long long ldx, unsigned
 int jm_rows8_restore(int m, int c, int type, const unsigned char* codes, int ldc, const unsigned char* exps, int lde, void* out, long long ldo,
                      jm_stream_t stream);
 /* out (m, c) = (kept value > 0) ? dy : 0: the gradient through a ReLU whose output was kept; out may be dy */
-int jm_rows8_relu_mask(int m, int c, const float* dy, int ldd, const unsigned char* codes, int ldc, float* out, int ldo, jm_stream_t stream);
+int jm_rows8_relu_mask(int m, int c, const float* dy, long long ldd, const unsigned char* codes, int ldc, float* out, long long ldo, jm_stream_t stream);
 /* dw (n, k) = dy (m, n)^T X (m, k) with X kept (codes, exps), dbias (n) = column sums of dy (NULL: skipped).  Sums in float32, in a
  * fixed order; lddy <= 2^22.  ws: >= jm_rows8_wgrad_workspace_bytes, 16-byte aligned. */
 size_t jm_rows8_wgrad_workspace_bytes(int m, int n, int k);
@@ -815,7 +816,7 @@ int jm_rows8_linear_wgrad(int m, int n, int k, int type, const void* dy, long lo
 /* ------------------------------------------------------------------ low-rank adapters (csrc/adapters.hip) -------- */
 #define JM_ADAPTER_MAX_RANK 128
 /* The rows of every adapter, in device memory: ids (m) names the adapter of each row; a value outside 0 .. adapters - 1 is a row
- * without one.  plan: jm_adapter_plan_elems(m, adapters) int32, 16-byte aligned; adapters <= 1023. */
+ * without one.  plan: jm_adapter_plan_elems(m, adapters) int32, 16-byte aligned; adapters <= 1023, m <= 2^28. */
 size_t jm_adapter_plan_elems(int m, int adapters);
 int jm_adapter_plan(int m, int adapters, const int* ids, int* plan, jm_stream_t stream);
 /* out[r] = base[r] + scales[a] b_a (a_a x[r]), a_a (rank, k), b_a (n, rank), a = the adapter of row r; rows without one: out = base.

@@ -224,7 +224,7 @@ SIGNATURES = {
     "jm_rows_sigmoid": (_I, [_I, _P, _I, _P, _P]),
     "jm_rows8_pack": (_I, [_I, _I, _I, _P, _L, _P, _I, _P, _I, _P]),
     "jm_rows8_restore": (_I, [_I, _I, _I, _P, _I, _P, _I, _P, _L, _P]),
-    "jm_rows8_relu_mask": (_I, [_I, _I, _P, _I, _P, _I, _P, _I, _P]),
+    "jm_rows8_relu_mask": (_I, [_I, _I, _P, _L, _P, _I, _P, _L, _P]),
     "jm_rows8_wgrad_workspace_bytes": (_Z, [_I, _I, _I]),
     "jm_rows8_linear_wgrad": (_I, [_I, _I, _I, _I, _P, _L, _P, _I, _P, _I, _P, _L, _P, _P, _Z, _P]),
     "jm_adapter_plan_elems": (_Z, [_I, _I]),

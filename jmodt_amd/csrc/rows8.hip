@@ -18,7 +18,7 @@
 namespace jm {
 
 constexpr int R8_BLOCK = 32;         // channels per scale
-constexpr int R8_MAX_ROWS = 1 << 30;        // (row counters of the weight gradient are 32 bits wide)
+constexpr int R8_MAX_ROWS = 1 << 30, R8_MAX_WIDTH = 1 << 22;        // (32-bit row counters, and offsets of up to 128 rows of codes)
 constexpr long long R8_MAX_LD = 1 << 22;      // (128 rows of it are addressed by 32-bit offsets there)
 constexpr int R8_GRID = 4096;         // workgroups of the element-wise kernels: 16 a CU, then they walk
 constexpr int R8_EMIN = -100;        // least scale exponent: 2^e and the smallest code 2^(e - 9) stay normal in float32 and bfloat16
@@ -143,17 +143,26 @@ rows8_restore_kernel(int m, int lde, int c, int groups, const unsigned char* __r
     }
 }
 
-// out = (the kept value > 0) ? dy : 0 — the gradient through a ReLU whose output was kept.  out may be dy.
+// out = (the kept value > 0) ? dy : 0 — the gradient through a ReLU whose output was kept.  out may be dy.  Four channels a lane, 9 bytes
+// moved an element: bound by memory.
 __global__ void __launch_bounds__(256)
-rows8_relu_mask_kernel(long long items, int c, int groups, const float* dy, int ldd, const unsigned char* __restrict__ codes, int ldc, float* out, int ldo) {
-    for (long long it = blockIdx.x * 256ll + threadIdx.x; it < items; it += gridDim.x * 256ll) {
-        const long long row = it / groups;
-        const int c0 = (int)(it - row * groups) * 4;
-        const unsigned w = *reinterpret_cast<const unsigned*>(codes + row * ldc + c0);
+rows8_relu_mask_kernel(int m, int c, int groups, const float* dy, long long ldd, const unsigned char* __restrict__ codes, int ldc, float* out, long long ldo) {
+    const long long step = gridDim.x * 256ll, rows = step / groups;
+    const int grps = (int)(step - rows * groups);
+    for (R8Walk at(blockIdx.x * 256ll + threadIdx.x, groups); at.row < m; at.advance(rows, grps, groups)) {
+        const int c0 = at.grp * 4;
+        const unsigned w = *reinterpret_cast<const unsigned*>(codes + at.row * ldc + c0);
+        const float* src = dy + at.row * ldd + c0;
+        float* dst = out + at.row * ldo + c0;
+        auto on = [&](int q) { const unsigned b = (w >> (8 * q)) & 0xffu; return b != 0u && b < 0x7fu; };
+        if (c0 + 4 <= c) {
+            f32x4 v;
+            __builtin_memcpy(&v, src, 16);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const unsigned b = (w >> (8 * q)) & 0xffu;
-            if (c0 + q < c) out[row * ldo + c0 + q] = (b != 0u && b < 0x7fu) ? dy[row * ldd + c0 + q] : 0.f;
+            for (int q = 0; q < 4; ++q) v[q] = on(q) ? v[q] : 0.f;
+            __builtin_memcpy(dst, &v, 16);
+        } else {
+            for (int q = 0; c0 + q < c; ++q) dst[q] = on(q) ? src[q] : 0.f;
         }
     }
 }
@@ -239,7 +248,7 @@ rows8_wgrad_kernel(Wgrad8 p) {
     if ((int)(blockIdx.x >> 3) >= (total + 7) / 8 || item >= total) return;
     const int split = item / tiles, tile = item % tiles;
     const int n0 = (tile / tk) * W8_T, k0 = (tile % tk) * W8_T;
-    const int r_begin = min((long long)split * p.rows_per, (long long)p.m), r_end = min(p.m, r_begin + p.rows_per);
+    const int r_begin = (int)min((long long)split * p.rows_per, (long long)p.m), r_end = (int)min((long long)p.m, (long long)r_begin + p.rows_per);
 
     // fetch: rows 8 oct .. + 7 of the 64, columns 4 l .. + 3 of both tiles
     const int l = tid % G, oct = tid / G;
@@ -267,7 +276,7 @@ rows8_wgrad_kernel(Wgrad8 p) {
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
             if (q < q0 || q >= q1) continue;
-            d.x[q] = __builtin_amdgcn_raw_buffer_load_b32(xbuf, xo, q * p.ldc, 0);
+            d.x[q] = __builtin_amdgcn_raw_buffer_load_b32(xbuf, xo + (unsigned)(q * p.ldc), 0, 0);
             if constexpr (SMALL) {                           // fewer than 4 columns, or rows that are not aligned to 4 bytes
                 const T* dy = yr + (long long)min(8 * oct + q, left - 1) * p.lddy;
                 T t[4];
@@ -276,9 +285,9 @@ rows8_wgrad_kernel(Wgrad8 p) {
                 d.y[q].load(t);
                 if (8 * oct + q >= left) d.y[q].zero();
             } else if constexpr (TY == JM_F32) {
-                d.y[q].v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ybuf, yo, q * (int)p.lddy * 4, 0));
+                d.y[q].v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ybuf, yo + (unsigned)(q * (int)p.lddy * 4), 0, 0));
             } else {
-                d.y[q].set(__builtin_amdgcn_raw_buffer_load_b64(ybuf, yo, q * (int)p.lddy * 2, 0));
+                d.y[q].set(__builtin_amdgcn_raw_buffer_load_b64(ybuf, yo + (unsigned)(q * (int)p.lddy * 2), 0, 0));
             }
         }
     };
@@ -549,7 +558,7 @@ extern "C" {
 
 int jm_rows8_pack(int m, int c, int type, const void* x, long long ldx, unsigned char* codes, int ldc, unsigned char* exps, int lde,
                   jm_stream_t stream) {
-    JM_REQUIRE(m >= 0 && c > 0 && type >= JM_F32 && type <= JM_F16, "rows8_pack: m %d, c %d, type %d", m, c, type);
+    JM_REQUIRE(m >= 0 && m <= R8_MAX_ROWS && c > 0 && c <= R8_MAX_WIDTH && type >= JM_F32 && type <= JM_F16, "rows8_pack: m %d, c %d, type %d", m, c, type);
     JM_REQUIRE(ldc >= c && ldc % 16 == 0 && lde >= m && lde % 16 == 0 && ldx >= c, "rows8_pack: codes and scales in multiples of 16 bytes (ldc %d, c %d, lde %d, m %d, ldx %lld)", ldc,
                c, lde, m, ldx);
     if (m == 0) return JM_OK;
@@ -565,7 +574,7 @@ int jm_rows8_pack(int m, int c, int type, const void* x, long long ldx, unsigned
 
 int jm_rows8_restore(int m, int c, int type, const unsigned char* codes, int ldc, const unsigned char* exps, int lde, void* out, long long ldo,
                      jm_stream_t stream) {
-    JM_REQUIRE(m >= 0 && c > 0 && type >= JM_F32 && type <= JM_F16, "rows8_restore: m %d, c %d, type %d", m, c, type);
+    JM_REQUIRE(m >= 0 && m <= R8_MAX_ROWS && c > 0 && c <= R8_MAX_WIDTH && type >= JM_F32 && type <= JM_F16, "rows8_restore: m %d, c %d, type %d", m, c, type);
     JM_REQUIRE(ldc >= c && ldc % 16 == 0 && lde >= m && lde % 16 == 0 && ldo >= c, "rows8_restore: codes and scales in multiples of 16 bytes (ldc %d, c %d, lde %d, m %d, ldo %lld)",
                ldc, c, lde, m, ldo);
     if (m == 0) return JM_OK;
@@ -579,26 +588,27 @@ int jm_rows8_restore(int m, int c, int type, const unsigned char* codes, int ldc
     return check_launch("rows8_restore");
 }
 
-int jm_rows8_relu_mask(int m, int c, const float* dy, int ldd, const unsigned char* codes, int ldc, float* out, int ldo, jm_stream_t stream) {
-    JM_REQUIRE(m >= 0 && c > 0 && ldd >= c && ldo >= c && ldc >= c && ldc % 16 == 0, "rows8_relu_mask: m %d, c %d, ldd %d, ldc %d, ldo %d", m, c, ldd, ldc, ldo);
+int jm_rows8_relu_mask(int m, int c, const float* dy, long long ldd, const unsigned char* codes, int ldc, float* out, long long ldo,
+                       jm_stream_t stream) {
+    JM_REQUIRE(m >= 0 && m <= R8_MAX_ROWS && c > 0 && c <= R8_MAX_WIDTH && ldd >= c && ldo >= c && ldc >= c && ldc % 16 == 0,
+               "rows8_relu_mask: m %d, c %d, ldd %lld, ldc %d, ldo %lld", m, c, ldd, ldc, ldo);
     if (m == 0) return JM_OK;
     JM_REQUIRE(dy && codes && out && ((uintptr_t)codes & 15) == 0, "rows8_relu_mask: NULL or unaligned buffers");
     const int groups = divup(c, 4);
-    const long long items = (long long)m * groups;
-    hipLaunchKernelGGL(rows8_relu_mask_kernel, dim3((unsigned)grid_for(items, 256, JM_EGRID)), dim3(256), 0, (hipStream_t)stream, items, c, groups, dy, ldd,
+    hipLaunchKernelGGL(rows8_relu_mask_kernel, dim3((unsigned)grid_for((long long)m * groups, 256, R8_GRID)), dim3(256), 0, (hipStream_t)stream, m, c, groups, dy, ldd,
                        codes, ldc, out, ldo);
     return check_launch("rows8_relu_mask");
 }
 
 size_t jm_rows8_wgrad_workspace_bytes(int m, int n, int k) {
-    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    if (m <= 0 || m > R8_MAX_ROWS || n <= 0 || n > R8_MAX_WIDTH || k <= 0 || k > R8_MAX_WIDTH) return 0;
     const Wgrad8Plan p = wgrad8_plan(m, n, k);               // per split dW, then per split and tile column the bias sums
     return p.splits > 1 ? (size_t)p.splits * ((size_t)n * (size_t)k + (size_t)divup(k, p.tile) * n) * sizeof(float) : 0;
 }
 
 int jm_rows8_linear_wgrad(int m, int n, int k, int type, const void* dy, long long lddy, const unsigned char* codes, int ldc, const unsigned char* exps,
                           int lde, float* dw, long long lddw, float* dbias, void* ws, size_t ws_bytes, jm_stream_t stream) {
-    JM_REQUIRE(m >= 0 && m <= R8_MAX_ROWS && n > 0 && k > 0 && type >= JM_F32 && type <= JM_F16 && dw, "rows8_linear_wgrad: m %d, n %d, k %d, type %d", m, n, k, type);
+    JM_REQUIRE(m >= 0 && m <= R8_MAX_ROWS && n > 0 && n <= R8_MAX_WIDTH && k > 0 && k <= R8_MAX_WIDTH && type >= JM_F32 && type <= JM_F16 && dw, "rows8_linear_wgrad: m %d, n %d, k %d, type %d", m, n, k, type);
     JM_REQUIRE(lddy >= n && lddy <= R8_MAX_LD && ldc >= k && ldc <= R8_MAX_LD && ldc % 16 == 0 && lde >= m && lde % 16 == 0 && lddw >= k,
                "rows8_linear_wgrad: lddy %lld, ldc %d, lde %d, lddw %lld for m %d, n %d, k %d", lddy, ldc, lde, lddw, m, n, k);
     JM_REQUIRE(m == 0 || (dy && codes && exps && (((uintptr_t)codes | (uintptr_t)exps) & 15) == 0), "rows8_linear_wgrad: NULL or unaligned buffers");

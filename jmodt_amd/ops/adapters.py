@@ -12,18 +12,20 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from .. import _lib as L
 from . import rows as R
-from .rows8 import TYPES, Rows8, _kept, _matrix, _on_device, checkpoint_rows, linear_wgrad8
+from .rows8 import TYPES, Rows8, _bytes, _disjoint, _kept, _matrix, _on_device, checkpoint_rows, linear_wgrad8
 
 _f32, _i32 = torch.float32, torch.int32
-MAX_RANK, MAX_ADAPTERS = 128, 1023
+MAX_RANK, MAX_ADAPTERS, MAX_ROWS = 128, 1023, 1 << 28
 
 
 class AdapterPlan:
     """The rows of every adapter, in device memory: ids (M,) int32, the adapter of each row; a value outside 0 .. adapters - 1 is a
-    row without one.  Built on the current stream; ids may be reused afterwards."""
+    row without one.  Built on the current stream; ids may be reused afterwards.  On another stream: order it behind this one and
+    keep the plan until it is done (or `data.record_stream`), as with every tensor."""
 
     def __init__(self, ids: torch.Tensor, adapters: int):
         adapters = int(adapters)
@@ -32,6 +34,8 @@ class AdapterPlan:
         _on_device(ids, "ids")
         if ids.dtype != _i32 or ids.dim() != 1 or not ids.is_contiguous():
             raise TypeError(f"ids must be a contiguous 1-D int32 tensor, got {ids.dtype} {tuple(ids.shape)}")
+        if ids.shape[0] > MAX_ROWS:
+            raise ValueError(f"{ids.shape[0]} rows; at most {MAX_ROWS} are supported")
         lib = L.load()
         self.rows, self.adapters = ids.shape[0], adapters
         self.data = torch.empty((lib.jm_adapter_plan_elems(self.rows, adapters),), dtype=_i32, device=ids.device)
@@ -64,27 +68,6 @@ def _weights(a, b, scales, plan, dtype, k: int, n: int, m: int):
     if scales.dtype != _f32 or scales.shape != (count,) or not scales.is_contiguous():
         raise TypeError(f"scales must be a contiguous float32 tensor of ({count},), got {scales.dtype} {tuple(scales.shape)}")
     return rank, count
-
-
-def _bytes(t: torch.Tensor) -> int:
-    """from the tensor's first byte to behind its last one"""
-    if t.is_contiguous():
-        return t.numel() * t.element_size()
-    return t.element_size() * (1 + sum((d - 1) * st for d, st in zip(t.shape, t.stride()))) if t.numel() else 0
-
-
-def _disjoint(p: int, size: int, out: torch.Tensor, other: torch.Tensor, name: str) -> None:
-    """refuses an output (`size` bytes at p) that shares elements with an input; columns beside each other in rows of one buffer are fine"""
-    q = other.data_ptr()
-    if q >= p + size or q + _bytes(other) <= p:
-        return
-    if other.dim() == 2 and out.element_size() == other.element_size() and out.shape[0] > 1 and other.shape[0] > 1:
-        ld = out.stride(0)
-        if ld == other.stride(0):
-            d = ((q - p) // out.element_size()) % ld          # columns from out's first to other's first
-            if d >= out.shape[1] and d + other.shape[1] <= ld:
-                return
-    raise RuntimeError(f"out shares memory with {name}")
 
 
 def _result(base, out, m: int, n: int, like: torch.Tensor, others):
@@ -175,6 +158,7 @@ class _AdapterLinear(Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         saved = ctx.saved_tensors
         if ctx.keep:

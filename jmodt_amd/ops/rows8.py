@@ -14,12 +14,14 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from .. import _lib as L
 
 _f32, _u8 = torch.float32, torch.uint8
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # JM_F32, JM_BF16, JM_F16
 BLOCK = 32
+MAX_ROWS, MAX_CHANNELS = 1 << 30, 1 << 22
 
 
 def _on_device(t, name: str) -> None:
@@ -37,7 +39,7 @@ def _matrix(t, name: str, dtype: Optional[torch.dtype] = None) -> Tuple[int, int
     try:
         if t.get_device() == L._current_device() and t.dim() == 2 and t.is_contiguous() and (t.dtype is dtype or (dtype is None and t.dtype in TYPES)):
             m, c = t.shape
-            if c:
+            if 0 < c <= MAX_CHANNELS and m <= MAX_ROWS:
                 return m, c, t.data_ptr(), c
     except AttributeError:
         pass                                                 # (not a tensor: refused below, like everything else that is not the usual case)
@@ -52,12 +54,35 @@ def _matrix(t, name: str, dtype: Optional[torch.dtype] = None) -> Tuple[int, int
     m, c = t.shape
     if c == 0:
         raise ValueError(f"{name} has no channels")
+    if m > MAX_ROWS or c > MAX_CHANNELS:
+        raise ValueError(f"{name}: {m} rows of {c} channels; at most {MAX_ROWS} rows and {MAX_CHANNELS} channels are supported")
     if c > 1 and t.stride(1) != 1:
         raise RuntimeError(f"{name} must have unit column stride")
     ld = t.stride(0) if m > 1 else c
     if ld < c:
         raise RuntimeError(f"{name}: rows {ld} apart overlap (width {c}); pass a contiguous tensor")
     return m, c, t.data_ptr(), ld
+
+
+def _bytes(t: torch.Tensor) -> int:
+    """from the tensor's first byte to behind its last one"""
+    if t.is_contiguous():
+        return t.numel() * t.element_size()
+    return t.element_size() * (1 + sum((d - 1) * st for d, st in zip(t.shape, t.stride()))) if t.numel() else 0
+
+
+def _disjoint(p: int, size: int, out: torch.Tensor, other: torch.Tensor, name: str) -> None:
+    """refuses an output (`size` bytes at p) that shares elements with an input; columns beside each other in rows of one buffer are fine"""
+    q = other.data_ptr()
+    if q >= p + size or q + _bytes(other) <= p:
+        return
+    if other.dim() == 2 and out.element_size() == other.element_size() and out.shape[0] > 1 and other.shape[0] > 1:
+        ld = out.stride(0)
+        if ld == other.stride(0):
+            d = ((q - p) // out.element_size()) % ld          # columns from out's first to other's first
+            if d >= out.shape[1] and d + other.shape[1] <= ld:
+                return
+    raise RuntimeError(f"out shares memory with {name}")
 
 
 def _sizes(m: int, c: int) -> Tuple[int, int, int]:
@@ -75,7 +100,7 @@ class Rows8:
         rows, channels = int(rows), int(channels)
         if not isinstance(data, torch.Tensor) or data.dtype != _u8 or data.dim() != 1 or not data.is_contiguous():
             raise TypeError("data must be a contiguous 1-D uint8 tensor")
-        if rows < 0 or channels <= 0:
+        if not 0 <= rows <= MAX_ROWS or not 0 < channels <= MAX_CHANNELS:
             raise ValueError(f"({rows}, {channels}) rows and channels")
         ld, nb, mp = _sizes(rows, channels)
         if data.shape[0] != rows * ld + nb * mp:
@@ -163,6 +188,9 @@ def relu_mask8(dy: torch.Tensor, y8: Rows8, out: Optional[torch.Tensor] = None) 
     mo, co, po, ldo = _matrix(out, "out", _f32)
     if (mo, co) != (m, c):
         raise ValueError(f"out {tuple(out.shape)}: expected ({m}, {c})")
+    if po != pdy or ldo != ldd:
+        _disjoint(po, _bytes(out), out, dy, "dy")
+    _disjoint(po, _bytes(out), out, y8.data, "y8")
     L.check(L.load().jm_rows8_relu_mask(m, c, pdy, ldd, pc, ld, po, ldo, L.stream_ptr()), "relu_mask8")
     return out
 
@@ -186,6 +214,9 @@ def linear_wgrad8(dy: torch.Tensor, x8: Rows8, want_bias: bool = True, out: Opti
         if nw != n or col0 < 0 or col0 + k > kw:
             raise ValueError(f"out {tuple(out.shape)} for columns {col0} .. {col0 + k - 1} of ({n}, ...)")
         pw += 4 * col0
+        block = out[:, col0:col0 + k]
+        for t, name in ((dy, "dy"), (x8.data, "x8")):
+            _disjoint(pw, _bytes(block), block, t, name)
     db = torch.empty((n,), dtype=_f32, device=device) if want_bias else None
     nbytes = lib.jm_rows8_wgrad_workspace_bytes(m, n, k)
     ws = torch.empty((nbytes // 4,), dtype=_f32, device=device) if nbytes else None
@@ -215,6 +246,7 @@ class _RowsMLP8(Function):
         return cur
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         from . import rows as R
         nk, acts, need = len(ctx.shapes), ctx.acts, ctx.needs_input_grad

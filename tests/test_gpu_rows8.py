@@ -261,3 +261,43 @@ def test_keep_at_the_end_of_a_buffer(m, c, dtype):
     codes, exps = encode_ref(x)
     assert np.array_equal(codes & 127, k.codes.cpu().numpy()[:, :c] & 127) and np.array_equal(exps, k.exps.cpu().numpy())
     assert torch.isnan(buf[:32]).all() and torch.isnan(buf[32 + m * c:]).all()
+
+
+@pytest.mark.parametrize("m,c", [(1, 1), (3, 4), (50, 7), (33, 130), (5000, 64)])
+def test_relu_mask_strides_and_in_place(m, c):
+    y = make(m, c, torch.float32, seed=m, relu=True)
+    k = R8.checkpoint_rows(y)
+    wide = torch.randn(2 * m, 2 * c + 5, device="cuda")
+    dy, out = wide[::2, 1:1 + c], wide[::2, 3 + c:3 + 2 * c]
+    want, before = torch.where(y > 0, dy, torch.zeros_like(dy)), wide.clone()
+    assert R8.relu_mask8(dy, k, out=out) is out and torch.equal(out, want)
+    before[::2, 3 + c:3 + 2 * c] = want
+    assert torch.equal(wide, before)                      # nothing beside it was written
+    assert R8.relu_mask8(dy, k, out=dy) is dy and torch.equal(dy, want)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (5, 4, 16), (65, 66, 40), (200, 131, 130), (20000, 8, 8)])
+def test_wgrad_at_the_end_of_a_buffer(m, n, k, dtype):
+    """gradient rows between guard values that are NaN: rows behind the last one are read as zeros, whatever lies there"""
+    dy, x8 = wgrad_case(m, n, k, dtype, 3)
+    want = R8.linear_wgrad8(dy, x8)
+    for lead in (64, 65):
+        buf = torch.full((m * n + 128 + 64 * n,), float("nan"), device="cuda", dtype=dtype)
+        inside = buf[lead:lead + m * n].view(m, n)
+        inside.copy_(dy)
+        got = R8.linear_wgrad8(inside, x8)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_outputs_over_inputs_are_refused():
+    x = torch.randn(40, 24, device="cuda")
+    with pytest.raises(RuntimeError):                     # other rows of dy
+        R8.relu_mask8(x[:-1], R8.checkpoint_rows(x[1:]), out=x[1:])
+    data = torch.empty(40 * 32 + 48 + 40 * 24 * 4, device="cuda", dtype=torch.uint8)
+    over = R8.Rows8(data[:40 * 32 + 48], 40, 24)
+    with pytest.raises(RuntimeError):                     # the kept rows
+        R8.relu_mask8(x, over, out=data[16:16 + 40 * 24 * 4].view(torch.float32).view(40, 24))
+    big = torch.randn(24, 24, device="cuda")
+    with pytest.raises(RuntimeError):
+        R8.linear_wgrad8(big, R8.checkpoint_rows(big), out=big)
