@@ -8,9 +8,9 @@
 //     dA_a   = s_a sum over the rows of a of u[r] x[r]^T,   dB_a = s_a sum dy[r] t[r]^T
 // t, u and every sum are float32; base + s B t is rounded once.
 //
-// The rows of an adapter are found by a plan in device memory (a stable counting sort of the rows by adapter, built by three small
-// kernels, one for up to PL_ROWS rows; the host never learns the counts): tiles of 16 or 32 rows and chunks of AD_CHUNK rows, each of one
-// adapter.
+// The rows of an adapter are found by a plan in device memory (a stable counting sort of the rows by adapter, built by two small
+// kernels, one for up to PL_ROWS rows; the host never learns the counts): tiles of 16 or 32 rows and chunks of 128 to 512 rows, each of
+// one adapter.
 #include "jm_elem.h"
 #include "jm_rows.h"
 #include <type_traits>
@@ -18,26 +18,33 @@
 namespace jm {
 
 // ------------------------------------------------------------------------------------------------ plan
-constexpr int PL_ROWS = 4096;        // rows of a counting block
+constexpr int PL_ROWS = 4096, PL_BLOCKS = 256;        // a counting block has a multiple of PL_ROWS rows, so that there are at most PL_BLOCKS
 constexpr int PL_THREADS = 1024;
 constexpr int PL_MAX_ADAPTERS = 1023;        // + the rows without an adapter: one counter a thread
 constexpr int AD_WIDE_ROWS = 16384;
-// rows of a tile: 16 while that leaves CUs idle, 32 where there are enough tiles (A and B are read once a tile)
+// rows of a tile: 16 while that leaves CUs idle, 32 where there are enough tiles (A and B are read once a tile).  Forward, k = n = 512, 16 | 32
+// rows: 4096 rows float32 rank 16 10.2 | 14.4 us, 8192 bfloat16 8.7 | 9.4; 16384 rank 64 47 | 43 and 24 | 20; 65536 rank 16 108 | 98, 40 | 38.
+// With tiles of 16 the backward gathers A and B transposed, with 32 a kernel transposes them first (gather | transpose, float32 rank 16:
+// 512 rows 11.0 | 15.1 us, 4096 rows 28.8 | 32.8, 8192 rows 35.4 | 38.6).
 static __host__ __device__ __forceinline__ int ad_tile(int m) { return m < AD_WIDE_ROWS ? 16 : 32; }
-constexpr int AD_CHUNK = 512;       // rows of a chunk (weight gradients)
-constexpr int AD_GATHER_ROWS = 2048;        // up to here the backward gathers A and B transposed instead of transposing them first
-static_assert(AD_GATHER_ROWS < AD_WIDE_ROWS, "there tiles have 16 rows");
-constexpr int AD_MAX_ROWS = 1 << 30, AD_MAX_WIDTH = 1 << 20;        // tile counts, grids and per-adapter element counts stay in range
+constexpr int AD_CHUNK = 512;
+// rows of a chunk (weight gradients).  Up to AD_CHUNK rows an adapter is one chunk and its workgroups write the gradients themselves (512 rows of
+// four adapters, float32 rank 16: 12.0 us for the backward, 14.0 with chunks of 128 and a second kernel; of a single adapter 19.4 | 14.9).
+// Beyond that small chunks fill the CUs, large ones write fewer partials (chunks of 128 | 256 | 512, float32 rank 16: 1024 rows of one
+// adapter 14.6 | 17.6 | 22 us; 4096 rows of eight 24.3 | 24.1 | 28.7; 8192 rows, rank 64: 58 | 53 | 62; 16383 rows, rank 64: 98 | 87 | 82).
+static __host__ __device__ __forceinline__ int ad_chunk(int m) { return m <= AD_CHUNK || m > 8192 ? AD_CHUNK : (m <= 4096 ? 128 : 256); }
+constexpr int AD_MAX_ROWS = 1 << 28, AD_MAX_WIDTH = 1 << 20;        // grids (2^32 threads) and per-adapter element counts stay in range
 
 struct PlanLayout {                  // offsets in ints; header: [0] tiles, [1] chunks
     size_t order, tiles, chunks, chunk_first, hist, total;
-    int max_tiles, max_chunks, blocks;
+    int max_tiles, max_chunks, blocks, block_rows;
 };
 static PlanLayout plan_layout(int m, int adapters) {
     PlanLayout l;
-    l.blocks = divup(m, PL_ROWS);
+    l.block_rows = PL_ROWS * imax(1, divup(m, PL_ROWS * PL_BLOCKS));
+    l.blocks = divup(m, l.block_rows);
     l.max_tiles = divup(m, ad_tile(m)) + (adapters + 1 < m ? adapters + 1 : m);
-    l.max_chunks = divup(m, AD_CHUNK) + (adapters < m ? adapters : m);
+    l.max_chunks = divup(m, ad_chunk(m)) + (adapters < m ? adapters : m);
     l.order = 4;
     l.tiles = align_up(l.order + (size_t)m, 4);
     l.chunks = l.tiles + 4 * (size_t)l.max_tiles;
@@ -71,12 +78,12 @@ __device__ __forceinline__ void plan_scan3(int (&v)[3], int (*wave_tot)[3]) {
     __syncthreads();
 }
 
-// bucket counts -> starts, and the tables of tiles and chunks.  `count`: this thread's bucket count (thread = bucket).
-// first[b] = {row start, first tile, first chunk} of bucket b, first[adapters + 1] = the totals.
-__device__ void plan_tables(int count, int adapters, int tile_rows, int (*first)[3], int (*wave_tot)[3], int* __restrict__ plan, size_t o_tiles, size_t o_chunks,
-                            size_t o_chunk_first) {
+// bucket counts -> starts, and the tables of tiles and chunks (entries part, part + parts, ... of every PL_THREADS).  `count`: this
+// thread's bucket count (thread = bucket).  first[b] = {row start, first tile, first chunk} of bucket b, first[adapters + 1] = the totals.
+__device__ void plan_tables(int count, int adapters, int tile_rows, int chunk_rows, int part, int parts, int (*first)[3], int (*wave_tot)[3], int* __restrict__ plan, size_t o_tiles,
+                            size_t o_chunks, size_t o_chunk_first) {
     const int b = threadIdx.x;
-    int v[3] = {count, (count + tile_rows - 1) / tile_rows, b < adapters ? (count + AD_CHUNK - 1) / AD_CHUNK : 0};
+    int v[3] = {count, (count + tile_rows - 1) / tile_rows, b < adapters ? (count + chunk_rows - 1) / chunk_rows : 0};
     const int mine[3] = {v[0], v[1], v[2]};
     plan_scan3(v, wave_tot);
     if (b <= adapters)
@@ -86,11 +93,11 @@ __device__ void plan_tables(int count, int adapters, int tile_rows, int (*first)
             if (b == adapters) first[b + 1][q] = v[q] + mine[q];
         }
     __syncthreads();
-    if (b <= adapters) plan[o_chunk_first + b] = first[b][2];
+    if (part == 0 && b <= adapters) plan[o_chunk_first + b] = first[b][2];
     const int nt = first[adapters + 1][1], nc = first[adapters + 1][2];
-    if (b == 0) { plan[0] = nt; plan[1] = nc; plan[2] = 0; plan[3] = 0; }
+    if (part == 0 && b == 0) { plan[0] = nt; plan[1] = nc; plan[2] = 0; plan[3] = 0; }
     // a table entry finds its bucket by bisection: the last bucket whose first tile is <= t
-    for (int t = b; t < nt; t += PL_THREADS) {
+    for (int t = part * PL_THREADS + b; t < nt; t += parts * PL_THREADS) {
         int lo = 0, hi = adapters;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -99,37 +106,35 @@ __device__ void plan_tables(int count, int adapters, int tile_rows, int (*first)
         const int start = first[lo][0] + (t - first[lo][1]) * tile_rows;
         *reinterpret_cast<int4*>(plan + o_tiles + 4 * (size_t)t) = make_int4(lo < adapters ? lo : -1, start, min(tile_rows, first[lo + 1][0] - start), 0);
     }
-    for (int t = b; t < nc; t += PL_THREADS) {
+    for (int t = part * PL_THREADS + b; t < nc; t += parts * PL_THREADS) {
         int lo = 0, hi = adapters - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (first[mid][2] <= t) lo = mid; else hi = mid - 1;
         }
-        const int start = first[lo][0] + (t - first[lo][2]) * AD_CHUNK;
-        *reinterpret_cast<int4*>(plan + o_chunks + 4 * (size_t)t) = make_int4(lo, start, min(AD_CHUNK, first[lo + 1][0] - start), 0);
+        const int start = first[lo][0] + (t - first[lo][2]) * chunk_rows;
+        *reinterpret_cast<int4*>(plan + o_chunks + 4 * (size_t)t) = make_int4(lo, start, min(chunk_rows, first[lo + 1][0] - start), 0);
     }
 }
 
 // rows row0 .. row0 + rows - 1 to their places, in row order within a bucket: next[b] = the bucket's next place.  A wave ranks its 64
-// rows by matching ids, the waves' counts (bytes: at most 64) are added in wave order.
+// rows among those of the same id, the waves' counts (bytes: at most 64) are added in wave order.
 __device__ void plan_scatter(const int* __restrict__ ids, long long row0, int rows, int adapters, int* next, unsigned char (*wcnt)[PL_THREADS],
                              int* __restrict__ order) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6;
     for (int r = 0; r < rows; r += PL_THREADS) {
         __syncthreads();
         for (int q = threadIdx.x; q < 16 * PL_THREADS / 4; q += PL_THREADS) reinterpret_cast<unsigned*>(wcnt)[q] = 0u;
         __syncthreads();
         const bool ok = r + (int)threadIdx.x < rows;
         const int b = ok ? plan_bucket(ids, row0 + r + threadIdx.x, adapters) : -1;
-        int rank = 0;
-        unsigned long long left = __ballot(ok);
-        while (left) {
-            const int lead = __shfl(b, (int)__builtin_ctzll(left));
-            const unsigned long long same = __ballot(b == lead) ;
-            if (b == lead) rank = mbcnt(same);
-            if (lane == 0) wcnt[wave][lead] = (unsigned char)__popcll(same);
-            left &= ~same;
+        unsigned long long same = __ballot(ok);              // the lanes of this wave with the same id, bit by bit of it
+        for (int bit = 1; bit <= adapters; bit <<= 1) {
+            const unsigned long long set = __ballot((b & bit) != 0);
+            same &= (b & bit) ? set : ~set;
         }
+        const int rank = mbcnt(same);
+        if (ok && rank == 0) wcnt[wave][b] = (unsigned char)__popcll(same);
         __syncthreads();
         if (ok) {
             int at = next[b] + rank;
@@ -149,19 +154,19 @@ __device__ void plan_scatter(const int* __restrict__ ids, long long row0, int ro
 // ids of one counting block counted in LDS; whole: the block is all there is and the plan is finished here (one launch)
 template <bool WHOLE>
 __global__ void __launch_bounds__(PL_THREADS)
-adapter_plan_count_kernel(int m, int adapters, const int* __restrict__ ids, int* __restrict__ plan, size_t o_order, size_t o_tiles, size_t o_chunks,
+adapter_plan_count_kernel(int m, int block_rows, int adapters, const int* __restrict__ ids, int* __restrict__ plan, size_t o_order, size_t o_tiles, size_t o_chunks,
                           size_t o_chunk_first, size_t o_hist) {
     __shared__ int cnt[PL_THREADS];
     __shared__ int first[WHOLE ? PL_THREADS + 2 : 1][3], wave_tot[16][3];
     __shared__ __attribute__((aligned(4))) unsigned char wcnt[WHOLE ? 16 : 1][PL_THREADS];
     cnt[threadIdx.x] = 0;
     __syncthreads();
-    const long long row0 = (long long)blockIdx.x * PL_ROWS;
-    const int rows = (int)min((long long)PL_ROWS, m - row0);
+    const long long row0 = (long long)blockIdx.x * block_rows;
+    const int rows = (int)min((long long)block_rows, m - row0);
     for (int r = threadIdx.x; r < rows; r += PL_THREADS) atomicAdd(&cnt[plan_bucket(ids, row0 + r, adapters)], 1);
     __syncthreads();
     if constexpr (WHOLE) {
-        plan_tables(cnt[threadIdx.x], adapters, ad_tile(m), first, wave_tot, plan, o_tiles, o_chunks, o_chunk_first);
+        plan_tables(cnt[threadIdx.x], adapters, ad_tile(m), ad_chunk(m), 0, 1, first, wave_tot, plan, o_tiles, o_chunks, o_chunk_first);
         __syncthreads();
         if ((int)threadIdx.x <= adapters) cnt[threadIdx.x] = first[threadIdx.x][0];
         plan_scatter(ids, 0, rows, adapters, cnt, wcnt, plan + o_order);
@@ -170,33 +175,28 @@ adapter_plan_count_kernel(int m, int adapters, const int* __restrict__ ids, int*
     }
 }
 
-// the blocks' counts -> every block's first place of every bucket (in place), and the tables
+// the rows to their places: every block adds up the counts of the blocks before it (and of all, for the starts of the buckets) and writes
+// its share of the tables
 __global__ void __launch_bounds__(PL_THREADS)
-adapter_plan_tables_kernel(int m, int blocks, int adapters, int* __restrict__ plan, size_t o_tiles, size_t o_chunks, size_t o_chunk_first, size_t o_hist) {
-    __shared__ int first[PL_THREADS + 2][3], wave_tot[16][3];
-    const int b = threadIdx.x;
-    int total = 0;
-    if (b <= adapters)
-        for (int k = 0; k < blocks; ++k) total += plan[o_hist + (size_t)k * (adapters + 1) + b];
-    plan_tables(total, adapters, ad_tile(m), first, wave_tot, plan, o_tiles, o_chunks, o_chunk_first);
-    if (b <= adapters) {
-        int at = first[b][0];
-        for (int k = 0; k < blocks; ++k) {
-            int* h = plan + o_hist + (size_t)k * (adapters + 1) + b;
-            const int c = *h;
-            *h = at;
-            at += c;
-        }
-    }
-}
-
-__global__ void __launch_bounds__(PL_THREADS)
-adapter_plan_scatter_kernel(int m, int adapters, const int* __restrict__ ids, int* __restrict__ plan, size_t o_order, size_t o_hist) {
+adapter_plan_scatter_kernel(int m, int block_rows, int adapters, const int* __restrict__ ids, int* __restrict__ plan, size_t o_order, size_t o_tiles, size_t o_chunks,
+                            size_t o_chunk_first, size_t o_hist) {
     __shared__ int next[PL_THREADS];
+    __shared__ int first[PL_THREADS + 2][3], wave_tot[16][3];
     __shared__ __attribute__((aligned(4))) unsigned char wcnt[16][PL_THREADS];
-    if ((int)threadIdx.x <= adapters) next[threadIdx.x] = plan[o_hist + (size_t)blockIdx.x * (adapters + 1) + threadIdx.x];
-    const long long row0 = (long long)blockIdx.x * PL_ROWS;
-    plan_scatter(ids, row0, (int)min((long long)PL_ROWS, m - row0), adapters, next, wcnt, plan + o_order);
+    const int b = threadIdx.x;
+    const int* hist = plan + o_hist + b;
+    int total = 0, before = 0;
+    if (b <= adapters)
+#pragma unroll 8
+        for (int k = 0; k < (int)gridDim.x; ++k) {
+            const int c = hist[k * (adapters + 1)];
+            total += c;
+            before += k < (int)blockIdx.x ? c : 0;
+        }
+    plan_tables(total, adapters, ad_tile(m), ad_chunk(m), blockIdx.x, gridDim.x, first, wave_tot, plan, o_tiles, o_chunks, o_chunk_first);
+    if (b <= adapters) next[b] = first[b][0] + before;
+    const long long row0 = (long long)blockIdx.x * block_rows;
+    plan_scatter(ids, row0, (int)min((long long)block_rows, m - row0), adapters, next, wcnt, plan + o_order);
 }
 
 // ------------------------------------------------------------------------------------------------ the product
@@ -893,13 +893,14 @@ int jm_adapter_plan(int m, int adapters, const int* ids, int* plan, jm_stream_t 
     const PlanLayout l = plan_layout(m, adapters);
     hipStream_t s = (hipStream_t)stream;
     if (l.blocks <= 1) {
-        hipLaunchKernelGGL((adapter_plan_count_kernel<true>), dim3(1), dim3(PL_THREADS), 0, s, m, adapters, ids, plan, l.order, l.tiles, l.chunks, l.chunk_first, l.hist);
-        return check_launch("adapter_plan");
+        hipLaunchKernelGGL((adapter_plan_count_kernel<true>), dim3(1), dim3(PL_THREADS), 0, s, m, l.block_rows, adapters, ids, plan, l.order, l.tiles, l.chunks,
+                           l.chunk_first, l.hist);
+    } else {
+        hipLaunchKernelGGL((adapter_plan_count_kernel<false>), dim3((unsigned)l.blocks), dim3(PL_THREADS), 0, s, m, l.block_rows, adapters, ids, plan, l.order, l.tiles,
+                           l.chunks, l.chunk_first, l.hist);
+        hipLaunchKernelGGL(adapter_plan_scatter_kernel, dim3((unsigned)l.blocks), dim3(PL_THREADS), 0, s, m, l.block_rows, adapters, ids, plan, l.order, l.tiles,
+                           l.chunks, l.chunk_first, l.hist);
     }
-    hipLaunchKernelGGL((adapter_plan_count_kernel<false>), dim3((unsigned)l.blocks), dim3(PL_THREADS), 0, s, m, adapters, ids, plan, l.order, l.tiles, l.chunks,
-                       l.chunk_first, l.hist);
-    hipLaunchKernelGGL(adapter_plan_tables_kernel, dim3(1), dim3(PL_THREADS), 0, s, m, l.blocks, adapters, plan, l.tiles, l.chunks, l.chunk_first, l.hist);
-    hipLaunchKernelGGL(adapter_plan_scatter_kernel, dim3((unsigned)l.blocks), dim3(PL_THREADS), 0, s, m, adapters, ids, plan, l.order, l.hist);
     return check_launch("adapter_plan");
 }
 
@@ -945,7 +946,7 @@ int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const
     q.dy = dy; q.lddy = lddy; q.t = t; q.u = (const float*)(w + gl.u); q.scales = scales; q.part = (float*)(w + gl.part); q.direct = m > 0 && m <= AD_CHUNK; q.da = da; q.db = db;
     const int groups = q.direct ? adapters : l.max_chunks;
     if (m > 0) {
-        const bool wt = m <= AD_GATHER_ROWS;
+        const bool wt = ad_tile(m) == 16;
         if (!wt) {
             const dim3 gt((unsigned)((divup(k, 32) + divup(n, 32)) * divup(rank, 32)), (unsigned)adapters);
             if (type == JM_F32) {

@@ -72,5 +72,28 @@ def test_plan_and_workspace_sizes():
     assert lib.jm_adapter_plan(4, 2000, PTR, PTR, None) == EINVAL and lib.jm_adapter_plan(4, 2, None, PTR, None) == EINVAL
     assert lib.jm_adapter_plan(4, 2, PTR, PTR + 4, None) == EINVAL
     assert lib.jm_adapter_grad_workspace_bytes(10, 8, 4, 200, 3, 0) == 0
-    big = lib.jm_adapter_grad_workspace_bytes(1 << 30, 1024, 1024, 128, 1023, 0)
-    assert big > (1 << 30) * 128 * 4                      # (beyond 32 bits)
+    big = lib.jm_adapter_grad_workspace_bytes(1 << 28, 1024, 1024, 128, 1023, 0)
+    assert big > (1 << 28) * 128 * 4                      # (beyond 32 bits)
+
+
+@pytest.mark.parametrize("args", [dict(m=-1), dict(c=0), dict(ldd=7), dict(ldo=7), dict(ldc=24), dict(ldc=0), dict(dy=None), dict(codes=None), dict(codes=PTR + 8),
+                                  dict(out=None), dict(m=2 ** 31 - 1), dict(c=2 ** 23, ldc=2 ** 23, ldd=2 ** 23, ldo=2 ** 23)])
+def test_relu_mask_refuses(args):
+    a = dict(m=2, c=8, dy=PTR, ldd=8, codes=PTR, ldc=16, out=PTR, ldo=8)
+    a.update(args)
+    assert L.load().jm_rows8_relu_mask(*a.values(), None) == EINVAL
+
+
+def test_sizes_beyond_the_counters_are_refused():
+    lib = L.load()
+    many, wide = 2 ** 30 + 16, 2 ** 22 + 32
+    for m, c in ((many, 8), (2, wide)):
+        lde, ldc = (m + 15) // 16 * 16, (c + 15) // 16 * 16
+        assert lib.jm_rows8_pack(m, c, 0, PTR, c, PTR, ldc, PTR, lde, None) == EINVAL
+        assert lib.jm_rows8_restore(m, c, 0, PTR, ldc, PTR, lde, PTR, c, None) == EINVAL
+        assert lib.jm_rows8_linear_wgrad(m, c, 8, 0, PTR, c, PTR, 16, PTR, lde, PTR, 8, None, PTR, 1 << 40, None) == EINVAL
+        assert lib.jm_rows8_wgrad_workspace_bytes(m, c, 8) == 0
+        with pytest.raises(ValueError):
+            R8.Rows8(torch.empty(16, dtype=torch.uint8), m, c)
+    assert lib.jm_rows8_linear_wgrad(2, 8, wide, 0, PTR, 8, PTR, wide, PTR, 16, PTR, wide, None, PTR, 1 << 40, None) == EINVAL
+    assert lib.jm_adapter_plan(2 ** 28 + 1, 2, PTR, PTR, None) == EINVAL and lib.jm_adapter_plan_elems(2 ** 28 + 1, 2) == 0

@@ -369,3 +369,106 @@ def test_beside_the_shared_projection_of_the_row_layers():
     AD.adapter_forward(y, d["x"], d["a"], d["b"], d["scales"], plan, out=y)
     none = d["ids"] < 0
     assert none.any() and torch.equal(y[none], plain[none]) and not torch.equal(y, plain)
+
+
+@pytest.mark.parametrize("m,count", [(16384, 5), (64 * 4096, 3), (64 * 4096 + 1, 1023), (300001, 2)])
+def test_plan_of_many_rows(m, count):
+    """the same for tiles of 32 rows, and around the number of counting blocks that need one more launch; chunks too"""
+    ids = np.random.default_rng(m).integers(-1, count, m)
+    p = AD.AdapterPlan(torch.from_numpy(ids.astype(np.int32)).cuda(), count).data.cpu().numpy()
+    bucket = np.where(ids >= 0, ids, count)
+    order = p[4:4 + m]
+    assert np.array_equal(order, np.argsort(bucket, kind="stable"))
+    rows = np.bincount(bucket, minlength=count + 1)
+    start = np.concatenate([[0], np.cumsum(rows)])
+
+    def table(width, buckets):
+        return np.array([(b if b < count else -1, start[b] + q, min(width, rows[b] - q)) for b in range(buckets) for q in range(0, rows[b], width)])
+    at = 4 + (m + 3) // 4 * 4
+    tiles, chunks = table(32, count + 1), table(512, count)
+    assert p[0] == len(tiles) and p[1] == len(chunks)
+    assert np.array_equal(p[at:at + 4 * p[0]].reshape(-1, 4)[:, :3], tiles)
+    at += 4 * ((m + 31) // 32 + min(count + 1, m))
+    assert np.array_equal(p[at:at + 4 * p[1]].reshape(-1, 4)[:, :3], chunks)
+    at += 4 * ((m + 511) // 512 + min(count, m))
+    assert np.array_equal(p[at:at + count + 1], np.concatenate([[0], np.cumsum((rows[:count] + 511) // 512)]))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("kept", [False, True])
+def test_no_rows(dtype, kept):
+    d = make(0, 24, 20, 4, 3, dtype)
+    plan = AD.AdapterPlan(d["ids"], 3)
+    out, t = AD.adapter_forward(d["base"], d["x"], d["a"], d["b"], d["scales"], plan, want_t=True)
+    assert out.shape == (0, 20) and t.shape == (0, 4)
+    x = R8.checkpoint_rows(d["x"]) if kept else d["x"]
+    dx, da, db = AD.adapter_grad(d["dy"], x, t, d["a"], d["b"], d["scales"], plan, base=d["dbase"])
+    assert dx.shape == (0, 24) and not da.any() and not db.any()
+
+
+def test_on_another_stream_and_two_graphs():
+    """a side stream; two captured graphs of different sizes, replayed in turn"""
+    runs = []
+    for seed, m, r in ((1, 900, 16), (2, 200, 40)):
+        d = make(m, 64, 72, r, 5, torch.bfloat16, seed=seed)
+
+        def step(d=d):
+            plan = AD.AdapterPlan(d["ids"], 5)
+            out, t = AD.adapter_forward(d["base"], d["x"], d["a"], d["b"], d["scales"], plan, want_t=True)
+            return (out,) + AD.adapter_grad(d["dy"], R8.checkpoint_rows(d["x"]), t, d["a"], d["b"], d["scales"], plan)
+        want = step()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got = step()
+        torch.cuda.current_stream().wait_stream(s)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        runs.append((graph, out, want, d))                # (a graph reads its inputs where they were: they live as long as it does)
+    for _ in range(3):
+        for _, out, _, _ in runs:
+            for v in out:
+                v.zero_()
+        for graph, _, _, _ in runs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, out, want, _ in runs:
+            assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+@pytest.mark.parametrize("keep", ["float32", "e4m3"])
+def test_layer_captured_forward_and_backward(keep):
+    """both directions in one graph, its leaves first used there; new values on every replay"""
+    d, w, bias, plan = layer_case(seed=21)
+    x = d["x"]
+
+    def step(ps):
+        y = AD.adapter_linear(x, ps[0], ps[1], ps[2], ps[3], d["scales"], plan, keep=keep)
+        return (y.detach(),) + torch.autograd.grad(y, ps, d["dy"])
+
+    def leaves():
+        return [v.detach().clone().requires_grad_() for v in (w, bias, d["a"], d["b"])]
+    step(leaves())
+    torch.cuda.synchronize()
+    ps = leaves()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(ps)
+    for i in range(4):
+        n = layer_case(seed=40 + i)[0]
+        x.copy_(n["x"])
+        d["dy"].copy_(n["dy"])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, step(leaves())))
+
+
+def test_layer_has_no_second_derivative():
+    d, w, bias, plan = layer_case(seed=22)
+    a = d["a"].clone().requires_grad_()
+    y = AD.adapter_linear(d["x"], w, bias, a, d["b"], d["scales"], plan)
+    g, = torch.autograd.grad(y.square().sum(), a, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
