@@ -571,35 +571,41 @@ struct GradRun {
     }
 };
 
-// the four waves' tiles through LDS, added in wave order, to their place
+// the four waves' tiles through LDS, added in wave order, to their place; 32 KB of LDS at a time (with 64 KB a CU
+// holds two workgroups, too few loads in flight)
+constexpr int ad_finish(int rb, int cw) { return rb * cw > 8 ? 8 / cw : rb; }
 template <int TY, int RB, int CW>
-__device__ __forceinline__ void adapter_wgrad_finish(const AdaptGrad& p, float* lds, int4 chunk, int ad, bool isA, int c0, int r0, const f32x4 (&acc)[RB][CW]) {
-    constexpr int TR = 16 * RB, TC = 16 * CW;
+__device__ __forceinline__ void adapter_wgrad_finish(const AdaptGrad& p, float* lds, float* part, int4 chunk, int ad, bool isA, int c0, int r0, const f32x4 (&acc)[RB][CW]) {
+    constexpr int FB = ad_finish(RB, CW), TR = 16 * FB, TC = 16 * CW;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6, width = isA ? p.k : p.n;
-    __syncthreads();
     // D: rows = rank index 4 g + q, column i = channel CW i + j of the tile.  Row r of a tile is turned by 4 r columns, so that it can be read
     // down the ranks, too (dB) without its lanes meeting in one bank
     float* const mine = lds + wave * TR * TC;
     auto place = [&](int r, int c) { return r * TC + ((c + 4 * r) & (TC - 1)); };
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int j = 0; j < CW; j += 4)
-                *reinterpret_cast<f32x4*>(mine + place(rb * 16 + 4 * g + q, CW * i + j)) = f32x4{acc[rb][j][q], acc[rb][j + 1][q], acc[rb][j + 2][q], acc[rb][j + 3][q]};
-    __syncthreads();
     typedef typename Elem<TY>::T E;
-    float* part = p.part + (size_t)blockIdx.x * p.rank * ((size_t)p.k + p.n);
     const float scale = p.direct ? p.scales[ad] : 1.f;
-    for (int e = threadIdx.x; e < TR * TC; e += 256) {       // (dA runs along the channels, dB along the rank)
-        const int rt = isA ? e / TC : e % TR, ct = isA ? e % TC : e / TR, r = r0 + rt, c = c0 + ct;
-        if (r >= p.rank || c >= width) continue;
-        const float* v = lds + place(rt, ct);
-        const float sum = (v[0] + v[TR * TC]) + (v[2 * TR * TC] + v[3 * TR * TC]);
-        const size_t at = isA ? (size_t)r * p.k + c : (size_t)c * p.rank + r;
-        if (p.direct) ((E*)(isA ? p.da : p.db))[(size_t)ad * p.rank * width + at] = (E)(chunk.z > 0 ? scale * sum : 0.f);
-        else part[(isA ? 0 : (size_t)p.rank * p.k) + at] = sum;
+#pragma unroll
+    for (int f = 0; f < RB; f += FB) {
+        __syncthreads();
+#pragma unroll
+        for (int rb = 0; rb < FB; ++rb)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int j = 0; j < CW; j += 4) {
+                    const f32x4* a = acc[f + rb];
+                    *reinterpret_cast<f32x4*>(mine + place(rb * 16 + 4 * g + q, CW * i + j)) = f32x4{a[j][q], a[j + 1][q], a[j + 2][q], a[j + 3][q]};
+                }
+        __syncthreads();
+        for (int e = threadIdx.x; e < TR * TC; e += 256) {   // (dA runs along the channels, dB along the rank)
+            const int rt = isA ? e / TC : e % TR, ct = isA ? e % TC : e / TR, r = r0 + 16 * f + rt, c = c0 + ct;
+            if (r >= p.rank || c >= width) continue;
+            const float* v = lds + place(rt, ct);
+            const float sum = (v[0] + v[TR * TC]) + (v[2 * TR * TC] + v[3 * TR * TC]);
+            const size_t at = isA ? (size_t)r * p.k + c : (size_t)c * p.rank + r;
+            if (p.direct) ((E*)(isA ? p.da : p.db))[(size_t)ad * p.rank * width + at] = (E)(chunk.z > 0 ? scale * sum : 0.f);
+            else part[(isA ? 0 : (size_t)p.rank * p.k) + at] = sum;
+        }
     }
 }
 
@@ -608,7 +614,7 @@ __device__ __forceinline__ void adapter_wgrad_finish(const AdaptGrad& p, float* 
 // multiplied, and add their tiles in wave order through LDS.  Bound by the loads' latency: a chunk's rows are 512 / 16 = 32 groups a wave.
 // With at most one chunk an adapter (direct) the workgroups are the adapters' and write dA and dB themselves.
 template <int TY, bool KEPT, int RB, int CW>
-__device__ __forceinline__ void adapter_wgrad_tile(const AdaptGrad& p, float* lds, int4 chunk, int ad, bool isA, int c0, int r0) {
+__device__ __forceinline__ void adapter_wgrad_tile(const AdaptGrad& p, float* lds, float* part, int4 chunk, int ad, bool isA, int c0, int r0) {
     constexpr int UR = 4;
     int* const rows = reinterpret_cast<int*>(lds);
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
@@ -674,7 +680,7 @@ __device__ __forceinline__ void adapter_wgrad_tile(const AdaptGrad& p, float* ld
             if (q + ST < chunk.z) multiply(b[1], q + ST);
         }
     }
-    adapter_wgrad_finish<TY, RB, CW>(p, lds, chunk, ad, isA, c0, r0, acc);
+    adapter_wgrad_finish<TY, RB, CW>(p, lds, part, chunk, ad, isA, c0, r0, acc);
 }
 
 // The same tile on the bf16 matrix pipe, for channels that are exact in bfloat16 (bfloat16 rows, kept rows): T enters as three bfloat16
@@ -682,7 +688,7 @@ __device__ __forceinline__ void adapter_wgrad_tile(const AdaptGrad& p, float* ld
 // float32 rate, and bound by memory up to a rank of 32.  A lane's 8 contraction elements are 8 rows; it holds 8 channels of each and turns
 // the 8 x 8 block over in its registers.
 template <bool KEPT, int RB>
-__device__ __forceinline__ void adapter_wgrad_tile_bf16(const AdaptGrad& p, float* lds, int4 chunk, int ad, bool isA, int c0, int r0) {
+__device__ __forceinline__ void adapter_wgrad_tile_bf16(const AdaptGrad& p, float* lds, float* part, int4 chunk, int ad, bool isA, int c0, int r0) {
     constexpr int CW = 8, STEP = 4 * 32;
     int* const rows = reinterpret_cast<int*>(lds);
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
@@ -769,34 +775,40 @@ __device__ __forceinline__ void adapter_wgrad_tile_bf16(const AdaptGrad& p, floa
             multiply(b, q);
         }
     }
-    adapter_wgrad_finish<JM_BF16, RB, CW>(p, lds, chunk, ad, isA, c0, r0, acc);
+    adapter_wgrad_finish<JM_BF16, RB, CW>(p, lds, part, chunk, ad, isA, c0, r0, acc);
 }
 
 template <int TY, bool KEPT, int RB, int CW>
 __global__ void __launch_bounds__(256)
 adapter_wgrad_kernel(AdaptGrad p) {
-    __shared__ __attribute__((aligned(16))) float lds[4 * 16 * RB * 16 * CW];       // the rows of the chunk, then the waves' tiles
+    __shared__ __attribute__((aligned(16))) float lds[4 * 16 * ad_finish(RB, CW) * 16 * CW];       // the rows of the chunk, then the waves' tiles
     static_assert(sizeof(lds) >= AD_CHUNK * (sizeof(int) + CW / 2), "the row list and the scales are kept there");
+    // workgroups are dealt to the 8 XCDs in turn: each takes an eighth of the (chunk, channels, ranks) list, so that the workgroups that read
+    // one chunk's rows share an L2
+    const int tk = (p.k + 16 * CW - 1) / (16 * CW), ny = tk + (p.n + 16 * CW - 1) / (16 * CW), per = ny * ((p.rank + 16 * RB - 1) / (16 * RB));
+    const int total = (p.direct ? p.adapters : p.plan[1]) * per, share = (total + 7) / 8;
+    const int item = (int)(blockIdx.x & 7) * share + (int)(blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= share || item >= total) return;
+    const int index = item / per, tile = item % per, r0 = tile / ny * 16 * RB;
+    const bool isA = tile % ny < tk;
+    const int c0 = (tile % ny - (isA ? 0 : tk)) * 16 * CW;
     int ad = 0;
     int4 chunk;
     if (p.direct) {
-        ad = blockIdx.x;
+        ad = index;
         const int c = p.plan[p.o_chunk_first + ad];
         chunk = make_int4(ad, 0, 0, 0);
         if (p.plan[p.o_chunk_first + ad + 1] > c) chunk = *reinterpret_cast<const int4*>(p.plan + p.o_chunks + 4 * (size_t)c);
     } else {
-        if ((int)blockIdx.x >= p.plan[1]) return;
-        chunk = *reinterpret_cast<const int4*>(p.plan + p.o_chunks + 4 * (size_t)blockIdx.x);
+        chunk = *reinterpret_cast<const int4*>(p.plan + p.o_chunks + 4 * (size_t)index);
     }
-    const int tk = (p.k + 16 * CW - 1) / (16 * CW), r0 = blockIdx.z * 16 * RB;
-    const bool isA = (int)blockIdx.y < tk;
-    const int c0 = (isA ? (int)blockIdx.y : (int)blockIdx.y - tk) * 16 * CW;
+    float* const part = p.part + (size_t)index * p.rank * ((size_t)p.k + p.n);
     if constexpr (TY == JM_BF16 && CW == 8) {
-        if (KEPT && isA) adapter_wgrad_tile_bf16<KEPT, RB>(p, lds, chunk, ad, true, c0, r0);
-        else adapter_wgrad_tile_bf16<false, RB>(p, lds, chunk, ad, isA, c0, r0);
+        if (KEPT && isA) adapter_wgrad_tile_bf16<KEPT, RB>(p, lds, part, chunk, ad, true, c0, r0);
+        else adapter_wgrad_tile_bf16<false, RB>(p, lds, part, chunk, ad, isA, c0, r0);
     } else {
-        if (KEPT && isA) adapter_wgrad_tile<TY, KEPT, RB, CW>(p, lds, chunk, ad, true, c0, r0);
-        else adapter_wgrad_tile<TY, false, RB, CW>(p, lds, chunk, ad, isA, c0, r0);
+        if (KEPT && isA) adapter_wgrad_tile<TY, KEPT, RB, CW>(p, lds, part, chunk, ad, true, c0, r0);
+        else adapter_wgrad_tile<TY, false, RB, CW>(p, lds, part, chunk, ad, isA, c0, r0);
     }
 }
 
@@ -851,7 +863,7 @@ template <int TY, bool KEPT>
 static void launch_wgrad(const AdaptGrad& p, int groups, hipStream_t s) {
     const bool wide = p.rank <= 32 || TY == JM_BF16;
     const int cw = wide ? 128 : 64, rw = p.rank <= 16 ? 16 : (wide ? 32 : 64);
-    const dim3 grid((unsigned)groups, (unsigned)(divup(p.k, cw) + divup(p.n, cw)), (unsigned)divup(p.rank, rw)), block(256);
+    const dim3 grid((unsigned)(divup(groups * (divup(p.k, cw) + divup(p.n, cw)) * divup(p.rank, rw), 8) * 8)), block(256);
     if (p.rank <= 16) hipLaunchKernelGGL((adapter_wgrad_kernel<TY, KEPT, 1, 8>), grid, block, 0, s, p);
     else if (wide) hipLaunchKernelGGL((adapter_wgrad_kernel<TY, KEPT, 2, 8>), grid, block, 0, s, p);
     else if constexpr (TY != JM_BF16) hipLaunchKernelGGL((adapter_wgrad_kernel<TY, KEPT, 4, 4>), grid, block, 0, s, p);
@@ -945,6 +957,7 @@ int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const
     q.o_chunk_first = l.chunk_first; q.x = x; q.ldx = ldx; q.codes = codes; q.ldc = ldc; q.exps = exps; q.lde = lde;
     q.dy = dy; q.lddy = lddy; q.t = t; q.u = (const float*)(w + gl.u); q.scales = scales; q.part = (float*)(w + gl.part); q.direct = m > 0 && m <= AD_CHUNK; q.da = da; q.db = db;
     const int groups = q.direct ? adapters : l.max_chunks;
+    JM_REQUIRE((long long)groups * (divup(k, 64) + divup(n, 64)) * divup(rank, 16) < 1 << 24, "adapter_grad: too many (chunk, tile) pairs (m %d, k %d, n %d, rank %d)", m, k, n, rank);
     if (m > 0) {
         const bool wt = ad_tile(m) == 16;
         if (!wt) {
