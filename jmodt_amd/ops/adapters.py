@@ -98,7 +98,9 @@ def adapter_forward(base: Optional[torch.Tensor], x: torch.Tensor, a: torch.Tens
                     out: Optional[torch.Tensor] = None, want_t: bool = False):
     """base (M, N) or None (zero), x (M, K), a (adapters, R, K), b (adapters, N, R), scales (adapters,) float32 ->
     out = base + scales[a] B_a (A_a x) row by row; rows without an adapter: base.  out: a tensor to write (base itself: in place),
-    else a new one.  want_t: (out, t), t (M, R) float32 = A_a x, zero in rows without an adapter — what `adapter_grad` needs."""
+    else a new one.  want_t: (out, t), t (M, R) float32 = A_a x, zero in rows without an adapter — what `adapter_grad` needs.
+    A value that is not finite reaches its own row (in x) or its adapter's rows (in a, b) only; in bfloat16 and float16, where t enters as a
+    sum of two values, an infinity in b gives NaN."""
     m, k, px, ldx = _matrix(x, "x")
     n = b.shape[1] if isinstance(b, torch.Tensor) and b.dim() == 3 else 0
     rank, count = _weights(a, b, scales, plan, x.dtype, k, n, m)
@@ -113,7 +115,7 @@ def adapter_grad(dy: torch.Tensor, x: Union[torch.Tensor, Rows8], t: torch.Tenso
                  base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """the gradients of adapter_forward: dy (M, N), x (M, K) or its kept form, t from the forward ->
     (dx (M, K) = base + scales[a] A_a^T (B_a^T dy), da like a, db like b).  base: the shared projection's data gradient, or None;
-    out: a tensor for dx (base itself: in place).  An adapter without rows gets zeros."""
+    out: a tensor for dx (base itself: in place).  An adapter without rows gets zeros.  Infinities in x or dy (bfloat16) may give NaN in da and db."""
     m, n, pdy, ldd = _matrix(dy, "dy")
     px, ldx, pc, ldc, pe, lde = None, 0, None, 0, None, 0
     if isinstance(x, Rows8):
@@ -182,7 +184,9 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor
                    plan: AdapterPlan, keep: str = "float32") -> torch.Tensor:
     """y (M, N) = x w^T + bias + scales[a] B_a (A_a x): ops.rows.linear_forward and the rows' adapters, float32, differentiable in x, w,
     bias, a and b (a frozen projection: w and bias without requires_grad).  keep = "e4m3": x is kept in 8 bits for the backward
-    (da and dw from the kept values), "float32": as it is.  Widths are multiples of 4, as everywhere in ops.rows."""
+    (da and dw from the kept values), "float32": as it is.  Widths are multiples of 4, as everywhere in ops.rows.
+    Forward and backward can be captured into a HIP graph together; as with every autograd function, no eager graph of the same leaves may be
+    alive then (autograd keeps a leaf's accumulation on the stream of its first live graph) — take torch.autograd.grad on fresh leaves."""
     if keep not in ("float32", "e4m3"):
         raise ValueError(f"keep must be 'float32' or 'e4m3', got {keep!r}")
     if isinstance(scales, torch.Tensor) and scales.requires_grad:
