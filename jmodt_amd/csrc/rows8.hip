@@ -634,14 +634,17 @@ int jm_rows8_linear_wgrad(int m, int n, int k, int type, const void* dy, long lo
         (void)hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         hipLaunchKernelGGL(kernel, grid, block, lds, s, p);
     };
-    auto pick = [&](auto small_, auto tile_) {
+    auto tile = [&](auto type_, auto small_) {
+        constexpr int TY = decltype(type_)::value;
         constexpr bool S = decltype(small_)::value;
-        constexpr int W = decltype(tile_)::value;
-        run(type == JM_F32 ? rows8_wgrad_kernel<JM_F32, S, W> : (type == JM_BF16 ? rows8_wgrad_kernel<JM_BF16, S, W> : rows8_wgrad_kernel<JM_F16, S, W>));
+        if (plan.tile == 64) run(rows8_wgrad_kernel<TY, S, 64>);
+        else if constexpr (!S || TY != JM_F32) run(rows8_wgrad_kernel<TY, S, 128>);        // (n < 4 has small tiles)
     };
-    if (n < 4 || (type != JM_F32 && (((uintptr_t)dy & 3) || (lddy & 1)))) pick(std::true_type{}, std::integral_constant<int, 64>{});
-    else if (plan.tile == 64) pick(std::false_type{}, std::integral_constant<int, 64>{});
-    else pick(std::false_type{}, std::integral_constant<int, 128>{});
+    const bool small = n < 4 || (type != JM_F32 && (((uintptr_t)dy & 3) || (lddy & 1)));
+    auto pick = [&](auto type_) { small ? tile(type_, std::true_type{}) : tile(type_, std::false_type{}); };
+    if (type == JM_F32) pick(std::integral_constant<int, JM_F32>{});
+    else if (type == JM_BF16) pick(std::integral_constant<int, JM_BF16>{});
+    else pick(std::integral_constant<int, JM_F16>{});
     if (splits > 1) {
         const long long items = (long long)n * k + (dbias ? n : 0);
         hipLaunchKernelGGL(rows8_wgrad_reduce_kernel, dim3((unsigned)((items + 31) / 32)), dim3(512), 0, s, n, k, splits, splits * divup(k, plan.tile), (const float*)ws,

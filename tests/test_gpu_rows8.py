@@ -301,3 +301,16 @@ def test_outputs_over_inputs_are_refused():
     big = torch.randn(24, 24, device="cuda")
     with pytest.raises(RuntimeError):
         R8.linear_wgrad8(big, R8.checkpoint_rows(big), out=big)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,n,k", [(16400, 512, 512), (65600, 129, 256), (4200, 1000, 1030)])
+def test_wgrad_of_large_products_from_unaligned_rows(m, n, k, dtype):
+    """sizes that take the large tiles; rows behind an offset of one element (16-bit rows that are not 4-byte aligned)"""
+    dy, x8 = wgrad_case(m, n, k, dtype, 5)
+    want = R8.linear_wgrad8(dy, x8)
+    wgrad_check(dy, x8, want)
+    wide = torch.full((m, n + 3 - n % 2), float("nan"), device="cuda", dtype=dtype)
+    wide[:, 1:1 + n] = dy
+    got = R8.linear_wgrad8(wide[:, 1:1 + n], x8)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
