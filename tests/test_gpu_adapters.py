@@ -371,9 +371,9 @@ def test_beside_the_shared_projection_of_the_row_layers():
     assert none.any() and torch.equal(y[none], plain[none]) and not torch.equal(y, plain)
 
 
-@pytest.mark.parametrize("m,count", [(16384, 5), (64 * 4096, 3), (64 * 4096 + 1, 1023), (300001, 2)])
+@pytest.mark.parametrize("m,count", [(16384, 5), (64 * 4096, 3), (64 * 4096 + 1, 1023), (300001, 2), (2 ** 20 + 4099, 7)])
 def test_plan_of_many_rows(m, count):
-    """the same for tiles of 32 rows, and around the number of counting blocks that need one more launch; chunks too"""
+    """the same for tiles of 32 rows and counting blocks of more rows; chunks too"""
     ids = np.random.default_rng(m).integers(-1, count, m)
     p = AD.AdapterPlan(torch.from_numpy(ids.astype(np.int32)).cuda(), count).data.cpu().numpy()
     bucket = np.where(ids >= 0, ids, count)
@@ -472,3 +472,21 @@ def test_layer_has_no_second_derivative():
     g, = torch.autograd.grad(y.square().sum(), a, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+MANY = [(16384, 40, 72, 5, 6), (16500, 72, 40, 24, 3), (16384, 33, 50, 50, 2), (17000, 31, 70, 100, 4), (6000, 130, 66, 16, 2), (8200, 40, 30, 33, 1), (16383, 20, 24, 8, 5)]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,k,n,r,count", MANY)
+def test_forward_of_many_rows(m, k, n, r, count, dtype):
+    """tiles of 32 rows and the largest ones of 16"""
+    test_forward(m, k, n, r, count, dtype)
+
+
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,k,n,r,count", MANY)
+def test_grad_of_many_rows(m, k, n, r, count, dtype, kept):
+    """the weights transposed first and gathered, chunks of 256 and 512 rows"""
+    test_grad(m, k, n, r, count, dtype, kept)

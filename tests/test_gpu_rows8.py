@@ -314,3 +314,27 @@ def test_wgrad_of_large_products_from_unaligned_rows(m, n, k, dtype):
     wide[:, 1:1 + n] = dy
     got = R8.linear_wgrad8(wide[:, 1:1 + n], x8)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_keep_and_mask_of_many_rows():
+    """more items than the element-wise kernels have threads"""
+    y = make(70000, 129, torch.float32, seed=8, relu=True)
+    k = R8.checkpoint_rows(y)
+    codes, exps = encode_ref(y)
+    assert np.array_equal(codes & 127, k.codes.cpu().numpy()[:, :129] & 127) and np.array_equal(exps, k.exps.cpu().numpy())
+    assert torch.equal(R8.restore_rows(k).cpu(), torch.from_numpy(values(k.codes.cpu().numpy()[:, :129], exps)).float())
+    dy = torch.randn(70000, 129, device="cuda")
+    assert torch.equal(R8.relu_mask8(dy, k), torch.where(y > 0, dy, torch.zeros_like(dy)))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,n,k", [(1100, 2000, 2100), (300, 40, 50), (9000, 130, 70), (16400, 500, 520)])
+def test_wgrad_into_columns(m, n, k, dtype):
+    """large and small tiles, with one split of the rows and with many, into columns of a wider tensor"""
+    dy, x8 = wgrad_case(m, n, k, dtype, 6)
+    want = R8.linear_wgrad8(dy, x8)
+    wgrad_check(dy, x8, want)
+    wide = torch.full((n, k + 11), 7.0, device="cuda")
+    out, db = R8.linear_wgrad8(dy, x8, out=wide, col0=5)
+    assert out is wide and torch.equal(wide[:, 5:5 + k], want[0]) and torch.equal(db, want[1])
+    assert (wide[:, :5] == 7).all() and (wide[:, 5 + k:] == 7).all()
