@@ -184,7 +184,7 @@ rows8_relu_mask_kernel(int m, int c, int groups, const float* dy, long long ldd,
 // the other multiplies its own (48 matrix instructions of 32 x 32 x 16 a wave) and asks for its next rows between them; their sums are
 // added through LDS at the end, so a CU writes one partial tile.  The splits' partials are added in split order by the second kernel (no
 // float atomics: the same bits every time).
-// Measured (float32 / bfloat16 gradients, both kernels): 65536 x 256 x 256 39 / 27 us, 131072 x 512 x 512 230 / 103 us — 0.9 and 0.67
+// Measured (float32 / bfloat16 gradients, both kernels): 65536 x 256 x 256 39 / 28 us, 131072 x 512 x 512 212 / 97 us — 1.0 and 0.7
 // PFLOP/s on the bf16 pipe, where a library product of 8192^3 reaches 1.2; 512 x 512 x 512 9 / 7 us.  Bound by the two phases' own latencies
 // (LDS, barrier) more than by any one unit: the matrix pipe is busy half of the time in float32.
 constexpr int W8_SLAB = 8192;          // elements of one operand piece of a step: 64 rows x 128 columns or 128 x 64
@@ -497,56 +497,83 @@ rows8_wgrad_kernel(Wgrad8 p) {
     }
 }
 
-// out = the sum of the splits' partials: items 0 .. n k - 1 are dW, then n of db.  A workgroup takes 32 items (a cache line of every
-// partial); its 16 groups of 32 lanes sum every 16th split on four chains, the groups are added in order through LDS.
+// out = the sum of the splits' partials: first dW's n k, then db's n, V consecutive values a lane.  G groups of 512 / G lanes take every
+// G-th split on four chains, their sums are added in order through LDS (no float atomics: the same bits every time).  Four values a
+// lane and few groups for large results (4096 x 512 x 512, 4 splits, whole call in bfloat16: 15.3 us, with one value and 16 groups 19.5), one value and
+// up to 16 groups for small ones, where lanes are what is short (65536 x 64 x 64, 256 splits: 10.4 us, with four 11.4).
+template <int V, int G>
 __global__ void __launch_bounds__(512)
-rows8_wgrad_reduce_kernel(int n, int k, int splits_w, int splits_b, const float* __restrict__ part_w, const float* __restrict__ part_b, float* __restrict__ dw,
-                          long long lddw, float* __restrict__ db) {
-    __shared__ float red[16][32];
-    const long long nk = (long long)n * k;
-    const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
-    const long long i = blockIdx.x * 32ll + lane;
-    const bool w = i < nk, ok = i < nk + (db ? n : 0);
-    const float* src = w ? part_w + i : part_b + (ok ? i - nk : 0);
-    const size_t step = w ? (size_t)nk : (size_t)n;
-    const int splits = w ? splits_w : splits_b;
-    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-    if (ok) {
-        int t = grp;
-        for (; t + 48 < splits; t += 64) {
-            s0 += src[(size_t)t * step];        s1 += src[(size_t)(t + 16) * step];
-            s2 += src[(size_t)(t + 32) * step]; s3 += src[(size_t)(t + 48) * step];
-        }
-        for (; t < splits; t += 16) s0 += src[(size_t)t * step];
-    }
-    red[grp][lane] = (s0 + s1) + (s2 + s3);
-    __syncthreads();
-    if (grp > 0 || !ok) return;
-    float s = red[0][lane];
+rows8_wgrad_reduce_kernel(int n, int k, int splits_w, int splits_b, const float* __restrict__ part_w, const float* __restrict__ part_b,
+                          float* __restrict__ dw, long long lddw, float* __restrict__ db) {
+    __shared__ float red[512][V];
+    constexpr int lanes = 512 / G;
+    const int lane = threadIdx.x & (lanes - 1), grp = threadIdx.x / lanes;
+    const long long nk = (long long)n * k, items = (nk + V - 1) / V, item = (long long)blockIdx.x * lanes + lane;
+    const bool w = item < items;
+    const long long i = V * (w ? item : item - items), len = w ? nk : n;
+    const int left = (w || db) && i < len ? (int)min((long long)V, len - i) : 0, splits = w ? splits_w : splits_b;
+    const float* src = (w ? part_w : part_b) + i;
+    float s[4][V];
 #pragma unroll
-    for (int g = 1; g < 16; ++g) s += red[g][lane];
-    if (w) dw[(i / k) * lddw + i % k] = s;
-    else db[i - nk] = s;
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[u][e] = 0.f;
+    auto add = [&](float (&to)[V], int t) {
+        float v[V];
+        __builtin_memcpy(v, src + (size_t)t * len, sizeof(v));
+#pragma unroll
+        for (int e = 0; e < V; ++e) to[e] += v[e];
+    };
+    if (left == V) {
+        int t = grp;
+        for (; t + 3 * G < splits; t += 4 * G)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) add(s[u], t + u * G);
+        for (; t < splits; t += G) add(s[0], t);
+    } else if (left > 0) {
+        for (int t = grp; t < splits; t += G)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[0][e] += e < left ? src[(size_t)t * len + e] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[0][e] = (s[0][e] + s[1][e]) + (s[2][e] + s[3][e]);
+    if constexpr (G > 1) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) red[threadIdx.x][e] = s[0][e];
+        __syncthreads();
+        if (grp > 0) return;
+#pragma unroll
+        for (int g = 1; g < G; ++g)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[0][e] += red[g * lanes + lane][e];
+    }
+    long long r = w ? i / k : 0;
+    int c = w ? (int)(i - r * k) : 0;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        if (e < left) (w ? dw[r * lddw + c] : db[i + e]) = s[0][e];
+        if (++c == k) { c = 0; ++r; }
+    }
 }
 
-// Tiles of 128 x 128 halve what is read from the L2 and feed the matrix pipe best, but there have to be enough of them: with at least 4096
-// (tile, 64 rows) steps and both sides wider than 64 (one form of this kernel, float32: 65536 x 256 x 256 47 us against 52, 16384 x 1024 x
-// 1024 144 against 338); 64 x 64 otherwise (65536 x 64 x 64: 13 us against 18; 4096 x 512 x 512: 26 against 33).  Splits: up to one
-// workgroup a CU; what a split saves in steps (about 1.5 us each where the CU has nothing else to do) is weighed against the partials it
-// writes and the second kernel reads.
+// The tile and the number of splits (up to one workgroup a CU) by the time they take: about 1 us a step of a workgroup (1.05 in float32, 0.6 in
+// bfloat16, at either tile), 3.6 us more for the larger tile's longer start and end, and for splits 2.5 us and 0.9 us a MB of partials,
+// written and read again.  What that decides, both sides measured in float32: 1024 x 512 x 512, 64 x 64, 1 | 4 splits: 13.3 | 14.0 us;
+// 2048 rows: 21.5 | 16.4; 4096 x 1024 x 1024, 64 x 64 and 1 split | 128 x 128 and 4: 41.5 | 42.5 (bfloat16 26.5 | 33.3), 8192 rows: 76 | 64; 16384 x
+// 512 x 512, 64 x 64 and 4 | 128 x 128 and 16: 47.7 | 41.1; 65536 x 256 x 256, 16 | 64: 47.8 | 40.7.
 struct Wgrad8Plan { int tile, splits; };
 static Wgrad8Plan wgrad8_plan(int m, int n, int k) {
-    Wgrad8Plan p;
-    const bool wide = n > 64 && k > 64 && (long long)divup(n, 128) * divup(k, 128) * (m / 64) >= 4096;
-    p.tile = wide ? 128 : 64;
-    const int steps = imax(1, m / (W8_SLAB / p.tile));
-    const long long tiles = (long long)divup(n, p.tile) * divup(k, p.tile);
-    p.splits = 1;
-    float best = 1.5f * (float)steps;
-    for (long long s = 256 / tiles; s > 1; s /= 2) {
-        const int t = (int)(s > 256 ? 256 : (s > steps ? steps : s));
-        const float us = 1.5f * (float)divup(steps, t) + 3.f + 2.f * (float)t * (float)n * (float)k * 1e-6f;
-        if (t > 1 && us < best) { best = us; p.splits = t; }
+    Wgrad8Plan p{64, 1};
+    float best = 0.f;
+    for (int tile = 64; tile <= (n > 64 && k > 64 ? 128 : 64); tile *= 2) {
+        const int steps = imax(1, divup(m, W8_SLAB / tile));
+        const long long tiles = (long long)divup(n, tile) * divup(k, tile);
+        const float start = tile == 64 ? 0.f : 3.6f, rounds = (float)((tiles + 255) / 256);
+        for (long long s = imax(1, (int)(256 / tiles)); s > 0; s /= 2) {
+            const int t = (int)(s > steps ? steps : s);
+            const float us = start + rounds * (float)divup(steps, t) + (t > 1 ? 2.5f + 3.6e-6f * (float)t * (float)n * (float)k : 0.f);
+            if (best == 0.f || us < best) { best = us; p = {tile, t}; }
+        }
     }
     return p;
 }
@@ -646,9 +673,15 @@ int jm_rows8_linear_wgrad(int m, int n, int k, int type, const void* dy, long lo
     else if (type == JM_BF16) pick(std::integral_constant<int, JM_BF16>{});
     else pick(std::integral_constant<int, JM_F16>{});
     if (splits > 1) {
-        const long long items = (long long)n * k + (dbias ? n : 0);
-        hipLaunchKernelGGL(rows8_wgrad_reduce_kernel, dim3((unsigned)((items + 31) / 32)), dim3(512), 0, s, n, k, splits, splits * divup(k, plan.tile), (const float*)ws,
-                           (const float*)part_b, dw, lddw, dbias);
+        auto reduce = [&](auto v_, auto g_) {
+            constexpr int V = decltype(v_)::value, G = decltype(g_)::value;
+            const long long items = ((long long)n * k + V - 1) / V + (dbias ? divup(n, V) : 0);
+            hipLaunchKernelGGL((rows8_wgrad_reduce_kernel<V, G>), dim3((unsigned)((items + 512 / G - 1) / (512 / G))), dim3(512), 0, s, n, k, splits,
+                               splits * divup(k, plan.tile), (const float*)ws, (const float*)part_b, dw, lddw, dbias);
+        };
+        if ((long long)n * k < (1 << 17)) reduce(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+        else if (splits > 4) reduce(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
+        else reduce(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
     }
     return check_launch("rows8_linear_wgrad");
 }
