@@ -185,8 +185,9 @@ rows8_relu_mask_kernel(int m, int c, int groups, const float* dy, long long ldd,
 // added through LDS at the end, so a CU writes one partial tile.  The splits' partials are added in split order by the second kernel (no
 // float atomics: the same bits every time).
 // Measured (float32 / bfloat16 gradients, both kernels): 65536 x 256 x 256 39 / 28 us, 131072 x 512 x 512 212 / 97 us — 1.0 and 0.7
-// PFLOP/s on the bf16 pipe, where a library product of 8192^3 reaches 1.2; 512 x 512 x 512 9 / 7 us.  Bound by the two phases' own latencies
-// (LDS, barrier) more than by any one unit: the matrix pipe is busy half of the time in float32.
+// PFLOP/s on the bf16 pipe, where a library product of 8192^3 reaches 1.2; 512 x 512 x 512 9 / 7 us.  No one unit bounds it: of the
+// large bfloat16 case's 97 us staging and LDS reads alone take 70, the products alone 57 and the loads alone 56; what is lost is their
+// overlap.  (Two steps between barriers: 2 % less; a tile of 128 x 256: registers spill.)
 constexpr int W8_SLAB = 8192;          // elements of one operand piece of a step: 64 rows x 128 columns or 128 x 64
 
 struct Wgrad8 {
