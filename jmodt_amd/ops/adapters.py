@@ -191,4 +191,7 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor
         raise ValueError(f"keep must be 'float32' or 'e4m3', got {keep!r}")
     if isinstance(scales, torch.Tensor) and scales.requires_grad:
         raise ValueError("scales are constants of the layer: their gradient is not computed")
+    if not torch.is_grad_enabled():                          # (nothing is kept without a backward)
+        y = R.linear_forward(x, w, bias)
+        return adapter_forward(y, x, a.contiguous(), b.contiguous(), scales, plan, out=y)
     return _AdapterLinear.apply(x, w, bias, a, b, scales, plan, keep == "e4m3")

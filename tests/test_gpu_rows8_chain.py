@@ -159,3 +159,21 @@ def test_joint_step_with_kept_activations():
     a = train_joint.joint_step(eng, xyz, img, xy, tids, opt, rois_per_frame=K, route="rows")
     b = train_joint.joint_step(eng, xyz, img, xy, tids, opt, rois_per_frame=K, route="rows", keep="e4m3")
     assert torch.isfinite(b) and abs(float(a) - float(b)) <= 1e-4 * max(1.0, abs(float(a)))
+
+
+def test_nothing_is_kept_without_a_backward():
+    """under no_grad the same values, and nothing but the result stays allocated"""
+    from jmodt_amd.ops import adapters as AD
+    x1, x2, layers, acts, _ = chain(4000, 64, 0, (96, 32), (1, 0), seed=3)
+    y = R.rows_mlp(x1, layers, acts, keep="e4m3").detach()
+    ids = torch.arange(4000, device="cuda", dtype=torch.int32) % 3
+    a, b = torch.randn(3, 8, 64, device="cuda"), torch.randn(3, 96, 8, device="cuda")
+    plan, scales = AD.AdapterPlan(ids, 3), torch.ones(3, device="cuda")
+    w, bias = layers[0]
+    z = AD.adapter_linear(x1, w.detach(), bias.detach(), a, b, scales, plan, keep="e4m3").detach()
+    with torch.no_grad():
+        before = torch.cuda.memory_allocated()
+        y2 = R.rows_mlp(x1, layers, acts, keep="e4m3")
+        z2 = AD.adapter_linear(x1, w, bias, a, b, scales, plan, keep="e4m3")
+        assert torch.cuda.memory_allocated() - before <= y.numel() * 4 + z.numel() * 4 + 2048
+    assert torch.equal(y, y2) and torch.equal(z, z2) and not y2.requires_grad and not z2.requires_grad
