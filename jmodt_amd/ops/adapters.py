@@ -184,7 +184,7 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor
                    plan: AdapterPlan, keep: str = "float32") -> torch.Tensor:
     """y (M, N) = x w^T + bias + scales[a] B_a (A_a x): ops.rows.linear_forward and the rows' adapters, float32, differentiable in x, w,
     bias, a and b (a frozen projection: w and bias without requires_grad).  keep = "e4m3": x is kept in 8 bits for the backward
-    (da and dw from the kept values), "float32": as it is.  Widths are multiples of 4, as everywhere in ops.rows.
+    (da and dw from the kept values), "float32": as it is.  Widths are multiples of 4 and there is at least one row, as everywhere in ops.rows.
     Forward and backward can be captured into a HIP graph together; as with every autograd function, no eager graph of the same leaves may be
     alive then (autograd keeps a leaf's accumulation on the stream of its first live graph) — take torch.autograd.grad on fresh leaves."""
     if keep not in ("float32", "e4m3"):

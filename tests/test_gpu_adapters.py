@@ -490,3 +490,16 @@ def test_forward_of_many_rows(m, k, n, r, count, dtype):
 def test_grad_of_many_rows(m, k, n, r, count, dtype, kept):
     """the weights transposed first and gathered, chunks of 256 and 512 rows"""
     test_grad(m, k, n, r, count, dtype, kept)
+
+
+@pytest.mark.parametrize("keep", ["float32", "e4m3"])
+def test_layer_of_one_row_and_of_none(keep):
+    d, w, bias, plan = layer_case(seed=31, m=1, count=2)
+    ps = [v.detach().clone().requires_grad_() for v in (d["x"], w, bias, d["a"], d["b"])]
+    y = AD.adapter_linear(*ps, d["scales"], plan, keep=keep)
+    want = formula(d["x"].double(), w.double(), bias.double(), d["a"].double(), d["b"].double(), d["scales"].double(), d["ids"])
+    assert (y.double() - want).abs().max() <= 1e-5 * want.abs().max()
+    assert torch.equal(torch.autograd.grad(y, ps, d["dy"])[2], d["dy"][0])
+    none = AD.AdapterPlan(d["ids"][:0], 2)
+    with pytest.raises(RuntimeError):                     # the dense layers take at least one row
+        AD.adapter_linear(d["x"][:0], w, bias, d["a"], d["b"], d["scales"], none, keep=keep)
