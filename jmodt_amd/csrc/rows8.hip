@@ -200,6 +200,7 @@ struct Wgrad8 {
 
 // four consecutive columns of a row.  The columns of a group that lies outside the matrix are whatever lies inside (they only reach
 // outputs that are never stored); a group that straddles the edge (`ragged`, widths that are no multiple of 4) is read from width - 4 and shifted
+// (16-bit rows of an odd width in rows of an even stride: that read starts 2 bytes off a word and is exact, the bits of the column-by-column route)
 template <int TY> struct Quad;
 template <> struct Quad<JM_F32> {
     f32x4 v;
