@@ -805,7 +805,8 @@ int jm_rows8_pack(int m, int c, int type, const void* x, long long ldx, unsigned
 /* the values that the codes stand for, rounded once to the type (float32 and bfloat16 hold them exactly) */
 int jm_rows8_restore(int m, int c, int type, const unsigned char* codes, int ldc, const unsigned char* exps, int lde, void* out, long long ldo,
                      jm_stream_t stream);
-/* out (m, c) = (kept value > 0) ? dy : 0: the gradient through a ReLU whose output was kept; out may be dy */
+/* out (m, c) = (kept value > 0) ? dy : 0: the gradient through a ReLU whose output was kept; a kept value that is not finite counts as
+ * positive (a ReLU's output is never below zero: it was +infinity).  out may be dy */
 int jm_rows8_relu_mask(int m, int c, const float* dy, long long ldd, const unsigned char* codes, int ldc, float* out, long long ldo, jm_stream_t stream);
 /* dw (n, k) = dy (m, n)^T X (m, k) with X kept (codes, exps), dbias (n) = column sums of dy (NULL: skipped).  Sums in float32, in a
  * fixed order; lddy <= 2^22.  ws: >= jm_rows8_wgrad_workspace_bytes, 16-byte aligned. */

@@ -5,7 +5,8 @@ it — the weight gradient from the codes, the ReLU's mask from the codes.
 The format.  For a block of 32 channels of a row: amax = the largest finite |x|; the scale 2^e = the smallest power of two with
 amax <= 448 * 2^e, e >= -100; a code is x / 2^e rounded to the nearest e4m3 value (ties to even: at most 2^-4 of the value, within
 2^14 of the block's maximum).  A value that is not zero never becomes zero, so the sign pattern survives and the mask of a ReLU is
-exact; a value that is not finite becomes NaN (e4m3 has no infinity).  Kept values are exact in bfloat16 and float32.
+exact (of a ReLU's outputs only +infinity is not finite, and its gradient passes); a value that is not finite becomes NaN (e4m3 has no
+infinity).  Kept values are exact in bfloat16 and float32.
 
 No CPU path: every entry raises on tensors that are not on the current GPU.
 """
@@ -178,7 +179,8 @@ def restore_rows(x8: Rows8, dtype: torch.dtype = _f32) -> torch.Tensor:
 
 
 def relu_mask8(dy: torch.Tensor, y8: Rows8, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """kept y > 0 ? dy : 0 in float32 (a new tensor, or `out`, which may be dy): the gradient through a ReLU from its kept output"""
+    """kept y > 0 ? dy : 0 in float32 (a new tensor, or `out`, which may be dy): the gradient through a ReLU from its kept output.  A kept
+    value that is not finite counts as positive (a ReLU's output is never below zero: it was +infinity)"""
     m, c, pdy, ldd = _matrix(dy, "dy", _f32)
     m8, c8, pc, ld, _, _ = _kept(y8, "y8")
     if (m, c) != (m8, c8):
