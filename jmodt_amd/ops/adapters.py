@@ -167,8 +167,7 @@ class _AdapterLinear(Function):
             x, (w, a, b, scales, t) = Rows8(saved[0], *ctx.shape), saved[1:]
         else:
             x, (w, a, b, scales, t) = saved[0], saved[1:]
-        if dy.dim() != 2 or dy.stride(1) != 1 or dy.stride(0) % 4 or dy.stride(0) < dy.shape[1] or dy.data_ptr() % 16:
-            dy = dy.contiguous()
+        dy = R._gradient(dy)
         need = ctx.needs_input_grad
         base = R.linear_dgrad(dy, w, 0, w.shape[1]) if need[0] else None
         dx = da = db = dw = dbias = None

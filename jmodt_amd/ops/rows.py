@@ -38,6 +38,14 @@ def _rows(t: torch.Tensor, name: str) -> Tuple[ctypes.c_void_p, int]:
     return ctypes.c_void_p(t.data_ptr()), int(ld)
 
 
+def _gradient(dy: torch.Tensor) -> torch.Tensor:
+    """a gradient autograd handed in, as the row kernels read it: itself, or a copy where its strides or its address do not fit (one row for
+    all rows, transposed, contiguous but off a 16-byte address)"""
+    if dy.stride(1) == 1 and dy.stride(0) % 4 == 0 and dy.stride(0) >= dy.shape[1] and dy.data_ptr() % 16 == 0:
+        return dy
+    return dy.clone(memory_format=torch.contiguous_format)
+
+
 def _ws(nbytes: int, device) -> torch.Tensor:
     return torch.empty(((int(nbytes) + 3) // 4,), dtype=_f32, device=device)
 
@@ -181,8 +189,7 @@ class _RowsMLP(Function):
         Ws, ys = saved[:nl], saved[nl:]
         dev = x1.device
         M = x1.shape[0]
-        if not (dout.stride(1) == 1 and dout.stride(0) % 4 == 0 and dout.data_ptr() % 16 == 0):
-            dout = dout.contiguous()
+        dout = _gradient(dout)
         d = _RowsMLP._desc(x1, x2, acts, Ws, [None] * nl, ys)
         g = L.RowsMlpGrad()
         g.dout, g.lddout = dout.data_ptr(), dout.stride(0) if M > 1 else dout.shape[1]

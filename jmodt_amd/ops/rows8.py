@@ -255,8 +255,7 @@ class _RowsMLP8(Function):
         kept = [Rows8(d, *s) for d, s in zip(ctx.saved_tensors[:nk], ctx.shapes)]
         Ws = ctx.saved_tensors[nk:]
         inputs, ys = kept[:2 if ctx.has_x2 else 1], kept[2 if ctx.has_x2 else 1:]
-        if dy.stride(1) != 1 or dy.stride(0) % 4 or dy.stride(0) < dy.shape[1] or dy.data_ptr() % 16:
-            dy = dy.contiguous()
+        dy = R._gradient(dy)
         if acts[-1] == 1:
             dy = relu_mask8(dy, ys[-1])
         grads = [None] * (2 * len(acts))
