@@ -228,7 +228,8 @@ def rows_mlp(x1: torch.Tensor, layers: Sequence[Tuple[torch.Tensor, Optional[tor
         from .rows8 import _RowsMLP8
         if any(int(a) not in (0, 1) for a in acts):
             raise ValueError("keep='e4m3' takes layers without activation or with ReLU (the gradient of tanh needs its output)")
-        if torch.is_grad_enabled():                          # (nothing is kept without a backward; the values are the same)
+        # (nothing is kept where no backward can follow; the values are the same)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x1, x2, *flat)):
             return _RowsMLP8.apply(x1, x2, tuple(int(a) for a in acts), *flat)
     elif keep != "float32":
         raise ValueError(f"keep must be 'float32' or 'e4m3', got {keep!r}")

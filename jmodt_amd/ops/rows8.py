@@ -230,47 +230,55 @@ def linear_wgrad8(dy: torch.Tensor, x8: Rows8, want_bias: bool = True, out: Opti
 class _RowsMLP8(Function):
     """ops.rows._RowsMLP with its inputs and its hidden activations kept in 8 bits: apply(x1, x2 or None, acts, W_0, b_0, W_1, b_1, ...), acts
     in {0 none, 1 ReLU}.  The forward's values are the float32 route's own; of the gradients only dW_l see the rounding of the kept
-    activations (the masks are exact, dx and db need none of them)."""
+    activations (the masks are exact, dx and db need none of them).  Only what a gradient needs is kept and computed: an input for its
+    layer's weight, an output for the mask of its ReLU, and nothing below the last layer that something trains in."""
 
     @staticmethod
     def forward(ctx, x1, x2, acts, *wb):
         from . import rows as R
-        Ws, bs = wb[0::2], wb[1::2]
-        kept = [checkpoint_rows(x1)] + ([checkpoint_rows(x2)] if x2 is not None else [])
+        Ws, bs, nl = wb[0::2], wb[1::2], len(acts)
+        need = ctx.needs_input_grad
+        need_w, train = need[3::2], [w or b for w, b in zip(need[3::2], need[4::2])]
+        # the last layer that the backward walks down to; -1: through all of them, to the inputs
+        ctx.low = -1 if need[0] or need[1] else train.index(True) if True in train else nl
+        kept = [checkpoint_rows(x) if x is not None and need_w[0] else None for x in (x1, x2)]
         cur, cur2 = x1, x2
         for l, act in enumerate(acts):
             cur, cur2 = R.linear_forward(cur, Ws[l], bs[l], act, x2=cur2), None
-            if act == 1 or l + 1 < len(acts):
-                kept.append(checkpoint_rows(cur))
-        ctx.acts, ctx.has_x2, ctx.has_b = acts, x2 is not None, tuple(b is not None for b in bs)
-        ctx.shapes = [k.shape for k in kept]
-        ctx.save_for_backward(*[k.data for k in kept], *Ws)
+            kept.append(checkpoint_rows(cur) if (act == 1 and l >= ctx.low) or (l + 1 < nl and need_w[l + 1]) else None)
+        ctx.acts, ctx.k = acts, (x1.shape[1], None if x2 is None else x2.shape[1])
+        ctx.shapes = [k and k.shape for k in kept]
+        ctx.save_for_backward(*[k and k.data for k in kept], *Ws)
         return cur
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         from . import rows as R
-        nk, acts, need = len(ctx.shapes), ctx.acts, ctx.needs_input_grad
-        kept = [Rows8(d, *s) for d, s in zip(ctx.saved_tensors[:nk], ctx.shapes)]
-        Ws = ctx.saved_tensors[nk:]
-        inputs, ys = kept[:2 if ctx.has_x2 else 1], kept[2 if ctx.has_x2 else 1:]
+        acts, nl, need = ctx.acts, len(ctx.acts), ctx.needs_input_grad
+        kept = [d if d is None else Rows8(d, *s) for d, s in zip(ctx.saved_tensors, ctx.shapes)]
+        Ws = ctx.saved_tensors[nl + 2:]
+        inputs, ys = kept[:2], kept[2:]
         dy = R._gradient(dy)
         if acts[-1] == 1:
             dy = relu_mask8(dy, ys[-1])
-        grads = [None] * (2 * len(acts))
-        for l in range(len(acts) - 1, 0, -1):
-            if need[3 + 2 * l] or need[4 + 2 * l]:
-                grads[2 * l], grads[2 * l + 1] = linear_wgrad8(dy, ys[l - 1], want_bias=ctx.has_b[l])
-            dy = R.linear_dgrad(dy, Ws[l], 0, Ws[l].shape[1])
-            if acts[l - 1] == 1:
-                relu_mask8(dy, ys[l - 1], out=dy)
-        if need[3] or need[4]:
-            dw = torch.empty(Ws[0].shape, dtype=_f32, device=dy.device)
-            k1 = inputs[0].shape[1]
-            grads[0], grads[1] = linear_wgrad8(dy, inputs[0], want_bias=ctx.has_b[0], out=dw)
-            if ctx.has_x2:
-                linear_wgrad8(dy, inputs[1], want_bias=False, out=dw, col0=k1)
-        dx1 = R.linear_dgrad(dy, Ws[0], 0, inputs[0].shape[1]) if need[0] else None
-        dx2 = R.linear_dgrad(dy, Ws[0], inputs[0].shape[1], inputs[1].shape[1]) if ctx.has_x2 and need[1] else None
+        grads = [None] * (2 * nl)
+        for l in range(nl - 1, max(ctx.low, 0) - 1, -1):
+            need_w, need_b = need[3 + 2 * l], need[4 + 2 * l]
+            if need_w and l > 0:
+                grads[2 * l], grads[2 * l + 1] = linear_wgrad8(dy, ys[l - 1], want_bias=need_b)
+            elif need_w:
+                k1, k2 = ctx.k
+                dw = torch.empty(Ws[0].shape, dtype=_f32, device=dy.device)
+                grads[0], grads[1] = linear_wgrad8(dy, inputs[0], want_bias=need_b, out=dw)
+                if k2 is not None:
+                    linear_wgrad8(dy, inputs[1], want_bias=False, out=dw, col0=k1)
+            elif need_b:
+                grads[2 * l + 1] = R.colsum(dy)
+            if l > max(ctx.low, 0):
+                dy = R.linear_dgrad(dy, Ws[l], 0, Ws[l].shape[1])
+                if acts[l - 1] == 1:
+                    relu_mask8(dy, ys[l - 1], out=dy)
+        dx1 = R.linear_dgrad(dy, Ws[0], 0, ctx.k[0]) if need[0] else None
+        dx2 = R.linear_dgrad(dy, Ws[0], ctx.k[0], ctx.k[1]) if need[1] else None
         return (dx1, dx2, None, *grads)
