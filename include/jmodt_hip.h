@@ -833,6 +833,15 @@ int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const
                     const unsigned char* codes, int ldc, const unsigned char* exps, int lde, const float* t, const void* a, const void* b, const float* scales,
                     const int* plan, const void* base, long long ldb, void* dx, long long lddx, void* da, void* db, void* ws, size_t ws_bytes,
                     jm_stream_t stream);
+/* the results named alone, the same bits: without dx neither base nor dx is touched, without da neither x nor its kept form is needed, without
+ * db no t */
+#define JM_ADAPTER_DX 1
+#define JM_ADAPTER_DA 2
+#define JM_ADAPTER_DB 4
+int jm_adapter_grad_select(int results, int m, int k, int n, int rank, int adapters, int type, const void* dy, long long lddy, const void* x, long long ldx,
+                           const unsigned char* codes, int ldc, const unsigned char* exps, int lde, const float* t, const void* a, const void* b, const float* scales,
+                           const int* plan, const void* base, long long ldb, void* dx, long long lddx, void* da, void* db, void* ws, size_t ws_bytes,
+                           jm_stream_t stream);
 
 #pragma GCC visibility pop
 #ifdef __cplusplus

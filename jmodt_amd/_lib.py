@@ -232,6 +232,7 @@ SIGNATURES = {
     "jm_adapter_forward": (_I, [_I] * 6 + [_P, _L, _P, _P, _P, _P, _P, _L, _P, _L, _P, _P]),
     "jm_adapter_grad_workspace_bytes": (_Z, [_I] * 6),
     "jm_adapter_grad": (_I, [_I] * 6 + [_P, _L, _P, _L, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _L, _P, _L, _P, _P, _P, _Z, _P]),
+    "jm_adapter_grad_select": (_I, [_I] * 7 + [_P, _L, _P, _L, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _L, _P, _L, _P, _P, _P, _Z, _P]),
     "jm_rows_gate_backward": (_I, [_I, _I, _I, _P, _I, _P, _I, _P, _P, _I, _P, _P, _P, _I, _P]),
 }
 

@@ -943,15 +943,17 @@ size_t jm_adapter_grad_workspace_bytes(int m, int k, int n, int rank, int adapte
     return grad_layout(m, k, n, rank, adapters, type).total;
 }
 
-int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const void* dy, long long lddy, const void* x, long long ldx,
-                    const unsigned char* codes, int ldc, const unsigned char* exps, int lde, const float* t, const void* a, const void* b, const float* scales,
-                    const int* plan, const void* base, long long ldb, void* dx, long long lddx, void* da, void* db, void* ws, size_t ws_bytes,
-                    jm_stream_t stream) {
+int jm_adapter_grad_select(int results, int m, int k, int n, int rank, int adapters, int type, const void* dy, long long lddy, const void* x, long long ldx,
+                           const unsigned char* codes, int ldc, const unsigned char* exps, int lde, const float* t, const void* a, const void* b, const float* scales,
+                           const int* plan, const void* base, long long ldb, void* dx, long long lddx, void* da, void* db, void* ws, size_t ws_bytes,
+                           jm_stream_t stream) {
     if (int e = adapter_check("adapter_grad", m, k, n, rank, adapters, type)) return e;
-    JM_REQUIRE(lddy >= n && lddx >= k && (!base || ldb >= k), "adapter_grad: lddy %lld, ldb %lld, lddx %lld for k %d, n %d", lddy, ldb, lddx, k, n);
-    JM_REQUIRE(x ? ldx >= k : (m == 0 || (codes && exps && ldc >= k && ldc % 16 == 0 && lde >= m && lde % 16 == 0 && (((uintptr_t)codes | (uintptr_t)exps) & 15) == 0)),
+    JM_REQUIRE(results >= 0 && results <= (JM_ADAPTER_DX | JM_ADAPTER_DA | JM_ADAPTER_DB), "adapter_grad: results %d", results);
+    const bool want_dx = results & JM_ADAPTER_DX, want_da = results & JM_ADAPTER_DA, want_db = results & JM_ADAPTER_DB;
+    JM_REQUIRE(lddy >= n && (!want_dx || (lddx >= k && (!base || ldb >= k))), "adapter_grad: lddy %lld, ldb %lld, lddx %lld for k %d, n %d", lddy, ldb, lddx, k, n);
+    JM_REQUIRE(!want_da || (x ? ldx >= k : (m == 0 || (codes && exps && ldc >= k && ldc % 16 == 0 && lde >= m && lde % 16 == 0 && (((uintptr_t)codes | (uintptr_t)exps) & 15) == 0))),
                "adapter_grad: x or its kept rows are needed (ldx %lld, ldc %d, k %d)", ldx, ldc, k);
-    JM_REQUIRE(a && b && scales && plan && da && db && (m == 0 || (dy && t && dx)), "adapter_grad: NULL buffers");
+    JM_REQUIRE(a && b && scales && plan && (!want_da || da) && (!want_db || db) && (m == 0 || (dy && (!want_db || t) && (!want_dx || dx))), "adapter_grad: NULL buffers");
     const GradLayout gl = grad_layout(m, k, n, rank, adapters, type);
     if (!ws || ws_bytes < gl.total || ((uintptr_t)ws & 15)) {
         set_error("adapter_grad: workspace of %zu bytes (16-byte aligned), need %zu", ws_bytes, gl.total);
@@ -961,12 +963,13 @@ int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const
     const PlanLayout l = plan_layout(m, adapters);
     char* w = (char*)ws;
     AdaptGrad q{};
-    q.m = m; q.k = k; q.n = n; q.rank = rank; q.adapters = adapters; q.plan = plan; q.o_order = l.order; q.o_chunks = l.chunks;
+    // (a weight gradient that is not wanted is a matrix without channels)
+    q.m = m; q.k = want_da ? k : 0; q.n = want_db ? n : 0; q.rank = rank; q.adapters = adapters; q.plan = plan; q.o_order = l.order; q.o_chunks = l.chunks;
     q.o_chunk_first = l.chunk_first; q.x = x; q.ldx = ldx; q.codes = codes; q.ldc = ldc; q.exps = exps; q.lde = lde;
     q.dy = dy; q.lddy = lddy; q.t = t; q.u = (const float*)(w + gl.u); q.scales = scales; q.part = (float*)(w + gl.part); q.direct = m > 0 && m <= AD_CHUNK; q.da = da; q.db = db;
     const int groups = q.direct ? adapters : l.max_chunks;
     JM_REQUIRE((long long)groups * (divup(k, 64) + divup(n, 64)) * divup(rank, 16) < 1 << 24, "adapter_grad: too many (chunk, tile) pairs (m %d, k %d, n %d, rank %d)", m, k, n, rank);
-    if (m > 0) {
+    if (m > 0 && (want_dx || want_da)) {
         const bool wt = ad_tile(m) == 16;
         if (!wt) {
             const dim3 gt((unsigned)((divup(k, 32) + divup(n, 32)) * divup(rank, 32)), (unsigned)adapters);
@@ -977,12 +980,17 @@ int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const
                 hipLaunchKernelGGL((adapter_transpose_kernel<u16>), gt, dim3(256), 0, s, rank, k, n, (const u16*)a, (u16*)(w + gl.at), (const u16*)b, (u16*)(w + gl.bt));
             }
         }
+        // (without dx: outputs without channels, u only)
         Adapt p{};
-        p.m = m; p.k = n; p.n = k; p.rank = rank; p.plan = plan; p.o_order = l.order; p.o_tiles = l.tiles; p.x = dy; p.ldx = lddy;
-        p.a = wt ? b : w + gl.bt; p.b = wt ? a : w + gl.at; p.scales = scales; p.base = base; p.ldb = ldb; p.out = dx; p.ldo = lddx; p.t = (float*)(w + gl.u);
-        p.copy = base != dx;
+        p.m = m; p.k = n; p.n = want_dx ? k : 0; p.rank = rank; p.plan = plan; p.o_order = l.order; p.o_tiles = l.tiles; p.x = dy; p.ldx = lddy;
+        p.a = wt ? b : w + gl.bt; p.b = wt ? a : w + gl.at; p.scales = scales; p.base = base; p.ldb = ldb; p.out = dx; p.ldo = lddx;
+        p.t = want_da ? (float*)(w + gl.u) : nullptr;
+        p.copy = want_dx && base != dx;
         launch_rows(type, p, wt, l.max_tiles, s);
-        if (x) {
+    }
+    if (!want_da && !want_db) return check_launch("adapter_grad");
+    if (m > 0) {
+        if (x || !want_da) {
             if (type == JM_F32) launch_wgrad<JM_F32, false>(q, groups, s);
             else if (type == JM_BF16) launch_wgrad<JM_BF16, false>(q, groups, s);
             else launch_wgrad<JM_F16, false>(q, groups, s);
@@ -993,11 +1001,19 @@ int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const
         }
     }
     if (q.direct) return check_launch("adapter_grad");
-    const dim3 gr((unsigned)divup(rank * (k + n), 256), (unsigned)adapters);
+    const dim3 gr((unsigned)divup(rank * (q.k + q.n), 256), (unsigned)adapters);
     if (type == JM_F32) hipLaunchKernelGGL((adapter_wgrad_reduce_kernel<float>), gr, dim3(256), 0, s, q);
     else if (type == JM_BF16) hipLaunchKernelGGL((adapter_wgrad_reduce_kernel<__bf16>), gr, dim3(256), 0, s, q);
     else hipLaunchKernelGGL((adapter_wgrad_reduce_kernel<_Float16>), gr, dim3(256), 0, s, q);
     return check_launch("adapter_grad");
+}
+
+int jm_adapter_grad(int m, int k, int n, int rank, int adapters, int type, const void* dy, long long lddy, const void* x, long long ldx,
+                    const unsigned char* codes, int ldc, const unsigned char* exps, int lde, const float* t, const void* a, const void* b, const float* scales,
+                    const int* plan, const void* base, long long ldb, void* dx, long long lddx, void* da, void* db, void* ws, size_t ws_bytes,
+                    jm_stream_t stream) {
+    return jm_adapter_grad_select(JM_ADAPTER_DX | JM_ADAPTER_DA | JM_ADAPTER_DB, m, k, n, rank, adapters, type, dy, lddy, x, ldx, codes, ldc, exps, lde, t, a, b, scales,
+                                  plan, base, ldb, dx, lddx, da, db, ws, ws_bytes, stream);
 }
 
 }  // extern "C"

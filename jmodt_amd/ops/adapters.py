@@ -111,72 +111,85 @@ def adapter_forward(base: Optional[torch.Tensor], x: torch.Tensor, a: torch.Tens
     return (out, t) if want_t else out
 
 
-def adapter_grad(dy: torch.Tensor, x: Union[torch.Tensor, Rows8], t: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, plan: AdapterPlan,
-                 base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def adapter_grad(dy: torch.Tensor, x: Union[torch.Tensor, Rows8, None], t: Optional[torch.Tensor], a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor,
+                 plan: AdapterPlan, base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                 need: Tuple[bool, bool, bool] = (True, True, True)) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
     """the gradients of adapter_forward: dy (M, N), x (M, K) or its kept form, t from the forward ->
     (dx (M, K) = base + scales[a] A_a^T (B_a^T dy), da like a, db like b).  base: the shared projection's data gradient, or None;
-    out: a tensor for dx (base itself: in place).  An adapter without rows gets zeros.  Infinities in x or dy (bfloat16) may give NaN in da and db."""
+    out: a tensor for dx (base itself: in place).  need: which of the three are wanted, the same bits; the others are None and not computed
+    (base and out belong to dx; x may be None without da, t without db).  An adapter without rows gets zeros.  Infinities in x or dy
+    (bfloat16) may give NaN in da and db."""
     m, n, pdy, ldd = _matrix(dy, "dy")
+    if len(need) != 3:
+        raise ValueError(f"need: three truth values for dx, da and db, got {need!r}")
     px, ldx, pc, ldc, pe, lde = None, 0, None, 0, None, 0
+    others = [(dy, "dy"), (a, "a"), (b, "b"), (scales, "scales")]
     if isinstance(x, Rows8):
         mx, k, pc, ldc, pe, lde = _kept(x, "x")
-        source = x.data
-    else:
+        others.append((x.data, "x"))
+    elif x is not None or need[1]:
         mx, k, px, ldx = _matrix(x, "x", dy.dtype)
-        source = x
+        others.append((x, "x"))
         if m == 0:
             px = a.data_ptr()          # (an empty tensor has no address; nothing is read)
+    else:
+        mx, k = m, a.shape[2] if isinstance(a, torch.Tensor) and a.dim() == 3 else 0
     if mx != m:
         raise ValueError(f"dy of {m} rows for an input of {mx}")
     rank, count = _weights(a, b, scales, plan, dy.dtype, k, n, m)
-    _on_device(t, "t")
-    if t.dtype != _f32 or t.shape != (m, rank) or not t.is_contiguous():
-        raise TypeError(f"t must be a contiguous float32 tensor of ({m}, {rank}), got {t.dtype} {tuple(t.shape)}")
-    pb, ldb, dx, po, ldo = _result(base, out, m, k, dy, ((dy, "dy"), (source, "x"), (t, "t"), (a, "a"), (b, "b"), (scales, "scales"), (plan.data, "plan")))
-    da, db = torch.empty_like(a), torch.empty_like(b)
+    if t is not None or need[2]:
+        _on_device(t, "t")
+        if t.dtype != _f32 or t.shape != (m, rank) or not t.is_contiguous():
+            raise TypeError(f"t must be a contiguous float32 tensor of ({m}, {rank}), got {t.dtype} {tuple(t.shape)}")
+        others.append((t, "t"))
+    pb, ldb, dx, po, ldo = None, 0, None, None, 0
+    if need[0]:
+        pb, ldb, dx, po, ldo = _result(base, out, m, k, dy, others + [(plan.data, "plan")])
+    elif base is not None or out is not None:
+        raise ValueError("base and out belong to dx, which is not wanted")
+    da, db = torch.empty_like(a) if need[1] else None, torch.empty_like(b) if need[2] else None
     lib = L.load()
     kind = TYPES[dy.dtype]
     nbytes = lib.jm_adapter_grad_workspace_bytes(m, k, n, rank, count, kind)
     ws = torch.empty(((nbytes + 3) // 4,), dtype=_f32, device=dy.device)
-    L.check(lib.jm_adapter_grad(m, k, n, rank, count, kind, pdy, ldd, px, ldx, pc, ldc, pe, lde, t.data_ptr(), a.data_ptr(), b.data_ptr(), scales.data_ptr(),
-                                plan.data.data_ptr(), pb, ldb, po, ldo, da.data_ptr(), db.data_ptr(), ws.data_ptr(), nbytes, L.stream_ptr()), "adapter_grad")
+    L.check(lib.jm_adapter_grad_select((1 if need[0] else 0) | (2 if need[1] else 0) | (4 if need[2] else 0), m, k, n, rank, count, kind, pdy, ldd, px, ldx, pc, ldc,
+                                       pe, lde, None if t is None else t.data_ptr(), a.data_ptr(), b.data_ptr(), scales.data_ptr(), plan.data.data_ptr(), pb, ldb, po, ldo,
+                                       da.data_ptr() if need[1] else None, db.data_ptr() if need[2] else None, ws.data_ptr(), nbytes, L.stream_ptr()), "adapter_grad")
     return dx, da, db
 
 
 class _AdapterLinear(Function):
-    """apply(x, w, bias, a, b, scales, plan, keep): the dense layer and its adapters; keep: x is kept in 8 bits for the backward"""
+    """apply(x, w, bias, a, b, scales, plan, keep): the dense layer and its adapters; keep: x is kept in 8 bits for the backward (where w
+    or a needs it at all)"""
 
     @staticmethod
     def forward(ctx, x, w, bias, a, b, scales, plan, keep):
+        need = ctx.needs_input_grad
         y = R.linear_forward(x, w, bias)
         a, b = a.contiguous(), b.contiguous()
-        y, t = adapter_forward(y, x, a, b, scales, plan, out=y, want_t=True)
-        ctx.plan, ctx.keep, ctx.shape, ctx.has_bias = plan, keep, tuple(x.shape), bias is not None
-        if keep:
-            x8 = checkpoint_rows(x)
-            ctx.save_for_backward(x8.data, w, a, b, scales, t)
-        else:
-            ctx.save_for_backward(x, w, a, b, scales, t)
+        y, t = adapter_forward(y, x, a, b, scales, plan, out=y, want_t=True) if need[4] else (adapter_forward(y, x, a, b, scales, plan, out=y), None)
+        ctx.plan, ctx.keep, ctx.shape = plan, keep, tuple(x.shape)
+        kept = None if not (need[1] or need[3]) else checkpoint_rows(x).data if keep else x
+        ctx.save_for_backward(kept, w, a, b, scales, t)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        saved = ctx.saved_tensors
-        if ctx.keep:
-            x, (w, a, b, scales, t) = Rows8(saved[0], *ctx.shape), saved[1:]
-        else:
-            x, (w, a, b, scales, t) = saved[0], saved[1:]
+        x, w, a, b, scales, t = ctx.saved_tensors
+        if ctx.keep and x is not None:
+            x = Rows8(x, *ctx.shape)
         dy = R._gradient(dy)
         need = ctx.needs_input_grad
-        base = R.linear_dgrad(dy, w, 0, w.shape[1]) if need[0] else None
         dx = da = db = dw = dbias = None
         if need[0] or need[3] or need[4]:
-            dx, da, db = adapter_grad(dy, x, t, a, b, scales, ctx.plan, base=base, out=base)
-        if need[1] or (ctx.has_bias and need[2]):
-            dw, dbias = linear_wgrad8(dy, x, want_bias=ctx.has_bias) if ctx.keep else R.linear_wgrad(dy, [x], want_bias=ctx.has_bias)
-        return (dx if need[0] else None, dw if need[1] else None, dbias if ctx.has_bias and need[2] else None, da if need[3] else None,
-                db if need[4] else None, None, None, None)
+            base = R.linear_dgrad(dy, w, 0, w.shape[1]) if need[0] else None
+            dx, da, db = adapter_grad(dy, x, t, a, b, scales, ctx.plan, base=base, out=base, need=(need[0], need[3], need[4]))
+        if need[1]:
+            dw, dbias = linear_wgrad8(dy, x, want_bias=need[2]) if ctx.keep else R.linear_wgrad(dy, [x], want_bias=need[2])
+        elif need[2]:
+            dbias = R.colsum(dy)
+        return dx, dw, dbias, da, db, None, None, None
 
 
 def adapter_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor,
@@ -190,7 +203,8 @@ def adapter_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor
         raise ValueError(f"keep must be 'float32' or 'e4m3', got {keep!r}")
     if isinstance(scales, torch.Tensor) and scales.requires_grad:
         raise ValueError("scales are constants of the layer: their gradient is not computed")
-    if not torch.is_grad_enabled():                          # (nothing is kept without a backward)
+    # (nothing is kept where no backward can follow)
+    if not (torch.is_grad_enabled() and any(isinstance(v, torch.Tensor) and v.requires_grad for v in (x, w, bias, a, b))):
         y = R.linear_forward(x, w, bias)
         return adapter_forward(y, x, a.contiguous(), b.contiguous(), scales, plan, out=y)
     return _AdapterLinear.apply(x, w, bias, a, b, scales, plan, keep == "e4m3")
