@@ -877,15 +877,17 @@ static void launch_wgrad(const AdaptGrad& p, int groups, hipStream_t s) {
     else if constexpr (TY != JM_BF16) hipLaunchKernelGGL((adapter_wgrad_kernel<TY, KEPT, 4, 4>), grid, block, 0, s, p);
 }
 
+// at, bt: the transposed weights, where they are transposed (tiles of 32 rows); part: the chunks' partials, where there are any
 struct GradLayout { size_t at, bt, u, part, total; };        // bytes
 static GradLayout grad_layout(int m, int k, int n, int rank, int adapters, int type) {
     const PlanLayout l = plan_layout(m, adapters);
+    const size_t transposed = ad_tile(m) == 32 ? (size_t)adapters * rank * elem_size(type) : 0, chunks = m > AD_CHUNK ? l.max_chunks : 0;
     GradLayout g;
     g.at = 0;
-    g.bt = align_up(g.at + (size_t)adapters * k * rank * elem_size(type), 256);
-    g.u = align_up(g.bt + (size_t)adapters * n * rank * elem_size(type), 256);
-    g.part = align_up(g.u + (size_t)m * rank * 4, 256);
-    g.total = g.part + (size_t)l.max_chunks * rank * ((size_t)k + n) * 4;
+    g.bt = align_up(g.at + transposed * k, 256);
+    g.u = align_up(g.bt + transposed * n, 256);
+    g.part = align_up(g.u + (size_t)imax(m, 1) * rank * 4, 256);
+    g.total = g.part + chunks * rank * ((size_t)k + n) * 4;
     return g;
 }
 
