@@ -217,23 +217,33 @@ class _RowsMLP(Function):
 
 
 def rows_mlp(x1: torch.Tensor, layers: Sequence[Tuple[torch.Tensor, Optional[torch.Tensor]]], acts: Sequence[int],
-             x2: Optional[torch.Tensor] = None, keep: str = "float32") -> torch.Tensor:
+             x2: Optional[torch.Tensor] = None, keep: str = "float32", held: Sequence[str] = (), kept=None, want_kept: bool = False):
     """[x1 | x2] (M, k1 + k2) through the dense layers [(W (n, k), b (n) or None), ...] with activations acts.
     keep: what the backward finds of the inputs and the hidden activations — "float32": themselves; "e4m3": their 8-bit form
-    (ops/rows8.py: a quarter of the memory, weight gradients from the rounded activations, everything else as before; no tanh)"""
+    (ops/rows8.py: a quarter of the memory, weight gradients from the rounded activations, everything else as before; no tanh).
+    With "e4m3" — held: those of "x1", "x2" and "y" (the result) that something else keeps in float32 until the backward anyway, another
+    node of the graph or the caller: an 8-bit copy would come on top, so they are saved as they are; kept: x1's kept form (ops/rows8.Rows8)
+    where the chain before made it; want_kept: (y, y's kept form or None) instead of y, for the chain behind."""
     flat = []
     for W, b in layers:
         flat += [W, b]
+    if keep not in ("float32", "e4m3"):
+        raise ValueError(f"keep must be 'float32' or 'e4m3', got {keep!r}")
+    if any(h not in ("x1", "x2", "y") for h in held):
+        raise ValueError(f"held names x1, x2 and y, got {tuple(held)!r}")
     if keep == "e4m3":
-        from .rows8 import _RowsMLP8
+        from .rows8 import Rows8, _RowsMLP8
         if any(int(a) not in (0, 1) for a in acts):
             raise ValueError("keep='e4m3' takes layers without activation or with ReLU (the gradient of tanh needs its output)")
+        if kept is not None and (not isinstance(kept, Rows8) or kept.shape != tuple(x1.shape)):
+            raise ValueError(f"kept: the kept form of x1 {tuple(x1.shape)}, got {kept.shape if isinstance(kept, Rows8) else type(kept).__name__}")
         # (nothing is kept where no backward can follow; the values are the same)
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x1, x2, *flat)):
-            return _RowsMLP8.apply(x1, x2, tuple(int(a) for a in acts), *flat)
-    elif keep != "float32":
-        raise ValueError(f"keep must be 'float32' or 'e4m3', got {keep!r}")
-    return _RowsMLP.apply(x1, x2, tuple(int(a) for a in acts), *flat)
+            box = []
+            y = _RowsMLP8.apply(x1, x2, tuple(int(a) for a in acts), tuple(held), kept, box, *flat)
+            return (y, box[0]) if want_kept else y
+    y = _RowsMLP.apply(x1, x2, tuple(int(a) for a in acts), *flat)
+    return (y, None) if want_kept else y
 
 
 # ---------------------------------------------------------------------------------------------------- set abstraction on rows

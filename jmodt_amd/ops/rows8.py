@@ -228,27 +228,35 @@ def linear_wgrad8(dy: torch.Tensor, x8: Rows8, want_bias: bool = True, out: Opti
 
 
 class _RowsMLP8(Function):
-    """ops.rows._RowsMLP with its inputs and its hidden activations kept in 8 bits: apply(x1, x2 or None, acts, W_0, b_0, W_1, b_1, ...), acts
-    in {0 none, 1 ReLU}.  The forward's values are the float32 route's own; of the gradients only dW_l see the rounding of the kept
-    activations (the masks are exact, dx and db need none of them).  Only what a gradient needs is kept and computed: an input for its
-    layer's weight, an output for the mask of its ReLU, and nothing below the last layer that something trains in."""
+    """ops.rows._RowsMLP with its inputs and its hidden activations kept in 8 bits: apply(x1, x2 or None, acts, held, k1, box, W_0, b_0, W_1,
+    b_1, ...), acts in {0 none, 1 ReLU}.  The forward's values are the float32 route's own; of the gradients only dW_l see the rounding of
+    the kept activations (the masks are exact, dx and db need none of them).  Only what a gradient needs is kept and computed: an input for
+    its layer's weight, an output for the mask of its ReLU, and nothing below the last layer that something trains in.
+    held: those of "x1", "x2", "y" that are kept in float32 elsewhere and saved as they are; k1: x1's kept form where there is one; box: a list
+    that takes y's (or None)."""
 
     @staticmethod
-    def forward(ctx, x1, x2, acts, *wb):
+    def forward(ctx, x1, x2, acts, held, k1, box, *wb):
         from . import rows as R
         Ws, bs, nl = wb[0::2], wb[1::2], len(acts)
         need = ctx.needs_input_grad
-        need_w, train = need[3::2], [w or b for w, b in zip(need[3::2], need[4::2])]
+        need_w, train = need[6::2], [w or b for w, b in zip(need[6::2], need[7::2])]
         # the last layer that the backward walks down to; -1: through all of them, to the inputs
         ctx.low = -1 if need[0] or need[1] else train.index(True) if True in train else nl
-        kept = [checkpoint_rows(x) if x is not None and need_w[0] else None for x in (x1, x2)]
+        keep = []
+        for x, name, k in ((x1, "x1", k1), (x2, "x2", None)):
+            keep.append(None if x is None or not need_w[0] else x if name in held else k or checkpoint_rows(x))
         cur, cur2 = x1, x2
         for l, act in enumerate(acts):
             cur, cur2 = R.linear_forward(cur, Ws[l], bs[l], act, x2=cur2), None
-            kept.append(checkpoint_rows(cur) if (act == 1 and l >= ctx.low) or (l + 1 < nl and need_w[l + 1]) else None)
+            if (act == 1 and l >= ctx.low) or (l + 1 < nl and need_w[l + 1]):
+                keep.append(cur if l + 1 == nl and "y" in held else checkpoint_rows(cur))
+            else:
+                keep.append(None)
+        box.append(keep[-1] if isinstance(keep[-1], Rows8) else None)
         ctx.acts, ctx.k = acts, (x1.shape[1], None if x2 is None else x2.shape[1])
-        ctx.shapes = [k and k.shape for k in kept]
-        ctx.save_for_backward(*[k and k.data for k in kept], *Ws)
+        ctx.shapes = [k.shape if isinstance(k, Rows8) else None for k in keep]
+        ctx.save_for_backward(*[k.data if isinstance(k, Rows8) else k for k in keep], *Ws)
         return cur
 
     @staticmethod
@@ -256,23 +264,29 @@ class _RowsMLP8(Function):
     def backward(ctx, dy):
         from . import rows as R
         acts, nl, need = ctx.acts, len(ctx.acts), ctx.needs_input_grad
-        kept = [d if d is None else Rows8(d, *s) for d, s in zip(ctx.saved_tensors, ctx.shapes)]
+        kept = [d if s is None else Rows8(d, *s) for d, s in zip(ctx.saved_tensors, ctx.shapes)]
         Ws = ctx.saved_tensors[nl + 2:]
         inputs, ys = kept[:2], kept[2:]
+
+        def wgrad(x, want_bias, out=None, col0=0):
+            if isinstance(x, Rows8):
+                return linear_wgrad8(dy, x, want_bias=want_bias, out=out, col0=col0)
+            return R.linear_wgrad(dy, [x], want_bias=want_bias, out=out, col0=col0)
+
         dy = R._gradient(dy)
         if acts[-1] == 1:
-            dy = relu_mask8(dy, ys[-1])
+            dy = relu_mask8(dy, ys[-1]) if isinstance(ys[-1], Rows8) else R.relu_mask(dy, ys[-1])
         grads = [None] * (2 * nl)
         for l in range(nl - 1, max(ctx.low, 0) - 1, -1):
-            need_w, need_b = need[3 + 2 * l], need[4 + 2 * l]
+            need_w, need_b = need[6 + 2 * l], need[7 + 2 * l]
             if need_w and l > 0:
-                grads[2 * l], grads[2 * l + 1] = linear_wgrad8(dy, ys[l - 1], want_bias=need_b)
+                grads[2 * l], grads[2 * l + 1] = wgrad(ys[l - 1], need_b)
             elif need_w:
                 k1, k2 = ctx.k
                 dw = torch.empty(Ws[0].shape, dtype=_f32, device=dy.device)
-                grads[0], grads[1] = linear_wgrad8(dy, inputs[0], want_bias=need_b, out=dw)
+                grads[0], grads[1] = wgrad(inputs[0], need_b, out=dw)
                 if k2 is not None:
-                    linear_wgrad8(dy, inputs[1], want_bias=False, out=dw, col0=k1)
+                    wgrad(inputs[1], False, out=dw, col0=k1)
             elif need_b:
                 grads[2 * l + 1] = R.colsum(dy)
             if l > max(ctx.low, 0):
@@ -281,4 +295,4 @@ class _RowsMLP8(Function):
                     relu_mask8(dy, ys[l - 1], out=dy)
         dx1 = R.linear_dgrad(dy, Ws[0], 0, ctx.k[0]) if need[0] else None
         dx2 = R.linear_dgrad(dy, Ws[0], ctx.k[0], ctx.k[1]) if need[1] else None
-        return (dx1, dx2, None, *grads)
+        return (dx1, dx2, None, None, None, None, *grads)

@@ -151,27 +151,29 @@ def _pad_rows(W: torch.Tensor, b: Optional[torch.Tensor], mult: int = 4):
 
 
 def _head_rows(fold: BnFold, head: nn.Sequential, x: torch.Tensor) -> torch.Tensor:
-    """a Conv1d head (rpn.py:34-58, rcnn.py:43-89) on rows: (M, C) -> (M, pad4(out)); Dropout between the units when active"""
+    """a Conv1d head (rpn.py:34-58, rcnn.py:43-89) on rows: (M, C) -> (M, pad4(out)); Dropout between the units when active.  x: features that
+    the caller returns, so in float32 they are there in any case"""
     units, cur_layers, cur_acts = list(head), [], []
-    out = x
+    out, held = x, ("x1",)
     for m in units:
         if isinstance(m, nn.Dropout):
             if m.training and m.p > 0:
                 if cur_layers:
-                    out = R.rows_mlp(out, cur_layers, cur_acts, keep=fold.keep)
+                    out = R.rows_mlp(out, cur_layers, cur_acts, keep=fold.keep, held=held)
                     cur_layers, cur_acts = [], []
-                out = F.dropout(out, m.p, True)
+                out, held = F.dropout(out, m.p, True), ()
             continue
         W, b = fold.unit(m)
         cur_layers.append(_pad_rows(W, b))
         cur_acts.append(1 if getattr(m, "activation", None) is not None else 0)
     if cur_layers:
-        out = R.rows_mlp(out, cur_layers, cur_acts, keep=fold.keep)
+        out = R.rows_mlp(out, cur_layers, cur_acts, keep=fold.keep, held=held)
     return out
 
 
-def _attention_rows(fold: BnFold, mod, point: torch.Tensor, img: torch.Tensor) -> torch.Tensor:
-    """AttentionFusion.forward (backbone.py:35-81) on rows: point (M, pc), img (M, ic) -> (M, oc)"""
+def _attention_rows(fold: BnFold, mod, point: torch.Tensor, img: torch.Tensor, out_held: bool = True) -> torch.Tensor:
+    """AttentionFusion.forward (backbone.py:35-81) on rows: point (M, pc), img (M, ic) -> (M, oc).  out_held: what takes the result keeps it
+    in float32 (set abstraction does, interpolation does not)"""
     ia = mod.IA_Layer
     rc = ia.fc1.weight.shape[0]
     # gate = sigmoid(fc3(tanh(fc1(img) + fc2(point)))): fc1 / fc2 as ONE two-operand layer
@@ -183,9 +185,11 @@ def _attention_rows(fold: BnFold, mod, point: torch.Tensor, img: torch.Tensor) -
     z = R.rows_mlp(t, [_pad_rows(w3, ia.fc3.bias)], [0])                                        # (M, 4): column 0 is the logit
     gate = torch.sigmoid(z[:, :1])
     Wi, bi = fold.conv(ia.conv1[0], ia.conv1[1])
-    j = R.rows_mlp(img, [(Wi, bi)], [1], keep=fold.keep) * gate
+    # in 8 bits only the gated image features, which nothing else holds: img and point are inputs of the tanh layer, whose backward has them
+    # in float32, and the multiplication by the gate keeps the projection's output
+    j = R.rows_mlp(img, [(Wi, bi)], [1]) * gate
     Wf, bf = fold.conv(mod.conv1, mod.bn1)
-    return R.rows_mlp(point, [(Wf, bf)], [1], x2=j, keep=fold.keep)
+    return R.rows_mlp(point, [(Wf, bf)], [1], x2=j, keep=fold.keep, held=("x1", "y") if out_held else ("x1",))
 
 
 def _sa_level_rows(fold: BnFold, sa, xyz: torch.Tensor, feats: Optional[torch.Tensor], new_xyz: torch.Tensor, grid=None,
@@ -357,7 +361,7 @@ def backbone_forward_rows(engine, xyz: torch.Tensor, image: torch.Tensor, pts_xy
                     torch.gather(l_xy[i], 1, idx.long().unsqueeze(-1).expand(-1, -1, 2)))
         main.wait_event(map_events[i])
         with prof.scope(f"li_fusion{i + 1}"):
-            feats = _attention_rows(fold, net.Fusion_Conv[i], feats, R.feature_gather_rows(maps[i], xy_i))
+            feats = _attention_rows(fold, net.Fusion_Conv[i], feats, R.feature_gather_rows(maps[i], xy_i), out_held=i + 1 < len(net.SA_modules))
         l_xyz.append(new_xyz); l_feats.append(feats); l_xy.append(xy_i)
     # the fused image map: issued here (under the feature-propagation modules), consumed by the final attention block
     if img_stream is not main:
@@ -376,7 +380,8 @@ def backbone_forward_rows(engine, xyz: torch.Tensor, image: torch.Tensor, pts_xy
             carried = R.three_interpolate_rows(l_feats[i], nn3, w)
             mlp = net.FP_modules[i].mlp
             layers = [fold.unit(u) for u in mlp]
-            l_feats[i - 1] = R.rows_mlp(carried, layers, [1] * len(layers), x2=l_feats[i - 1], keep=fold.keep)
+            # (the skip features are an input of set abstraction, the last module's result one of the final attention block: float32 both)
+            l_feats[i - 1] = R.rows_mlp(carried, layers, [1] * len(layers), x2=l_feats[i - 1], keep=fold.keep, held=("x2", "y") if i == -nfp else ("x2",))
     main.wait_event(fused_ev)
     with prof.scope("li_fusion_final"):
         out = _attention_rows(fold, net.final_fusion_img_point, l_feats[0], R.feature_gather_rows(fused_img, pts_xy))
@@ -418,9 +423,10 @@ def rcnn_forward_rows(engine, pts_input: torch.Tensor, fold: BnFold, count: Opti
     up = [fold.unit(u) for u in net.xyz_up_layer]
     W0, b0 = up[0]
     up[0] = (_pad_dim(W0, 1, x5.shape[1] - W0.shape[1]), b0)
-    xyz_feat = R.rows_mlp(x5, up, [1] * len(up), keep=fold.keep)
+    xyz_feat, kept = R.rows_mlp(x5, up, [1] * len(up), keep=fold.keep, want_kept=True)
     Wm, bm = fold.unit(net.merge_down_layer[0])
-    feats = R.rows_mlp(xyz_feat, [(Wm, bm)], [1], x2=rpn_feat, keep=fold.keep)              # (R S, C): merge_down on [xyz_feature | rpn_feature]
+    # (R S, C): merge_down on [xyz_feature | rpn_feature], the input of a set abstraction
+    feats = R.rows_mlp(xyz_feat, [(Wm, bm)], [1], x2=rpn_feat, keep=fold.keep, held=("y",), kept=kept)
     l_xyz = xyz
     canon = None
     if count is not None:
@@ -513,8 +519,8 @@ def joint_forward_rows(engine, xyz, image, pts_xy, rois_per_frame: int = 64, pyr
     Its backward runs on three streams (main, image, RCNN), each node on the stream of its forward; gradients cross streams only
     through the autograd engine's own hand-over.  Safe next to other live autograd graphs over the same parameters (an earlier
     step's outputs, DDP's stashed AccumulateGrad nodes: tests/test_gpu_rows.py holds two of them across ten asynchronous steps).
-    keep: "e4m3" = the dense layers keep their activations in 8 bits for the backward (ops.rows.rows_mlp; the set-abstraction scales and
-    the attention's tanh layer stay in float32)."""
+    keep: "e4m3" = the dense layers keep their activations in 8 bits for the backward (ops.rows.rows_mlp), but for those that a set-abstraction
+    scale, the attention's tanh layer and gate or the caller has in float32 anyway."""
     fold = BnFold(engine.rpn, keep=keep)
     out = rpn_forward_rows(engine, xyz, image, pts_xy, fold, pyr)
     rois, pts_input, count = pooled_rois(engine, xyz, out, rois_per_frame)
