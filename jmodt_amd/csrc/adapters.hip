@@ -238,9 +238,11 @@ struct Run16 {
 //      registers of the 16 x 16 products (lane: 8 consecutive elements of one row), UK steps in flight; the quarters are added through LDS.
 //   2  out (channels x rows) = base + s B t^T: a wave takes 64 channels; the rows of B are permuted so that a lane ends up with 16
 //      consecutive channels of its row, which it reads from base and writes to out.
-// t enters the second product as the sum of two values of the 16-bit type (16 significant bits in bfloat16, 22 in float16, where the
-// row is scaled by a power of two first: t may leave float16's range although out does not); as it is in float32.  With a rank of up
-// to 16 both values share one product: the contraction is 32 long, [hi | lo] times [B | B].
+// t enters the second product as it is in float32, as the sum of three values in bfloat16 (8 + 8 + 8 bits: all of float32's) and of two in
+// float16 (11 + 11 bits and the signs: 2^-23 of the row's largest value; the row is scaled by a power of two first, as t may leave float16's
+// range although out does not).  With two values in bfloat16, too (2^-17 of t), 0.1 % of the outputs rounded to the neighbouring value, and
+// where base and the adapter cancel it was more than out's own rounding.  With a rank of up to 16 two values share one product: the contraction
+// is 32 long, [hi | lo] times [B | B].
 // WT: A and B are given transposed, (k, rank) and (rank, n) — the backward on B and A as they are: their elements are gathered one by one,
 // which few tiles can afford and many cannot (there a kernel of its own transposes them first).
 // Bound by memory with many rows (x and base read, out written once: 65536 x 256 x 256 bfloat16, rank 32, t written: 29 us, 3.7 TB/s;
@@ -388,7 +390,8 @@ adapter_rows_kernel(Adapt p) {
     auto tval = [&](int mb, int r) { return r < p.rank ? ts[0][mb * 16 + i][r] + ts[1][mb * 16 + i][r] : 0.f; };
     float back[MB];
     f32x4 t32[TY == JM_F32 ? MB : 1][RS];
-    V8 hi[MB][RS], lo[MB][RS];
+    constexpr bool THREE = TY == JM_BF16;
+    V8 hi[MB][RS], lo[MB][RS], rest[THREE ? MB : 1][RS];
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
         back[mb] = scale;
@@ -419,9 +422,11 @@ adapter_rows_kernel(Adapt p) {
                 for (int e = 0; e < 8; ++e) {
                     const float f = v[s][e] * fit;
                     const T h = (T)f;
-                    const T r = (T)(fabsf((float)h) < __builtin_inff() ? f - (float)h : 0.f);
+                    const float left = fabsf((float)h) < __builtin_inff() ? f - (float)h : 0.f;
+                    const T r = (T)left;
                     hi[mb][s][e] = (PAIR && g >= 2) ? r : h;
                     lo[mb][s][e] = r;
+                    if constexpr (THREE) rest[mb][s][e] = (PAIR && g >= 2) ? (T)0.f : (T)(left - (float)r);
                 }
         }
     }
@@ -473,6 +478,7 @@ adapter_rows_kernel(Adapt p) {
                     for (int mb = 0; mb < MB; ++mb) {
                         d[mb][j] = mma16(d[mb][j], b8, hi[mb][s]);
                         if constexpr (!PAIR) d[mb][j] = mma16(d[mb][j], b8, lo[mb][s]);
+                        if constexpr (THREE) d[mb][j] = mma16(d[mb][j], b8, rest[mb][s]);
                     }
                 }
             }

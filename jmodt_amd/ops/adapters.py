@@ -100,7 +100,7 @@ def adapter_forward(base: Optional[torch.Tensor], x: torch.Tensor, a: torch.Tens
     out = base + scales[a] B_a (A_a x) row by row; rows without an adapter: base.  out: a tensor to write (base itself: in place),
     else a new one.  want_t: (out, t), t (M, R) float32 = A_a x, zero in rows without an adapter — what `adapter_grad` needs.
     A value that is not finite reaches its own row (in x) or its adapter's rows (in a, b) only; in bfloat16 and float16, where t enters as a
-    sum of two values, an infinity in b gives NaN."""
+    sum of several values, an infinity in b gives NaN."""
     m, k, px, ldx = _matrix(x, "x")
     n = b.shape[1] if isinstance(b, torch.Tensor) and b.dim() == 3 else 0
     rank, count = _weights(a, b, scales, plan, x.dtype, k, n, m)
