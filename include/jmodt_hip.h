@@ -806,7 +806,7 @@ int jm_rows8_pack(int m, int c, int type, const void* x, long long ldx, unsigned
 int jm_rows8_restore(int m, int c, int type, const unsigned char* codes, int ldc, const unsigned char* exps, int lde, void* out, long long ldo,
                      jm_stream_t stream);
 /* out (m, c) = (kept value > 0) ? dy : 0: the gradient through a ReLU whose output was kept; a kept value that is not finite counts as
- * positive (a ReLU's output is never below zero: it was +infinity).  out may be dy */
+ * positive (a ReLU's output is never below zero: it was +infinity).  out may be dy (with ldo == ldd) */
 int jm_rows8_relu_mask(int m, int c, const float* dy, long long ldd, const unsigned char* codes, int ldc, float* out, long long ldo, jm_stream_t stream);
 /* dw (n, k) = dy (m, n)^T X (m, k) with X kept (codes, exps), dbias (n) = column sums of dy (NULL: skipped).  Sums in float32, in a
  * fixed order; lddy <= 2^22.  ws: >= jm_rows8_wgrad_workspace_bytes, 16-byte aligned. */
@@ -825,7 +825,7 @@ int jm_adapter_plan(int m, int adapters, const int* ids, int* plan, jm_stream_t 
  * plan: jm_adapter_plan's for the same m and adapters. */
 int jm_adapter_forward(int m, int k, int n, int rank, int adapters, int type, const void* x, long long ldx, const void* a, const void* b,
                        const float* scales, const int* plan, const void* base, long long ldb, void* out, long long ldo, float* t, jm_stream_t stream);
-/* dx[r] = base[r] + scales[a] a_a^T (b_a^T dy[r]) (base NULL: zero; base == dx: in place); da_a = scales[a] sum (b_a^T dy[r]) x[r]^T,
+/* dx[r] = base[r] + scales[a] a_a^T (b_a^T dy[r]) (base NULL: zero; base == dx and ldb == lddx: in place); da_a = scales[a] sum (b_a^T dy[r]) x[r]^T,
  * db_a = scales[a] sum dy[r] t[r]^T over the rows of a (none: zero), float32 sums in a fixed order, rounded once.  x: rows of the
  * type, or NULL with the kept form (codes, exps) of jm_rows8_pack.  ws: 16-byte aligned. */
 size_t jm_adapter_grad_workspace_bytes(int m, int k, int n, int rank, int adapters, int type);

@@ -936,6 +936,7 @@ int jm_adapter_forward(int m, int k, int n, int rank, int adapters, int type, co
                        const float* scales, const int* plan, const void* base, long long ldb, void* out, long long ldo, float* t, jm_stream_t stream) {
     if (int e = adapter_check("adapter_forward", m, k, n, rank, adapters, type)) return e;
     JM_REQUIRE(ldx >= k && ldo >= n && (!base || ldb >= n), "adapter_forward: ldx %lld, ldb %lld, ldo %lld for k %d, n %d", ldx, ldb, ldo, k, n);
+    JM_REQUIRE(m <= 1 || !base || base != out || ldb == ldo, "adapter_forward: in place with rows %lld and %lld apart", ldb, ldo);
     if (m == 0) return JM_OK;
     JM_REQUIRE(x && a && b && scales && plan && out, "adapter_forward: NULL buffers");
     const PlanLayout l = plan_layout(m, adapters);
@@ -959,6 +960,7 @@ int jm_adapter_grad_select(int results, int m, int k, int n, int rank, int adapt
     JM_REQUIRE(results >= 0 && results <= (JM_ADAPTER_DX | JM_ADAPTER_DA | JM_ADAPTER_DB), "adapter_grad: results %d", results);
     const bool want_dx = results & JM_ADAPTER_DX, want_da = results & JM_ADAPTER_DA, want_db = results & JM_ADAPTER_DB;
     JM_REQUIRE(lddy >= n && (!want_dx || (lddx >= k && (!base || ldb >= k))), "adapter_grad: lddy %lld, ldb %lld, lddx %lld for k %d, n %d", lddy, ldb, lddx, k, n);
+    JM_REQUIRE(m <= 1 || !want_dx || !base || base != dx || ldb == lddx, "adapter_grad: in place with rows %lld and %lld apart", ldb, lddx);
     JM_REQUIRE(!want_da || (x ? ldx >= k : (m == 0 || (codes && exps && ldc >= k && ldc % 16 == 0 && lde >= m && lde % 16 == 0 && (((uintptr_t)codes | (uintptr_t)exps) & 15) == 0))),
                "adapter_grad: x or its kept rows are needed (ldx %lld, ldc %d, k %d)", ldx, ldc, k);
     JM_REQUIRE(a && b && scales && plan && (!want_da || da) && (!want_db || db) && (m == 0 || (dy && (!want_db || t) && (!want_dx || dx))), "adapter_grad: NULL buffers");

@@ -623,6 +623,7 @@ int jm_rows8_relu_mask(int m, int c, const float* dy, long long ldd, const unsig
                        jm_stream_t stream) {
     JM_REQUIRE(m >= 0 && m <= R8_MAX_ROWS && c > 0 && c <= R8_MAX_WIDTH && ldd >= c && ldo >= c && ldc >= c && ldc % 16 == 0,
                "rows8_relu_mask: m %d, c %d, ldd %lld, ldc %d, ldo %lld", m, c, ldd, ldc, ldo);
+    JM_REQUIRE(m <= 1 || !dy || dy != out || ldd == ldo, "rows8_relu_mask: in place with rows %lld and %lld apart", ldd, ldo);
     if (m == 0) return JM_OK;
     JM_REQUIRE(dy && codes && out && ((uintptr_t)codes & 15) == 0, "rows8_relu_mask: NULL or unaligned buffers");
     const int groups = divup(c, 4);
