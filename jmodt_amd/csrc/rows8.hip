@@ -314,9 +314,8 @@ rows8_wgrad_kernel(Wgrad8 p) {
         }
         if (do_bias && (p.splits == 1 || ((r - r_begin) / W8_R) % tk == kt)) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) bs[c] += y[q].get(c);
+            for (int c = 0; c < 4; ++c)                      // (pairs of pairs: an addition rounds at most 3 times before the step's sum)
+                bs[c] += ((y[0].get(c) + y[1].get(c)) + (y[2].get(c) + y[3].get(c))) + ((y[4].get(c) + y[5].get(c)) + (y[6].get(c) + y[7].get(c)));
         }
         if constexpr (P > 1) {
             float top = 0.f;
@@ -490,8 +489,11 @@ rows8_wgrad_kernel(Wgrad8 p) {
         sums[threadIdx.x] = f32x4{bs[0], bs[1], bs[2], bs[3]};       // (oct * G + l)
         __syncthreads();
         if (grp == 0 && tid < G) {
-            f32x4 s = sums[tid];
-            for (int o = 1; o < 512 / G; ++o) s += sums[o * G + tid];
+            f32x4 part[4] = {sums[tid], sums[G + tid], sums[2 * G + tid], sums[3 * G + tid]};
+            for (int o = 4; o < 512 / G; o += 4)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) part[u] += sums[(o + u) * G + tid];
+            const f32x4 s = (part[0] + part[1]) + (part[2] + part[3]);
             float* db = p.db + (p.splits > 1 ? ((size_t)split * tk + kt) * p.n : 0);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
