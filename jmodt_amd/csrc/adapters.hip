@@ -152,7 +152,7 @@ __device__ void plan_scatter(const int* __restrict__ ids, long long row0, int ro
 }
 
 // The plan reads ids twice and writes 4 bytes a row; launches and one block's barriers bound it: 4096 rows 10 us in one launch, 65536 rows
-// 12 us (4 adapters) and 13 us (64 in mixed order) in two, 2^20 rows 24 us.
+// 15 us (4 adapters) and 13 us (64 in mixed order) in two, 2^20 rows 25 us.
 // ids of one counting block counted in LDS; whole: the block is all there is and the plan is finished here (one launch)
 template <bool WHOLE>
 __global__ void __launch_bounds__(PL_THREADS)
@@ -245,9 +245,9 @@ struct Run16 {
 // is 32 long, [hi | lo] times [B | B].
 // WT: A and B are given transposed, (k, rank) and (rank, n) — the backward on B and A as they are: their elements are gathered one by one,
 // which few tiles can afford and many cannot (there a kernel of its own transposes them first).
-// Bound by memory with many rows (x and base read, out written once: 65536 x 256 x 256 bfloat16, rank 32, t written: 29 us, 3.7 TB/s;
-// 65536 x 512 x 512 float32, rank 16: 98 us, 4.1 TB/s, rank 64: 161 us — there the float32 pipe has 56 us of it), by the chain of loads through both
-// products with few (1024 x 512 x 512 float32, rank 16: 6.7 us).
+// Bound by memory with many rows (x and base read, out written once: 65536 x 256 x 256 bfloat16, rank 32, t written: 30 us, 3.7 TB/s;
+// 65536 x 512 x 512 float32, t written, rank 16: 105 us, 3.9 TB/s, rank 64: 184 us — there the float32 pipe has 56 us of it), by the chain of loads
+// through both products with few (1024 x 512 x 512 float32, rank 16: 7.4 us).
 template <int TY, int RB, int MB, bool WT>
 __global__ void __launch_bounds__(256)
 adapter_rows_kernel(Adapt p) {
@@ -495,7 +495,7 @@ adapter_rows_kernel(Adapt p) {
 }
 
 // (adapters, rank, k) -> (adapters, k, rank) and (adapters, n, rank) -> (adapters, rank, n): blockIdx.x walks the 32 x 32 tiles of both.  A launch's
-// latency: 4.8 us for four adapters of 512 x 256, rank 16.
+// latency: 4.2 us for four adapters of 512 x 256, rank 16.
 template <typename T>
 __global__ void __launch_bounds__(256)
 adapter_transpose_kernel(int rank, int k, int n, const T* __restrict__ a, T* __restrict__ at, const T* __restrict__ b, T* __restrict__ bt) {
@@ -624,7 +624,7 @@ __device__ __forceinline__ void adapter_wgrad_finish(const AdaptGrad& p, float* 
 // Workgroup = (chunk of one adapter's rows) x (16 CW channels of x, then of dy) x (16 RB rank indices); its four waves take every fourth
 // group of four rows, 16 x 16 x 4 float32 products of T (t or u: rank) with X (CW channels a lane), UR groups in flight while UR are
 // multiplied, and add their tiles in wave order through LDS.  Bound by the loads' latency with few rows (512 x 512 x 512, rank 16, four
-// adapters: 6.4 us), by the memory and the float32 pipe together with many (65536 x 512 x 512, rank 16: 53 us of 268 MB, 5 TB/s).
+// adapters: 6.4 us), by the memory and the float32 pipe together with many (65536 x 512 x 512, rank 16: 63 us of 268 MB, 4.3 TB/s).
 // With at most one chunk an adapter (direct) the workgroups are the adapters' and write dA and dB themselves.
 template <int TY, bool KEPT, int RB, int CW>
 __device__ __forceinline__ void adapter_wgrad_tile(const AdaptGrad& p, float* lds, float* part, int4 chunk, int ad, bool isA, int c0, int r0) {
@@ -700,7 +700,7 @@ __device__ __forceinline__ void adapter_wgrad_tile(const AdaptGrad& p, float* ld
 // pieces that add up to it (rows8.hip's cut), so products are exact and only the float32 additions round — at a third of sixteen times the
 // float32 rate.  A lane's 8 contraction elements are 8 rows; it holds 8 channels of each and turns the 8 x 8 block over in its registers.
 // One batch in flight a wave and many waves: 65536 rows, kept x of 512, dy of 256, rank 16: 18 us of 76 MB, 4.2 TB/s; 131072 x 512 x 512,
-// rank 64: 145 us, the loads of the few workgroups that fit (147 registers a lane).
+// rank 64: 119 us, the loads of the few workgroups that fit (147 registers a lane).
 template <bool KEPT, int RB>
 __device__ __forceinline__ void adapter_wgrad_tile_bf16(const AdaptGrad& p, float* lds, float* part, int4 chunk, int ad, bool isA, int c0, int r0) {
     constexpr int CW = 8, STEP = 4 * 32;
@@ -826,7 +826,7 @@ adapter_wgrad_kernel(AdaptGrad p) {
     }
 }
 
-// dA, dB of an adapter = s times the sum of its chunks' partials, in chunk order (zero without rows): 4.7 us for four adapters of 32 chunks
+// dA, dB of an adapter = s times the sum of its chunks' partials, in chunk order (zero without rows): 4.3 us for four adapters of 32 chunks
 template <typename T>
 __global__ void __launch_bounds__(256)
 adapter_wgrad_reduce_kernel(AdaptGrad p) {

@@ -48,7 +48,7 @@ struct R8Walk {
 
 // Four lanes hold a block, 8 channels each; the block's maximum by two quad permutations.  One read of X, one write of the codes: bound
 // by memory.  A value's smallest magnitude is raised to the smallest code before the conversion (zeros keep zero); values that are not
-// finite are looked for once a wave.  65536 x 128 float32: 10 us (4.2 TB/s); 100003 x 196 bfloat16: 17 us (3.6 TB/s).
+// finite are looked for once a wave.  65536 x 128 float32: 9 us (4.7 TB/s); 100003 x 196 bfloat16: 17 us (3.6 TB/s).
 template <int TY>
 __global__ void __launch_bounds__(256)
 rows8_pack_kernel(int m, int lde, int c, int groups, const typename Elem<TY>::T* __restrict__ x, long long ldx, unsigned char* __restrict__ codes, int ldc,
@@ -112,7 +112,7 @@ __device__ __forceinline__ void r8_decode4(unsigned w, float scale, float (&v)[4
     v[0] = lo[0] * scale; v[1] = lo[1] * scale; v[2] = hi[0] * scale; v[3] = hi[1] * scale;
 }
 
-// One read of the codes, one write of the values: bound by memory.  65536 x 128 float32: 10 us (4.2 TB/s); 100003 x 196 bfloat16: 12 us (5 TB/s).
+// One read of the codes, one write of the values: bound by memory.  65536 x 128 float32: 10.6 us (4 TB/s); 100003 x 196 bfloat16: 12 us (5 TB/s).
 template <int TY>
 __global__ void __launch_bounds__(256)
 rows8_restore_kernel(int m, int lde, int c, int groups, const unsigned char* __restrict__ codes, int ldc, const unsigned char* __restrict__ exps,
@@ -146,7 +146,7 @@ rows8_restore_kernel(int m, int lde, int c, int groups, const unsigned char* __r
 
 // out = (the kept value > 0) ? dy : 0 — the gradient through a ReLU whose output was kept.  A ReLU's output is never negative, so the code of
 // values that are not finite stands for +infinity there and counts as positive.  out may be dy.  Four channels a lane, 9 bytes
-// moved an element: bound by memory.  65536 x 128: 12 us, 131072 x 512: 113 us (5.3 TB/s); 512 x 512: 2.4 us.
+// moved an element: bound by memory.  65536 x 128: 12 us (6.2 TB/s), 131072 x 512: 115 us (5.2 TB/s); 512 x 512: 2.6 us.
 __global__ void __launch_bounds__(256)
 rows8_relu_mask_kernel(int m, int c, int groups, const float* dy, long long ldd, const unsigned char* __restrict__ codes, int ldc, float* out, long long ldo) {
     const long long step = gridDim.x * 256ll, rows = step / groups;
@@ -185,10 +185,11 @@ rows8_relu_mask_kernel(int m, int c, int groups, const float* dy, long long ldd,
 // the other multiplies its own (48 matrix instructions of 32 x 32 x 16 a wave) and asks for its next rows between them; their sums are
 // added through LDS at the end, so a CU writes one partial tile.  The splits' partials are added in split order by the second kernel (no
 // float atomics: the same bits every time).
-// Measured (float32 / bfloat16 gradients, both kernels): 65536 x 256 x 256 39 / 28 us, 131072 x 512 x 512 212 / 97 us — 1.0 and 0.7
-// PFLOP/s on the bf16 pipe, where a library product of 8192^3 reaches 1.2; 512 x 512 x 512 9 / 7 us.  No one unit bounds it: of the
-// large bfloat16 case's 97 us staging and LDS reads alone take 70, the products alone 57 and the loads alone 56; what is lost is their
-// overlap.  (Two steps between barriers: 2 % less; a tile of 128 x 256: registers spill.)
+// Measured (float32 | bfloat16 gradients, both kernels, alone and on inputs that change from call to call): 65536 x 256 x 256 41 | 28 us, 131072 x
+// 512 x 512 249 | 127 us; calls one behind the other 37 us for the first and 108 for the last (93 on the same inputs again, which the caches then
+// hold in part) — 0.7 and 0.63 PFLOP/s on the bf16 pipe, where a library product of 8192^3 reaches 1.4; 512 x 512 x 512 9.7 | 7.5 us.  No one unit
+// bounds it: copies of the kernel with only the staging and LDS reads, only the products or only the loads took 70, 57 and 56 us of the 97 that
+// the whole took then on the same inputs; what is lost is their overlap.  (Two steps between barriers: 2 % less; a tile of 128 x 256: registers spill.)
 constexpr int W8_SLAB = 8192;          // elements of one operand piece of a step: 64 rows x 128 columns or 128 x 64
 
 struct Wgrad8 {
@@ -561,9 +562,9 @@ rows8_wgrad_reduce_kernel(int n, int k, int splits_w, int splits_b, const float*
     }
 }
 
-// The tile and the number of splits (up to one workgroup a CU) by the time they take: about 1 us a step of a workgroup (1.05 in float32, 0.6 in
-// bfloat16, at either tile), 3.6 us more for the larger tile's longer start and end, and for splits 2.5 us and 0.9 us a MB of partials,
-// written and read again.  What that decides, both sides measured in float32: 1024 x 512 x 512, 64 x 64, 1 | 4 splits: 13.3 | 14.0 us;
+// The tile and the number of splits (up to one workgroup a CU) by the time they take: 1 us a step of a workgroup for every type (measured 1.05 in
+// float32, 0.6 in bfloat16, at either tile: in bfloat16 the rule counts steps too dear and splits early), 3.6 us more for the larger tile's
+// longer start and end, and for splits 2.5 us and 0.9 us a MB of partials, written and read again.  What that decides, both sides measured in float32: 1024 x 512 x 512, 64 x 64, 1 | 4 splits: 13.3 | 14.0 us;
 // 2048 rows: 21.5 | 16.4; 4096 x 1024 x 1024, 64 x 64 and 1 split | 128 x 128 and 4: 41.5 | 42.5 (bfloat16 26.5 | 33.3), 8192 rows: 76 | 64; 16384 x
 // 512 x 512, 64 x 64 and 4 | 128 x 128 and 16: 47.7 | 41.1; 65536 x 256 x 256, 16 | 64: 47.8 | 40.7.
 struct Wgrad8Plan { int tile, splits; };

@@ -112,7 +112,8 @@ class Rows8:
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, exps: torch.Tensor) -> "Rows8":
-        """from codes (rows, channels) and exps (rows, ceil(channels / 32)), e.g. read from a file"""
+        """from codes (rows, channels) and exps (rows, ceil(channels / 32)), e.g. read from a file.  They are taken as they are: scale bytes as
+        checkpoint_rows writes them are 27 .. 247 (0 and 255 are no scales)"""
         if codes.dtype != _u8 or codes.dim() != 2 or exps.dtype != _u8 or exps.dim() != 2:
             raise TypeError("codes and exps must be 2-D uint8 tensors")
         m, c = codes.shape
@@ -200,7 +201,7 @@ def relu_mask8(dy: torch.Tensor, y8: Rows8, out: Optional[torch.Tensor] = None) 
 def linear_wgrad8(dy: torch.Tensor, x8: Rows8, want_bias: bool = True, out: Optional[torch.Tensor] = None,
                   col0: int = 0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(dw (N, K) = dy^T x, dbias (N) or None) in float32, dy (M, N) float32 / bfloat16 / float16, x (M, K) kept: ops.rows.linear_wgrad
-    with the input as `checkpoint_rows` left it.  out / col0: write the block into columns col0 .. of an (N, >= col0 + K) tensor."""
+    with the input as `checkpoint_rows` left it.  Rows of dy are at most 2^22 elements apart.  out / col0: write the block into columns col0 .. of an (N, >= col0 + K) tensor."""
     m, n, pdy, ldd = _matrix(dy, "dy")
     m8, k, pc, ld, pe, mp = _kept(x8, "x8")
     if m8 != m:
