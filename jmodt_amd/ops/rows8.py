@@ -201,7 +201,8 @@ def relu_mask8(dy: torch.Tensor, y8: Rows8, out: Optional[torch.Tensor] = None) 
 def linear_wgrad8(dy: torch.Tensor, x8: Rows8, want_bias: bool = True, out: Optional[torch.Tensor] = None,
                   col0: int = 0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(dw (N, K) = dy^T x, dbias (N) or None) in float32, dy (M, N) float32 / bfloat16 / float16, x (M, K) kept: ops.rows.linear_wgrad
-    with the input as `checkpoint_rows` left it.  Rows of dy are at most 2^22 elements apart.  out / col0: write the block into columns col0 .. of an (N, >= col0 + K) tensor."""
+    with the input as `checkpoint_rows` left it.  Rows of dy are at most 2^22 elements apart.  out / col0: write the block
+    into columns col0 .. of an (N, >= col0 + K) tensor."""
     m, n, pdy, ldd = _matrix(dy, "dy")
     m8, k, pc, ld, pe, mp = _kept(x8, "x8")
     if m8 != m:
